@@ -48,6 +48,35 @@ class Dispatch(C.Structure):
                 ("bitlinear_row_worker", _vp), ("ssm_inner", _vp), ("name", C.c_char_p)]
 
 
+_i64 = C.c_int64
+F32, BF16, F16 = 0, 1, 2
+
+
+class Conv(C.Structure):
+    """bm_hip_conv_t (include/bm_hip.h)."""
+    _fields_ = [("type", _i), ("channels", _i), ("width", _i), ("silu", _i), ("n_seqs", _i),
+                ("n_tokens", _i), ("seq_start", _vp), ("slots", _vp), ("fresh", _vp), ("x", _vp),
+                ("x_stride", _i64), ("w", _vp), ("bias", _vp), ("state", _vp),
+                ("state_stride", _i64), ("n_slots", _i), ("y", _vp), ("y_stride", _i64)]
+
+
+class Ssm(C.Structure):
+    """bm_hip_ssm_t (include/bm_hip.h)."""
+    _fields_ = [("type", _i), ("n_heads", _i), ("head_dim", _i), ("n_groups", _i), ("d_state", _i),
+                ("dt_softplus", _i), ("n_seqs", _i), ("n_tokens", _i), ("seq_start", _vp),
+                ("slots", _vp), ("fresh", _vp), ("x", _vp), ("B", _vp), ("C", _vp), ("dt", _vp),
+                ("z", _vp), ("x_stride", _i64), ("B_stride", _i64), ("C_stride", _i64),
+                ("dt_stride", _i64), ("z_stride", _i64), ("A", _vp), ("dt_bias", _vp), ("D", _vp),
+                ("state", _vp), ("state_stride", _i64), ("n_slots", _i), ("y", _vp),
+                ("y_stride", _i64)]
+
+
+class Slots(C.Structure):
+    """bm_hip_slots_t (include/bm_hip.h)."""
+    _fields_ = [("base", _vp), ("n_slots", _i), ("n_layers", _i), ("slot_bytes", _i64),
+                ("slot_stride", _i64), ("layer_stride", _i64)]
+
+
 # name -> (restype, argtypes); every symbol of include/bm_hip.h
 SIGNATURES = {
     "bm_hip_init": (C.c_bool, []),
@@ -92,6 +121,14 @@ SIGNATURES = {
     "bm_hip_noalloc_scratch_bytes": (_sz, []),
     "bm_hip_i8_act_bytes": (_sz, [_i, _i]),
     "bm_hip_ternary_gemm_i32_dev": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "bm_hip_conv_dev": (_i, [C.POINTER(Conv), _vp]),
+    "bm_hip_conv_step_dev": (_i, [C.POINTER(Conv), _vp]),
+    "bm_hip_ssm_workspace_bytes": (_sz, [C.POINTER(Ssm)]),
+    "bm_hip_ssm_dev": (_i, [C.POINTER(Ssm), _vp, _vp]),
+    "bm_hip_ssm_step_dev": (_i, [C.POINTER(Ssm), _vp]),
+    "bm_hip_slots_copy_dev": (_i, [C.POINTER(Slots), _i, _vp, _vp, _i, _vp]),
+    "bm_hip_slots_compact_workspace_bytes": (_sz, [_i]),
+    "bm_hip_slots_compact_dev": (_i, [C.POINTER(Slots), _i, _vp, _vp, _i, _vp, _vp, _vp]),
     "bm_hip_model_load": (_vp, [_vp, _sz]),
     "bm_hip_model_free": (None, [_vp]),
     "bm_hip_model_config": (_i, [_vp, _i]),

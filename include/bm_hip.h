@@ -331,6 +331,135 @@ int bm_hip_ternary_gemm_i32_dev(const int8_t *xq,
                                 void *stream);
 
 /* ------------------------------------------------------------------ */
+/* Batched recurrence on device buffers (asynchronous on `stream`): the */
+/* short causal convolution and the selective scan between in_proj and  */
+/* out_proj, for many sequences at once, and the slots that hold their  */
+/* state.  The mathematics of scalar_ssm_inner (src/kernel.c:34-70) and */
+/* ssm_batch_worker (src/block.c:127-160) with d_state values per       */
+/* channel and B, C shared by groups of heads; n_groups = n_heads and   */
+/* d_state = 1 are the reference's block.  Sums run in another order    */
+/* than the scalar kernels': results agree to fp32 rounding, they are   */
+/* not the reference's bits (the device-resident model below keeps      */
+/* those).                                                              */
+/*                                                                      */
+/* Common to the calls:                                                 */
+/* - Tensors of the descriptor's `type` are read and written at any     */
+/*   row stride (in elements) and any element alignment; everything is  */
+/*   computed in fp32 or more, y is rounded once.                       */
+/* - Prompts are joined rows: sequence b has rows seq_start[b] ..       */
+/*   seq_start[b + 1] - 1 (device, n_seqs + 1 ascending entries;        */
+/*   NULL for one sequence of n_tokens rows).  Entries are clamped to   */
+/*   0..n_tokens.  Rows that belong to no sequence are not touched.     */
+/* - Single tokens (_step): row b is the next token of sequence b;      */
+/*   seq_start, fresh and n_tokens are not read.                        */
+/* - The state of sequence b is slot slots[b] of the pool (device;      */
+/*   NULL: slot b), carried from call to call: read, and replaced by    */
+/*   the state after the sequence's last token.  A sequence whose entry */
+/*   is outside 0..n_slots-1, or that an earlier sequence of the call   */
+/*   also names, is padding: its rows of y and every slot stay as they  */
+/*   are.  fresh[b] != 0 (device, nullable) starts sequence b from      */
+/*   zeros whatever its slot holds.  state = NULL starts every sequence */
+/*   from zeros and keeps nothing (slots and fresh are not read).       */
+/* - y must not overlap the inputs or the pool; the step calls may      */
+/*   write y over x itself (same address and stride).                   */
+/* - Calls allocate nothing and may be captured into a graph; a replay  */
+/*   reads seq_start, slots and fresh as they are then.  Calls on       */
+/*   different streams need workspaces and slots of their own.          */
+/* - 0, -2 for arguments that do not fit (nothing is launched), -1 for  */
+/*   a HIP error; the reason is in bm_hip_last_error().                 */
+/* ------------------------------------------------------------------ */
+enum { BM_HIP_F32 = 0, BM_HIP_BF16 = 1, BM_HIP_F16 = 2 };
+
+/* y[t][c] = act(bias[c] + sum_k w[k][c] * x[t - (width - 1) + k][c]), per
+ * sequence; rows before its first token are the slot's rows. */
+typedef struct {
+    int type;                 /* of x and y */
+    int channels, width;      /* width 2..4 taps */
+    int silu;                 /* act(v) = v / (1 + exp(-v)), else v */
+    int n_seqs, n_tokens;
+    const int32_t *seq_start; /* device [n_seqs + 1], or NULL */
+    const int32_t *slots;     /* device [n_seqs], or NULL */
+    const uint8_t *fresh;     /* device [n_seqs], or NULL */
+    const void *x;
+    int64_t x_stride;
+    const float *w;           /* [width][channels], the last row is the token's own tap */
+    const float *bias;        /* [channels], or NULL */
+    float *state;             /* slot i at state + i * state_stride: [width - 1][channels], oldest row first */
+    int64_t state_stride;
+    int n_slots;
+    void *y;
+    int64_t y_stride;
+} bm_hip_conv_t;
+
+int bm_hip_conv_dev(const bm_hip_conv_t *op, void *stream);
+int bm_hip_conv_step_dev(const bm_hip_conv_t *op, void *stream);
+
+/* Per head h of group g = h / (n_heads / n_groups), with d = dt[t][h] +
+ * dt_bias[h], taken through log(1 + exp(d)) if dt_softplus, and a =
+ * exp(A[h] * d):
+ *   S[p][n] = a * S[p][n] + d * x[t][h][p] * B[t][g][n]
+ *   y[t][h][p] = (sum_n C[t][g][n] * S[p][n] + D[h][p] * x[t][h][p])
+ *                * z[t][h][p] / (1 + exp(-z[t][h][p])) */
+typedef struct {
+    int type;                      /* of x, B, C, dt, z, y */
+    int n_heads, head_dim;         /* x, z, y rows: [n_heads][head_dim] */
+    int n_groups, d_state;         /* B, C rows: [n_groups][d_state]; n_groups divides n_heads, d_state <= 256 */
+    int dt_softplus;
+    int n_seqs, n_tokens;
+    const int32_t *seq_start;      /* device [n_seqs + 1], or NULL */
+    const int32_t *slots;          /* device [n_seqs], or NULL */
+    const uint8_t *fresh;          /* device [n_seqs], or NULL */
+    const void *x, *B, *C, *dt, *z; /* z: NULL for no gate */
+    int64_t x_stride, B_stride, C_stride, dt_stride, z_stride;
+    const float *A;                /* [n_heads]; at most 0 for states that stay bounded */
+    const float *dt_bias;          /* [n_heads], or NULL */
+    const float *D;                /* [n_heads][head_dim], or NULL */
+    float *state;                  /* slot i at state + i * state_stride: [n_heads][head_dim][d_state] */
+    int64_t state_stride;
+    int n_slots;
+    void *y;
+    int64_t y_stride;
+} bm_hip_ssm_t;
+
+/* Prompts.  workspace: bm_hip_ssm_workspace_bytes(op) bytes of device
+ * memory on 256 bytes with any contents (NULL where that is 0; it depends
+ * on the sizes of op alone, not on the pointers). */
+size_t bm_hip_ssm_workspace_bytes(const bm_hip_ssm_t *op);
+int bm_hip_ssm_dev(const bm_hip_ssm_t *op, void *workspace, void *stream);
+/* One token of each sequence. */
+int bm_hip_ssm_step_dev(const bm_hip_ssm_t *op, void *stream);
+
+/* A pool of slots: slot i of layer l is slot_bytes bytes at base +
+ * l * layer_stride + i * slot_stride (strides in bytes). */
+typedef struct {
+    void *base;
+    int n_slots, n_layers;
+    int64_t slot_bytes, slot_stride, layer_stride;
+} bm_hip_slots_t;
+
+/* Slot dst[i] takes over slot src[i] of every layer of every pool, for all
+ * pairs at once (device lists): each pair reads what stood there before the
+ * call, so lists may fork (one src, many dst), swap, rotate or reorder.
+ * src[i] = -1 clears the slot to zero bytes.  Pairs with another src or a
+ * dst outside the pool do nothing; of several pairs with one dst the first
+ * such pair counts.  At most 1024 pairs and 8 pools (of equal n_slots). */
+int bm_hip_slots_copy_dev(const bm_hip_slots_t *pools, int n_pools,
+                          const int32_t *src, const int32_t *dst, int n, void *stream);
+
+/* Moves the slots that a table of n entries (device) names to the front:
+ * with `live` different slots named, those below `live` stay and the others
+ * go, in ascending order, to the free slots below it.  new_slots (may be
+ * slots itself) gets the table after the moves; entries outside the pool
+ * (ended sequences) are copied as they are.  Freed slots keep their bytes.
+ * n_live (device, nullable) gets `live`.  At most 65536 slots and 8 pools
+ * (of equal n_slots).  workspace: bm_hip_slots_compact_workspace_bytes
+ * bytes of device memory on 16 bytes with any contents. */
+size_t bm_hip_slots_compact_workspace_bytes(int n_slots);
+int bm_hip_slots_compact_dev(const bm_hip_slots_t *pools, int n_pools,
+                             const int32_t *slots, int32_t *new_slots, int n,
+                             int32_t *n_live, void *workspace, void *stream);
+
+/* ------------------------------------------------------------------ */
 /* Device-resident model: the reference's model API (src/bitmamba.h:    */
 /* 282-294, src/model.c:477-1314) with weights, activations and the    */
 /* recurrent state in HBM.  Greedy or sampled next tokens              */

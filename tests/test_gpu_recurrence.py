@@ -1,0 +1,351 @@
+"""The batched convolution and selective scan (bm_hip_conv_dev,
+bm_hip_conv_step_dev, bm_hip_ssm_dev, bm_hip_ssm_step_dev) against the same
+in 64 bits, with the bounds of tests/recurrence.py."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import native
+from native import bh
+from recurrence import (MARK, ConvCase, SsmCase, at, check_rows, close, conv_ref, f64, gpu, silu,
+                        softplus)
+
+pytestmark = pytest.mark.gpu
+ALL = ["f32", "bf16", "f16"]
+
+
+def note(msg):
+    print("[case] " + msg, flush=True)
+
+
+# ---------------------------------------------------------------------------
+# convolution
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("type_name", ALL)
+@pytest.mark.parametrize("width", [2, 3, 4])
+@pytest.mark.parametrize("channels", [1, 7, 64, 1030])
+def test_conv_prompts(hip, type_name, width, channels):
+    """Lengths around the unit of 32 rows and shorter than the window, rows
+    before the first and behind the last sequence, odd strides."""
+    for lens, pads in (([0, 1, 2, 3, 31, 32, 33, 64, 65, 5], dict(front=3, tail=2)),
+                       ([100], dict(lead=3, row_pad=2)), ([1, 1, 1], dict(lead=8, slot_pad=5))):
+        c = ConvCase(type_name, channels, width, lens, act=channels != 7, bias=width != 3,
+                     seed=channels + width, **pads)
+        note("conv %s width=%d channels=%d lens=%s" % (type_name, width, channels, lens))
+        c.check(hip, "conv")
+
+
+@pytest.mark.parametrize("type_name", ALL)
+@pytest.mark.parametrize("channels", [1, 9, 512, 2056])
+def test_conv_tokens(hip, type_name, channels):
+    for n, width in ((1, 4), (5, 2), (70, 3)):
+        note("conv_step %s channels=%d n=%d" % (type_name, channels, n))
+        ConvCase(type_name, channels, width, [1] * n, step=True, seed=n, lead=channels % 3,
+                 slot_pad=channels % 5).check(hip, "conv_step")
+
+
+def test_conv_token_over_its_input(hip):
+    c = ConvCase("f32", 300, 4, [1] * 6, step=True)
+    rows, tols, pool = c.want()
+    d = c.descriptor()
+    d.y, d.y_stride = d.x, d.x_stride
+    torch.cuda.synchronize()
+    bh.check(hip.bm_hip_conv_step_dev(C.byref(d), None))
+    torch.cuda.synchronize()
+    check_rows(c.buf, c.x, rows, tols, "f32", (300,), "in place")
+    assert np.array_equal(c.pool(), pool)
+
+
+# ---------------------------------------------------------------------------
+# what both have in common: slots, padding, fresh sequences, bad row starts
+# ---------------------------------------------------------------------------
+def make(kind, lens, step=False, **k):
+    if kind == "conv":
+        return ConvCase("f32", 130, 4, lens, step=step, **k)
+    H, P, G, N = {"scan1": (6, 10, 6, 1), "scan5": (4, 10, 2, 5), "scan24": (4, 40, 2, 24)}[kind]
+    return SsmCase("f32", H, P, G, N, lens, step=step, **k)
+
+
+KINDS = ["conv", "scan1", "scan5", "scan24"]
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("kind", KINDS)
+def test_padding_and_repeated_slots(hip, kind, step):
+    """Entries outside the pool and repeated ones: rows and slots untouched;
+    the first that names a slot has it, also 64 and more entries earlier."""
+    for slots in ([2, -1, 0, 9, 2, 1, 0, 1 << 30, -(1 << 31)], [-1] * 4, [3],
+                  [5] + [-7] * 70 + [5, 4, 4]):
+        lens = [1] * len(slots) if step else [3 + i % 5 for i in range(len(slots))]
+        c = make(kind, lens, step, slots=slots, seed=len(slots), spare=9 - len(slots)
+                 if len(slots) < 9 else 0)
+        note("%s step=%s slots=%s" % (kind, step, slots[:10]))
+        c.check(hip, "padding")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_slots_in_order_and_no_pool(hip, kind):
+    make(kind, [4, 40, 0, 7], slots=None, spare=0).check(hip, "slot b")
+    make(kind, [4, 40, 0, 7], slots=[1, 1, 2, 0], pool=False).check(hip, "no pool")
+    make(kind, [1, 1, 1], True, slots=None, spare=1).check(hip, "step, slot b")
+    make(kind, [1, 1, 1], True, pool=False).check(hip, "step, no pool")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_fresh(hip, kind):
+    """Fresh sequences start from zeros, an empty one's slot becomes zero."""
+    c = make(kind, [5, 0, 0, 2, 70], seed=3)
+    c.fresh = [1, 1, 0, 0, 1]
+    c.check(hip, "fresh")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_one_sequence_without_starts(hip, kind):
+    c = make(kind, [150], seed=4)
+    d = c.descriptor()
+    rows, tols, pool = c.want()[:3]
+    d.seq_start = None
+    w = c.workspace(hip, d) if kind != "conv" else None
+    torch.cuda.synchronize()
+    if kind == "conv":
+        bh.check(hip.bm_hip_conv_dev(C.byref(d), None))
+    else:
+        bh.check(hip.bm_hip_ssm_dev(C.byref(d), w, None))
+    torch.cuda.synchronize()
+    shape = (130,) if kind == "conv" else (c.H, c.P)
+    check_rows(c.ybuf, c.y, rows, tols, "f32", shape, "one sequence")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_row_starts_out_of_range(hip, kind):
+    """Starts below 0, above n_tokens and descending are clamped: nothing
+    outside the rows is read or written, and no slot that is not named."""
+    for starts in ([-5, 10, 20, 1 << 30], [0, 30, 10, 20], [1 << 30, 3, 3, -1]):
+        c = make(kind, [10, 10, 10], seed=5)
+        c.starts = starts
+        rest = [k for k in range(c.n_slots) if k not in c.slots]
+        before = c.pool_buf.clone()
+        note("%s starts=%s" % (kind, starts))
+        c.run(hip)
+        assert torch.equal(before[rest], c.pool_buf[rest])
+        if starts[0] == -5:  # still ascending: ordinary rows
+            c = make(kind, [10, 10, 10], seed=5)
+            c.starts = starts
+            c.check(hip, "clamped")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_split_prompt_is_the_whole(hip, kind):
+    """A prompt in one call, in two, and token by token: the same results
+    within their bounds, the state carried by the slot."""
+    n = 75
+    whole, parts = make(kind, [n], seed=6), make(kind, [n], seed=6)
+    rows, tols, pool = whole.want()[:3]
+    whole.check(hip, "whole")
+    d = parts.descriptor()
+    d.seq_start, d.n_seqs = None, 1
+    es = 4
+    f_prompt = hip.bm_hip_conv_dev if kind == "conv" else hip.bm_hip_ssm_dev
+    f_step = hip.bm_hip_conv_step_dev if kind == "conv" else hip.bm_hip_ssm_step_dev
+    fields = ["x", "y"] if kind == "conv" else ["x", "y", "z", "B", "C", "dt"]
+    base = {f: getattr(d, f) for f in fields}
+    torch.cuda.synchronize()
+    at_row, work = 0, []
+    for take in (40, 1, 0, 30, 1, 1, 1, 1):
+        for f in fields:
+            stride = getattr(d, f + "_stride")
+            setattr(d, f, base[f] + at_row * stride * es)
+        d.n_tokens = take
+        if take == 1:
+            bh.check(f_step(C.byref(d), None))
+        elif kind == "conv":
+            bh.check(f_prompt(C.byref(d), None))
+        else:
+            work.append(parts.workspace(hip, d))
+            torch.cuda.synchronize()
+            bh.check(f_prompt(C.byref(d), work[-1], None))
+        at_row += take
+    assert at_row == n
+    torch.cuda.synchronize()
+    shape = (130,) if kind == "conv" else (parts.H, parts.P)
+    check_rows(parts.ybuf, parts.y, rows, tols, "f32", shape, "parts")
+
+
+# ---------------------------------------------------------------------------
+# scan
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("type_name", ALL)
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 8])
+def test_scan_few_values(hip, type_name, N):
+    for H, P, G in ((3, 64, 3), (8, 5, 2), (1, 1, 1), (2, 300, 1)):
+        note("scan %s H=%d P=%d G=%d N=%d" % (type_name, H, P, G, N))
+        SsmCase(type_name, H, P, G, N, [0, 1, 2, 31, 33, 64, 100, 17], seed=N, front=2, tail=1,
+                lead=P % 4, gate=N != 3, skip=N != 4, bias=N != 5).check(hip, "scan")
+
+
+@pytest.mark.parametrize("type_name", ALL)
+@pytest.mark.parametrize("N", [9, 16, 20, 31, 32, 33, 64, 100, 128, 129, 256])
+def test_scan_many_values(hip, type_name, N):
+    for H, P, G in ((4, 64, 1), (6, 7, 3), (1, 33, 1), (2, 130, 2)):
+        note("scan %s H=%d P=%d G=%d N=%d" % (type_name, H, P, G, N))
+        SsmCase(type_name, H, P, G, N, [1, 0, 31, 32, 33, 65, 20], seed=N + P, front=1, tail=3,
+                lead=N % 4, gate=N != 16, skip=N != 20, bias=N != 33).check(hip, "scan")
+
+
+@pytest.mark.parametrize("type_name", ["f32", "bf16"])
+@pytest.mark.parametrize("N", [1, 6, 16, 128])
+@pytest.mark.parametrize("lens", [[1500], [700, 3, 1100]])
+def test_scan_long(hip, type_name, N, lens):
+    """Sequences long enough to be worked on in parts."""
+    note("scan %s N=%d lens=%s" % (type_name, N, lens))
+    SsmCase(type_name, 2, 32, 2 if N == 1 else 1, N, lens, seed=N).check(hip, "long")
+
+
+@pytest.mark.parametrize("N", [1, 24])
+def test_scan_steps_given(hip, N):
+    """Without softplus, and without bias: dt is the step itself."""
+    for bias in (True, False):
+        SsmCase("f32", 2, 20, 2, N, [50, 3], soft=False, bias=bias, rate=16.0).check(hip, "steps")
+
+
+@pytest.mark.parametrize("N", [1, 24])
+def test_scan_decays_that_vanish(hip, N):
+    """Steps so large that a state is forgotten within a token, and so small
+    that none is: softplus at both ends."""
+    c = SsmCase("f32", 4, 12, 4, N, [90, 40], seed=8, bias=False)
+    c.dt[:, 0] = 50.0
+    c.dt[:, 1] = -60.0
+    c.dt[::3, 2] = 25.0
+    c.A[0] = -16.0
+    c.check(hip, "decays")
+
+
+def run_y(c, hip):
+    c.run(hip)
+    return f64(c.y).copy(), c.pool().copy()
+
+
+@pytest.mark.parametrize("what", ["x", "B", "Cm", "dt", "z"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("N", [1, 5, 24, 128])
+def test_scan_later_tokens_do_not_reach_earlier_ones(hip, N, what, value):
+    """Infinities and NaN from one token on: earlier rows and other sequences
+    are bit for bit what they were."""
+    H, P = 2, 40
+    G = H if N == 1 else 1
+    lens = [37, 90, 20]
+    clean = SsmCase("f32", H, P, G, N, lens, seed=9)
+    y0, p0 = run_y(clean, hip)
+    for row in (37 + 13, 37 + 50):
+        c = SsmCase("f32", H, P, G, N, lens, seed=9)
+        t = getattr(c, what)
+        t[row] = value
+        if what in ("dt", "z", "x"):
+            t[row, -1] = 0.25
+        note("scan N=%d %s=%r from row %d" % (N, what, value, row))
+        y1, p1 = run_y(c, hip)
+        keep = [r for r in range(sum(lens)) if r < row or r >= 37 + 90]
+        assert np.array_equal(y0[keep], y1[keep])
+        for b in (0, 2):
+            assert np.array_equal(p0[c.slots[b]], p1[c.slots[b]])
+        if what == "z":
+            assert np.array_equal(p0, p1)
+        if np.isnan(value):
+            assert np.isnan(y1[row]).any()
+
+
+@pytest.mark.parametrize("N", [1, 24])
+def test_scan_infinite_values_come_through(hip, N):
+    """A single infinite x makes its channel infinite or NaN from its row on,
+    and leaves the others as they are."""
+    c = SsmCase("f32", 1, 40, 1, N, [70], seed=10, gate=False, skip=False)
+    rows, tols, pool, stol = c.want()
+    c.x[20, 7] = float("inf")
+    c.run(hip)
+    y = f64(c.y)
+    assert not np.isfinite(y[20:, 7]).any()
+    for t in range(70):
+        k = [p for p in range(40) if p != 7 or t < 20]
+        close(y[t][k], rows[t].reshape(-1)[k], tols[t].reshape(-1)[k], "f32", "row %d" % t)
+
+
+def test_scan_overflow_of_a_growing_state(hip):
+    """A > 0: the state grows past fp32 and becomes infinite, not wrong."""
+    for N in (1, 24):
+        c = SsmCase("f32", 2, 8, 2, N, [200], seed=11, gate=False, skip=False, bias=False)
+        c.A[:] = 3.0
+        c.A[1] = -1.0
+        c.dt[:] = 1.0
+        c.run(hip)
+        y, p = f64(c.y), c.pool()[c.slots[0]]
+        assert not np.isfinite(y[-1, :8]).any() and np.isfinite(y[:, 8:]).all()
+        assert not np.isfinite(p[0]).any() and np.isfinite(p[1]).all()
+
+
+# ---------------------------------------------------------------------------
+# single tokens
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("type_name", ALL)
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 7, 8, 16, 17, 32, 40, 64, 96, 128, 200, 256, 255])
+def test_scan_tokens(hip, type_name, N):
+    for H, P, G, n in ((3, 64, 3, 1), (8, 5, 2, 4), (2, 130, 1, 66)):
+        for slot_pad in (0, 1):
+            note("step %s H=%d P=%d G=%d N=%d n=%d" % (type_name, H, P, G, N, n))
+            SsmCase(type_name, H, P, G, N, [1] * n, step=True, seed=N, lead=N % 3,
+                    slot_pad=slot_pad, gate=N != 3, skip=N != 4, bias=N != 7).check(hip, "step")
+
+
+def test_scan_token_over_its_input(hip):
+    for what in ("x", "z"):
+        c = SsmCase("f32", 3, 70, 1, 12, [1] * 5, step=True)
+        rows, tols = c.want()[:2]
+        d = c.descriptor()
+        d.y, d.y_stride = getattr(d, what), d.x_stride
+        torch.cuda.synchronize()
+        rc = hip.bm_hip_ssm_step_dev(C.byref(d), None)
+        if what == "z":
+            assert rc == -2 and "overlaps z" in bh.last_error()
+            continue
+        torch.cuda.synchronize()
+        for t in rows:
+            close(f64(c.x)[t].reshape(3, 70), rows[t], tols[t], "f32", "in place")
+
+
+def test_offsets_past_32_bits(hip):
+    """The last slot of a pool of more than 2^32 floats, rows of a buffer of
+    more than 2^32 values: prompts and single tokens."""
+    H, P, N, far = 2, 16, 16, 3
+    stride = (1 << 31) + 64
+    pool = torch.empty(far * stride, dtype=torch.float32, device="cuda")
+    xs = (1 << 29) + 16
+    rows = torch.empty(9 * xs + 64, dtype=torch.float32, device="cuda")
+    for step in (False, True):
+        c = SsmCase("f32", H, P, 1, N, [1] * 9 if step else [9], step=step, slots=None, spare=0)
+        if step:
+            c.slots = [2] + [-1] * 8
+        else:
+            c.slots = [2]
+        c.n_slots = 3
+        state = torch.randn(H * P * N, device="cuda")
+        pool[2 * stride:2 * stride + H * P * N] = state
+        c.pool_buf = torch.zeros((3, H * P * N), device="cuda")
+        c.pool_buf[2] = state
+        want, tols, new, stol = c.want()
+        d = c.descriptor()
+        d.state, d.state_stride = at(pool), stride
+        wide = rows[:9 * xs].view(9, xs)
+        wide[:, :H * P] = c.x
+        d.x, d.x_stride = at(rows), xs
+        d.y, d.y_stride = at(rows) + 4 * H * P, xs
+        w = None if step else c.workspace(hip, d)
+        torch.cuda.synchronize()
+        bh.check(hip.bm_hip_ssm_step_dev(C.byref(d), None) if step
+                 else hip.bm_hip_ssm_dev(C.byref(d), w, None))
+        torch.cuda.synchronize()
+        got = f64(wide[:, H * P:2 * H * P])
+        for t in want:
+            close(got[t].reshape(H, P), want[t], tols[t], "f32", "row %d" % t)
+        close(f64(pool[2 * stride:2 * stride + H * P * N]).reshape(H, P, N), new[2], stol[2],
+              "f32", "state")
