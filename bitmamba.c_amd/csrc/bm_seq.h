@@ -29,6 +29,95 @@ __device__ __forceinline__ void store_f32(T* p, const float (&o)[N]) {
   *(Pack<T, N>*)p = k;
 }
 
+// Up to 32 rows of a tensor as a buffer resource: an offset at or past its
+// end reads zeros and writes nothing, so neither the last rows nor lanes
+// without a column (offset kNoColumn) need a branch around a load, which would
+// keep it from being issued with the others.  Row strides are below 2^24
+// elements (check_rows), so 32 rows end below kNoColumn, and kNoColumn plus
+// an offset within them does not wrap.
+constexpr uint32_t kNoColumn = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* p, int64_t row,
+                                                          int64_t stride, int rows) {
+  return rows_at((const T*)p + row * stride, (uint32_t)rows * (uint32_t)stride * sizeof(T));
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_row(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  constexpr int B = sizeof(T) * N;
+  static_assert(B == 2 || B == 4 || B == 8 || B == 16, "one load");
+  if constexpr (B == 2) {
+    return __builtin_bit_cast(Pack<T, N>, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+  } else if constexpr (B == 4) {
+    return __builtin_bit_cast(Pack<T, N>, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+  } else if constexpr (B == 8) {
+    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+    return __builtin_bit_cast(Pack<T, N>, v);
+  } else {
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+    return __builtin_bit_cast(Pack<T, N>, v);
+  }
+}
+// A value or four of them as the load leaves them, for loads that are issued
+// well ahead: as T they would be packed into pairs at once, which waits.
+template <typename T>
+__device__ __forceinline__ uint32_t load_raw(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+  else return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ float raw_f32(uint32_t v) {
+  if constexpr (sizeof(T) == 2) return (float)__builtin_bit_cast(T, (uint16_t)v);
+  else return __uint_as_float(v);
+}
+template <typename T>
+struct Raw4 {
+  uint32_t w[sizeof(T)];  // four values
+};
+template <typename T>
+__device__ __forceinline__ Raw4<T> load_raw4(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  Raw4<T> o;
+  if constexpr (sizeof(T) == 2) {
+    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+    o.w[0] = v[0];
+    o.w[1] = v[1];
+  } else {
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.w[i] = v[i];
+  }
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ float raw4_f32(const Raw4<T>& v, int i) {
+  if constexpr (sizeof(T) == 2)
+    return (float)__builtin_bit_cast(T, (uint16_t)(v.w[i >> 1] >> (16 * (i & 1))));
+  else
+    return __uint_as_float(v.w[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_row(__amdgpu_buffer_rsrc_t r, uint32_t off,
+                                          const float (&o)[N]) {
+  constexpr int B = sizeof(T) * N;
+  static_assert(B == 2 || B == 4 || B == 8 || B == 16, "one store");
+  Pack<T, N> k;
+#pragma unroll
+  for (int i = 0; i < N; ++i) k.v[i] = (T)o[i];
+  if constexpr (B == 2) {
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, k), r, off, 0, 0);
+  } else if constexpr (B == 4) {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, k), r, off, 0, 0);
+  } else if constexpr (B == 8) {
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, k), r, off, 0, 0);
+  } else {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, k), r, off, 0, 0);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // fp32 functions on the hardware's base-2 exponential (1 ulp): the argument's
 // product with log2(e) is carried in two parts, so that its rounding, which
@@ -44,13 +133,28 @@ __device__ __forceinline__ float exp_f32(float x) {
   return __builtin_fabsf(hi) < 256.0f ? r : e;
 }
 __device__ __forceinline__ float silu_f32(float x) {
-  // x rcp(1 + exp(-x)); -inf * 0 is 0 here, the limit
-  const float r = x * __builtin_amdgcn_rcpf(1.0f + exp_f32(-x));
-  return x < -126.0f ? -0.0f : r;
+  return x * __builtin_amdgcn_rcpf(1.0f + exp_f32(-x));
 }
-// log(1 + exp(x)) = max(x, 0) + log1p(exp(-|x|))
+// the same to 2^-20, for what is rounded to bf16
+__device__ __forceinline__ float silu_short(float x) {
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e));
+}
+// log(1 + exp(x)) = max(x, 0) + log(1 + e), e = exp(-|x|) <= 1, by
+// log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the series up to s^13
+// leaves less than s^15 / 15 < 2^-26 of it
 __device__ __forceinline__ float softplus_f32(float x) {
-  return fmaxf(x, 0.0f) + log1pf(expf(-__builtin_fabsf(x)));
+  const float e = exp_f32(-__builtin_fabsf(x)), q = 2.0f + e;
+  float r = __builtin_amdgcn_rcpf(q);
+  r = __builtin_fmaf(r, __builtin_fmaf(-q, r, 1.0f), r);
+  const float s = e * r, s2 = s * s;
+  float p = 1.0f / 13.0f;
+  p = __builtin_fmaf(p, s2, 1.0f / 11.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 9.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 7.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 5.0f);
+  p = __builtin_fmaf(p, s2, 1.0f / 3.0f);
+  p = __builtin_fmaf(p, s2, 1.0f);
+  return __builtin_fmaf(2.0f * s, p, fmaxf(x, 0.0f));
 }
 
 // ---------------------------------------------------------------------------

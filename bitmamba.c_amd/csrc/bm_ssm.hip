@@ -7,6 +7,7 @@
 //   y[p] = (sum_n C[n] S[p][n] + D[p] x[p]) z[p] / (1 + exp(-z[p]))
 //
 // State, sums and decays in fp32; y rounded once.
+#include "bm_dev.h"
 #include "bm_seq.h"
 
 namespace bm {
@@ -24,8 +25,11 @@ struct SsmArgs {
   int64_t ys;
 };
 
-__device__ __forceinline__ float step_of(const SsmArgs& a, float dt, int h) {
-  if (a.dt_bias) dt += a.dt_bias[h];
+__device__ __forceinline__ float bias_of(const SsmArgs& a, int h) {
+  return a.dt_bias ? a.dt_bias[h] : 0.0f;
+}
+__device__ __forceinline__ float step_of(const SsmArgs& a, float dt, float bias) {
+  dt += bias;
   return a.softplus ? softplus_f32(dt) : dt;
 }
 
@@ -56,7 +60,7 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs a) {
   const int slot = find_slot(a.q, b);
   if (slot == kNoSlot) return;
   const int g = h / (a.heads / a.groups);
-  const float d = step_of(a, (float)((const T*)a.dt)[(int64_t)b * a.dts + h], h);
+  const float d = step_of(a, (float)((const T*)a.dt)[(int64_t)b * a.dts + h], bias_of(a, h));
   const float decay = exp_f32(a.A[h] * d);
   float* st = slot >= 0 ? a.state + (int64_t)slot * a.ss + (int64_t)h * a.hd * a.n : nullptr;
   const T* Bp = (const T*)a.B + (int64_t)b * a.Bs + (int64_t)g * a.n;
@@ -144,17 +148,18 @@ static hipError_t launch_step_t(const SsmArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Prompts.  The rows of a sequence are cut into units of `len` rows.  Every
-// unit but a sequence's last is first run from a zero state for the state it
-// ends with and its whole decay (pass FULL = false); the second pass runs all
-// units, each from the state that its predecessors' results give,
-//   S = S decay_j + end_j over the units j before it,
-// and writes y.  Where no sequence can have two units there is one pass.
+// Prompts.  The rows of a sequence are cut into units of `len` rows, where a
+// sequence may have more than one in three launches:
+//   the first pass runs every unit but a sequence's last from a zero state,
+//   for the state it ends with and its whole decay;
+//   the join turns these into the state that each unit starts from,
+//     start_0 = the sequence's own, start_{j+1} = start_j decay_j + end_j;
+//   the second pass runs all units from there and writes y.
+// Otherwise the second pass alone runs.
 //
-// Workspace: per unit, `ends` (the state's layout is the kernel's) and
-// `decays` (one per head).  A sequence's last unit has no end of its own
-// there: its place holds a copy of the state that the sequence starts from,
-// since the slot is rewritten while other units still need it.
+// Workspace: per unit `ends` (laid out as the kernels hold a state) and
+// `decays` (one per head).  A sequence's last unit has no end of its own: the
+// first pass leaves the sequence's own state in its place.
 // ---------------------------------------------------------------------------
 struct ScanPlan {
   int len;         // rows per unit
@@ -181,6 +186,47 @@ __device__ __forceinline__ bool scan_unit(const SeqView& q, int index, int len, 
   w.slot = find_slot(q, w.u.b);
   w.keep = w.slot >= 0 && !(q.fresh && q.fresh[w.u.b]);
   return w.slot != kNoSlot;
+}
+
+// The join: a thread takes V neighbouring floats of a sequence's units in
+// turn, kAhead of them loaded before the first is used.  Where the floats'
+// head lies: (float / head_stride) % heads.
+template <int V>
+__global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64_t unit_floats,
+                                                   int head_stride, int heads) {
+  constexpr int kAhead = 8;
+  ScanUnit w;
+  if (!scan_unit(q, blockIdx.x, pl.len, w) || w.u.k != 0 || w.last == 0) return;
+  const int64_t at = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V;
+  if (at >= unit_floats) return;
+  float* e = pl.ends + (int64_t)blockIdx.x * unit_floats + at;
+  const float* dec = pl.decays + (int64_t)blockIdx.x * heads + at / head_stride % heads;
+  float S[V];
+  load_f32<float, V>(S, e + w.last * unit_floats);
+  for (int j0 = 0; j0 < w.last; j0 += kAhead) {
+    float v[kAhead][V], d[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = min(j0 + i, w.last - 1);
+      load_f32<float, V>(v[i], e + j * unit_floats);
+      d[i] = dec[(int64_t)j * heads];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (j0 + i >= w.last) break;
+      store_f32<float, V>(e + (j0 + i) * unit_floats, S);
+#pragma unroll
+      for (int k = 0; k < V; ++k) S[k] = __builtin_fmaf(S[k], d[i], v[i][k]);
+    }
+  }
+  store_f32<float, V>(e + w.last * unit_floats, S);
+}
+template <int V>
+static void launch_join(const SsmArgs& a, const ScanPlan& pl, int64_t unit_floats, int head_stride,
+                        hipStream_t s) {
+  hipLaunchKernelGGL((k_scan_join<V>),
+                     dim3((unsigned)pl.units, (unsigned)((unit_floats / V + 255) / 256)), dim3(256),
+                     0, s, a.q, pl, unit_floats, head_stride, a.heads);
 }
 
 // ---- up to 8 state values per channel -------------------------------------
@@ -240,37 +286,29 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int t
         for (int i = 0; i < VC; ++i) S[n][i] = 0.0f;
     }
   } else if (w.last > 0 && on) {
-    const float* e = pl.ends + (unit0 + w.last) * channels * a.n;
+    const float* e = pl.ends + (int64_t)blockIdx.x * channels * a.n;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
       if (n < a.n) load_f32<float, VC>(S[n], e + (int64_t)n * channels + c);
-    for (int j = 0; j < w.u.k; ++j) {
-      e = pl.ends + (unit0 + j) * channels * a.n;
-      const float dec = pl.decays[(unit0 + j) * a.heads + h];
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-        if (n < a.n) {
-          float v[VC];
-          load_f32<float, VC>(v, e + (int64_t)n * channels + c);
-#pragma unroll
-          for (int i = 0; i < VC; ++i) S[n][i] = __builtin_fmaf(S[n][i], dec, v[i]);
-        }
-    }
   }
 
   float D[VC], all = 1.0f;
 #pragma unroll
   for (int i = 0; i < VC; ++i) D[i] = FULL && on && a.D ? a.D[c + i] : 0.0f;
-  const T* xp = (const T*)a.x + c;
-  const T* zp = (const T*)a.z + c;
-  T* yp = (T*)a.y + c;
+  const uint32_t col = on ? (uint32_t)(c * sizeof(T)) : kNoColumn;
+  const uint32_t xs = (uint32_t)(a.xs * sizeof(T)), zs = (uint32_t)(a.zs * sizeof(T)),
+                 ys = (uint32_t)(a.ys * sizeof(T));
   for (int t = w.t0; t < w.t1; t += tile) {
     const int rows = min(tile, w.t1 - t);
+    const auto bx = rows_of<T>(a.x, t, a.xs, rows);
+    const auto bz = rows_of<T>(a.z, t, a.zs, FULL && a.z ? rows : 0);
+    const auto by = rows_of<T>(a.y, t, a.ys, rows);
     for (int i = lane; i < rows * nh; i += 64) {
       const int r = i / nh, hh = i - r * nh;
       const int64_t row = t + r;
       const int g = (h0 + hh) / per;
-      const float d = step_of(a, (float)((const T*)a.dt)[row * a.dts + h0 + hh], h0 + hh);
+      const float d = step_of(a, (float)((const T*)a.dt)[row * a.dts + h0 + hh],
+                              bias_of(a, h0 + hh));
       float* s = sh + (r * heads_max + hh) * EW;
       s[0] = exp_f32(a.A[h0 + hh] * d);
 #pragma unroll
@@ -283,13 +321,12 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int t
     }
     __syncthreads();
     for (int r0 = 0; r0 < rows; r0 += kSmallRows) {
-      float x[kSmallRows][VC], z[kSmallRows][VC];
+      Pack<T, VC> xr[kSmallRows], zr[kSmallRows];
 #pragma unroll
-      for (int r = 0; r < kSmallRows; ++r)
-        if (on && r0 + r < rows) {
-          load_f32<T, VC>(x[r], xp + (int64_t)(t + r0 + r) * a.xs);
-          if (FULL && a.z) load_f32<T, VC>(z[r], zp + (int64_t)(t + r0 + r) * a.zs);
-        }
+      for (int r = 0; r < kSmallRows; ++r) {
+        xr[r] = load_row<T, VC>(bx, col + (r0 + r) * xs);
+        if (FULL) zr[r] = load_row<T, VC>(bz, col + (r0 + r) * zs);
+      }
 #pragma unroll
       for (int r = 0; r < kSmallRows; ++r) {
         if (r0 + r >= rows) break;
@@ -297,14 +334,17 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int t
         const float4* s = (const float4*)(sh + ((r0 + r) * heads_max + (h - h0)) * EW);
 #pragma unroll
         for (int k = 0; k < EW / 4; ++k) *(float4*)(e + 4 * k) = s[k];
-        float y[VC];
+        float x[VC], y[VC];
 #pragma unroll
-        for (int i = 0; i < VC; ++i) y[i] = FULL ? D[i] * x[r][i] : 0.0f;
+        for (int i = 0; i < VC; ++i) {
+          x[i] = (float)xr[r].v[i];
+          y[i] = FULL ? D[i] * x[i] : 0.0f;
+        }
 #pragma unroll
         for (int n = 0; n < NS; ++n)
 #pragma unroll
           for (int i = 0; i < VC; ++i) {
-            S[n][i] = __builtin_fmaf(S[n][i], e[0], x[r][i] * e[1 + n]);
+            S[n][i] = __builtin_fmaf(S[n][i], e[0], x[i] * e[1 + n]);
             // a value beyond d_state stays zero even where the decay is infinite
             if (NS > 2) S[n][i] = n < a.n ? S[n][i] : 0.0f;
             if (FULL) y[i] = __builtin_fmaf(S[n][i], e[1 + NS + n], y[i]);
@@ -313,8 +353,8 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int t
         if (FULL) {
           if (a.z)
 #pragma unroll
-            for (int i = 0; i < VC; ++i) y[i] *= silu_f32(z[r][i]);
-          if (on) store_f32<T, VC>(yp + (int64_t)(t + r0 + r) * a.ys, y);
+            for (int i = 0; i < VC; ++i) y[i] *= silu_f32((float)zr[r].v[i]);
+          store_row<T, VC>(by, col + (r0 + r) * ys, y);
         }
       }
     }
@@ -347,9 +387,11 @@ static hipError_t launch_small(const SsmArgs& a, const ScanPlan& pl, hipStream_t
   const int row = heads_max * small_entry(NS) * 4;
   int tile = 32;
   while (tile * row > 32768) tile /= 2;
-  if (pl.split)
+  if (pl.split) {
     hipLaunchKernelGGL((k_scan_small<T, NS, VC, false>), dim3((unsigned)pl.units, by), dim3(64),
                        tile * row, s, a, pl, tile, heads_max);
+    launch_join<1>(a, pl, (int64_t)channels * a.n, a.hd, s);
+  }
   hipLaunchKernelGGL((k_scan_small<T, NS, VC, true>), dim3((unsigned)pl.units, by), dim3(64),
                      tile * row, s, a, pl, tile, heads_max);
   return hipGetLastError();
@@ -401,18 +443,34 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
-// bf16 pieces of the elements [8 s, 8 s + 8) of v
+// bf16 pieces of two values, as the halves of a word each
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 template <int N>
-__device__ __forceinline__ void split8(v8bf (&p)[N], const float* v) {
+__device__ __forceinline__ void split2(uint32_t (&p)[N], float x, float y) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float x = v[e];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      p[k][e] = (__bf16)x;
-      if (k + 1 < N) x -= (float)p[k][e];
+  for (int k = 0; k < N; ++k) {
+    const v2f v = {x, y};
+    p[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2bf));
+    if (k + 1 < N) {
+      x -= __uint_as_float(p[k] << 16);
+      y -= __uint_as_float(p[k] & 0xffff0000u);
     }
   }
+}
+// of eight values, as MFMA operands
+template <int N>
+__device__ __forceinline__ void split8(v8bf (&p)[N], const float* v) {
+  u32x4 w[N];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t q[N];
+    split2<N>(q, v[2 * e], v[2 * e + 1]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[k][e] = q[k];
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) p[k] = __builtin_bit_cast(v8bf, w[k]);
 }
 
 // c += (sum of a) (sum of b), pieces whose indices add up to less than ORD
@@ -442,34 +500,96 @@ struct Pieces<__bf16> {
 };
 constexpr int kStatePieces = 3;
 
-// LDS of a block, in bytes.  B by rows and B^T share a place: the first is
-// done with when C B^T is.
+// LDS of a block, in bytes
 template <typename T, int NT>
 struct MmLds {
   static constexpr int NP = 32 * NT;
   static constexpr int kRowB = (NP + 8) * 2;  // a row of B or C, padded by 16 bytes
   static constexpr int kRowT = (kQ + 8) * 2;  // a row of B^T
   static constexpr int kPieceB = kQ * kRowB, kPieceT = NP * kRowT;
-  static constexpr int kB = Pieces<T>::IN * (kPieceB > kPieceT ? kPieceB : kPieceT);
-  static constexpr int kC = Pieces<T>::IN * kPieceB;
   static constexpr int kRowCb = kQ + 4;  // floats
   static constexpr int kCb = kQ * kRowCb * 4;
   static constexpr int kScal = 5 * kQ * 4;  // per wave: c (two parts), d, e^c, e^{c_Q - c} d
-  static constexpr int bytes(int nw) { return kB + kC + kCb + nw * kScal; }
+  static constexpr int whole(int nw) {
+    return Pieces<T>::IN * (2 * kPieceB + kPieceT) + kCb + nw * kScal;
+  }
+  // B by rows and B^T share a place where they do not both fit: the first is
+  // done with when C B^T is
+  static constexpr bool kShared = whole(4) > 80 * 1024;
+  static constexpr int kC = Pieces<T>::IN * (kShared && kPieceT > kPieceB ? kPieceT : kPieceB);
+  static constexpr int kT = kShared ? 0 : kC + Pieces<T>::IN * kPieceB;
+  static constexpr int kAfter = kC + Pieces<T>::IN * (kPieceB + (kShared ? 0 : kPieceT));
+  static constexpr int bytes(int nw) { return kAfter + kCb + nw * kScal; }
 };
 
+// running sums over each half of the wave
+__device__ __forceinline__ double half_scan(double v) {
+  auto add = [&](auto dpp) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)dpp((int)(uint32_t)b), hi = (uint32_t)dpp((int)(uint32_t)(b >> 32));
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);  // +0 without a source
+  };
+  add([](int x) { return dpp_or0<0x111>(x); });
+  add([](int x) { return dpp_or0<0x112>(x); });
+  add([](int x) { return dpp_or0<0x114>(x); });
+  add([](int x) { return dpp_or0<0x118>(x); });
+  add([](int x) { return dpp_or0<0x142, 0xa>(x); });
+  return v;
+}
+
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane),
+                 hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// keeps the compiler from working the offsets of 16 rows out ahead of the
+// loop and holding them in registers
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// a state tile in `ends`
+template <int NT>
+__device__ __forceinline__ void put_tile(float* e, const v16f (&S)[NT]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *(float4*)(e + (nt * 4 + q) * 256) =
+          make_float4(S[nt][4 * q], S[nt][4 * q + 1], S[nt][4 * q + 2], S[nt][4 * q + 3]);
+}
+template <int NT>
+__device__ __forceinline__ void get_tile(v16f (&S)[NT], const float* e) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 v = *(const float4*)(e + (nt * 4 + q) * 256);
+      S[nt][4 * q] = v.x;
+      S[nt][4 * q + 1] = v.y;
+      S[nt][4 * q + 2] = v.z;
+      S[nt][4 * q + 3] = v.w;
+    }
+}
+
 template <typename T, int NT, int NW, bool FULL>
-__global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int tiles, int wide) {
+__global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, ScanPlan pl, int tiles, int wide) {
   using L = MmLds<T, NT>;
   constexpr int IN = Pieces<T>::IN, YP = Pieces<T>::Y;
+  constexpr bool kExact = YP == 3;  // y to better than bf16
   constexpr int kThreads = 64 * NW;
   constexpr int kBlocks = 64 * NT;  // 4x4 blocks of B (or C) in a chunk
   constexpr int kItems = ((FULL ? 2 : 1) * kBlocks + kThreads - 1) / kThreads;
   extern __shared__ float4 sh4[];
   uint8_t* shB = (uint8_t*)sh4;
-  uint8_t* shC = shB + L::kB;
-  float* shCb = (float*)(shC + L::kC);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, li = lane & 31;
+  uint8_t* shC = shB + L::kC;
+  uint8_t* shT = shB + L::kT;
+  float* shCb = (float*)(shB + L::kAfter);
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, li = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   float* scal = (float*)((uint8_t*)shCb + L::kCb) + wave * (L::kScal / 4);
   float *shHi = scal, *shLo = scal + kQ, *shD = scal + 2 * kQ, *shE = scal + 3 * kQ,
         *shW = scal + 4 * kQ;
@@ -487,8 +607,8 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
   const bool on = active && p < a.hd;
   const int64_t c = (int64_t)h * a.hd + p;
   const int64_t unit0 = (int64_t)blockIdx.x - w.u.k;
-  constexpr int kTile = NT * 16 * 64;  // floats of a state tile in `ends`
-  const int64_t tile_at = ((int64_t)h * ptiles + pt) * kTile + lane;
+  constexpr int kTile = NT * 16 * 64;  // floats of a state tile in `ends`: [nt][r / 4][lane][4]
+  const int64_t tile_at = ((int64_t)h * ptiles + pt) * kTile + 4 * lane;
   const int64_t unit_floats = (int64_t)a.heads * ptiles * kTile;
 
   v16f S[NT];
@@ -496,143 +616,155 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) S[nt][r] = 0.0f;
-  if (on && w.keep && (FULL ? w.last == 0 : w.u.k == 0)) {
-    const float* st = a.state + (int64_t)w.slot * a.ss + c * a.n;
+  // the tile's part of the slot
+  const auto bst = rows_at(a.state + (w.slot >= 0 ? (int64_t)w.slot * a.ss : 0) + (c - li) * a.n,
+                           w.slot >= 0 && active ? (uint32_t)(min(32, a.hd - pt * 32) * a.n * 4) : 0);
+  auto state_off = [&](int nt, int r) {
+    const int n = nt * 32 + acc_row(r, half);
+    return n < a.n ? (uint32_t)((li * a.n + n) * 4) : kNoColumn;
+  };
+  if (w.keep && (FULL ? w.last == 0 : w.u.k == 0)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = nt * 32 + acc_row(r, half);
-        if (n < a.n) S[nt][r] = st[n];
-      }
+      for (int r = 0; r < 16; ++r) S[nt][r] = load_row<float, 1>(bst, state_off(nt, r)).v[0];
   }
   if constexpr (!FULL) {
     if (w.u.k == 0) {
       if (active) {
         float* e = pl.ends + (unit0 + w.last) * unit_floats + tile_at;
+        put_tile(e, S);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            e[(nt * 16 + r) * 64] = S[nt][r];
-            S[nt][r] = 0.0f;
-          }
+          for (int r = 0; r < 16; ++r) S[nt][r] = 0.0f;
       }
     }
   } else if (w.last > 0 && active) {
-    const float* e = pl.ends + (unit0 + w.last) * unit_floats + tile_at;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) S[nt][r] = e[(nt * 16 + r) * 64];
-    for (int j = 0; j < w.u.k; ++j) {
-      e = pl.ends + (unit0 + j) * unit_floats + tile_at;
-      const float dec = pl.decays[(unit0 + j) * a.heads + h];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          S[nt][r] = __builtin_fmaf(S[nt][r], dec, e[(nt * 16 + r) * 64]);
-    }
+    get_tile(S, pl.ends + (int64_t)blockIdx.x * unit_floats + tile_at);
   }
 
-  const float A = a.A[h];
+  const float A = a.A[h], bias = bias_of(a, h);
   const float Dp = FULL && on && a.D ? a.D[c] : 0.0f;
   double total = 0.0;  // of the unit's exponents, in powers of two
 
-  // the next chunk's values, loaded while a chunk is worked on
-  T nx[16], nz[16], ndt = (T)0.0f;
-  Pack<T, 4> nb[kItems][4];
-  auto fetch = [&](int t) {
+  const uint32_t xs = (uint32_t)(a.xs * sizeof(T)), zs = (uint32_t)(a.zs * sizeof(T)),
+                 ys = (uint32_t)(a.ys * sizeof(T));
+  const uint32_t col = (uint32_t)(c * sizeof(T));
+  const uint32_t xoff = on ? col + 4 * half * xs : kNoColumn,
+                 zoff = on ? col + 4 * half * zs : kNoColumn,
+                 yoff = on ? col + 4 * half * ys : kNoColumn;
+  // the next chunk's B, C and dt, and in the first pass x, are loaded while a
+  // chunk is worked on; x and z of the second pass are not needed before B
+  // and C have been through LDS
+  uint32_t nx[16], ndt = 0;
+  Raw4<T> nb[kItems][4];
+  auto fetch_bc = [&](int t, auto load4) {
+    const int rows = min(kQ, w.t1 - t);
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      const int id = tid + k * kThreads;
-      if (id >= (FULL ? 2 : 1) * kBlocks) continue;
-      const bool isC = id >= kBlocks;
-      const int blk = isC ? id - kBlocks : id;
+      const int first = wave * 64 + k * kThreads;  // kBlocks: whole waves
+      if (first >= (FULL ? 2 : 1) * kBlocks) break;
+      const bool isC = first >= kBlocks;
+      const int blk = tid + k * kThreads - (isC ? kBlocks : 0);
       const int n = blk % (8 * NT) * 4, j = blk / (8 * NT) * 4;
-      const T* src = (const T*)(isC ? a.C : a.B) + (int64_t)g * a.n + n;
-      const int64_t stride = isC ? a.Cs : a.Bs;
+      const auto src = rows_of<T>(isC ? a.C : a.B, t, isC ? a.Cs : a.Bs, rows);
+      const uint32_t stride = (uint32_t)((isC ? a.Cs : a.Bs) * sizeof(T));
+      const uint32_t off = here(j * stride + (uint32_t)((g * a.n + n) * sizeof(T)));
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bool row = t + j + q < w.t1;
-        const T* s = src + (int64_t)(t + j + q) * stride;
-        if (wide) {
-          if (row && n < a.n) nb[k][q] = *(const Pack<T, 4>*)s;
-          else nb[k][q] = Pack<T, 4>{{(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f}};
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) nb[k][q].v[i] = row && n + i < a.n ? s[i] : (T)0.0f;
-        }
-      }
+      for (int q = 0; q < 4; ++q) nb[k][q] = load4(src, off + q * stride, n);
     }
-    const T* xp = (const T*)a.x + c;
-    const T* zp = (const T*)a.z + c;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int64_t row = t + acc_row(r, half);
-      const bool in = on && row < w.t1;
-      nx[r] = in ? xp[row * a.xs] : (T)0.0f;
-      if (FULL && a.z) nz[r] = in ? zp[row * a.zs] : (T)0.0f;
-    }
-    if (active && t + li < w.t1) ndt = ((const T*)a.dt)[(int64_t)(t + li) * a.dts + h];
   };
-  if (w.t0 < w.t1) fetch(w.t0);
-
-  for (int t = w.t0; t < w.t1; t += kQ) {
-    // this chunk's values out of the fetched ones; B and C by rows into LDS
-    float x[16], z[16];
+  auto fetch_x = [&](int t) {
+    const auto bx = rows_of<T>(a.x, t, a.xs, min(kQ, w.t1 - t));
+    const uint32_t xo = here(xoff);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] = (float)nx[r];
-      if (FULL) z[r] = (float)nz[r];
-    }
-    Pack<T, 4> b[kItems][4];
+    for (int r = 0; r < 16; ++r) nx[r] = load_raw<T>(bx, xo + acc_row(r, 0) * xs);
+  };
+  auto fetch = [&](int t) {
+    const int rows = min(kQ, w.t1 - t);
+    if (wide)
+      fetch_bc(t, [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
+        return load_raw4<T>(r, n < a.n ? off : kNoColumn);
+      });
+    if (!FULL) fetch_x(t);
+    const auto bdt = rows_of<T>(a.dt, t, a.dts, rows);
+    ndt = load_raw<T>(bdt, li * (uint32_t)(a.dts * sizeof(T)) + h * (uint32_t)sizeof(T));
+  };
+  // value by value, where four do not lie on one load's alignment: not ahead
+  auto fetch_narrow = [&](int t) {
+    fetch_bc(t, [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
+      Raw4<T> o;
+      uint32_t v[4];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k)
+      for (int i = 0; i < 4; ++i)
+        v[i] = load_raw<T>(r, n + i < a.n ? off + i * (uint32_t)sizeof(T) : kNoColumn);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) b[k][q] = nb[k][q];
-    const float d = active && t + li < w.t1 ? step_of(a, (float)ndt, h) : 0.0f;
-    if (t + kQ < w.t1) fetch(t + kQ);
-    if constexpr (FULL) {
+      for (int i = 0; i < (int)sizeof(T); ++i)
+        o.w[i] = sizeof(T) == 2 ? v[2 * i & 3] | v[(2 * i + 1) & 3] << 16 : v[i];
+      return o;
+    });
+  };
+  // four values of four rows (or columns) of B or C as pieces in LDS: `at`
+  // is the first one's place, rows `row` bytes and pieces `piece` bytes apart
+  auto put = [&](uint8_t* at, int row, int piece, const Raw4<T> (&b)[4], bool turn) {
 #pragma unroll
-      for (int k = 0; k < kItems; ++k) {
-        const int id = tid + k * kThreads;
-        if (id >= 2 * kBlocks) continue;
-        const bool isC = id >= kBlocks;
-        const int blk = isC ? id - kBlocks : id;
-        const int n = blk % (8 * NT) * 4, j = blk / (8 * NT) * 4;
-        // four values' place in their 16: quarters 0, 2 | 1, 3
-        const int at = (n & ~15) + ((n >> 2) & 1) * 8 + ((n >> 3) & 1) * 4;
+    for (int q = 0; q < 4; ++q) {
+      float v[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4];
+      for (int i = 0; i < 4; ++i) v[i] = turn ? raw4_f32(b[i], q) : raw4_f32(b[q], i);
+      uint32_t lo[IN], hi[IN];
+      split2<IN>(lo, v[0], v[1]);
+      split2<IN>(hi, v[2], v[3]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = (float)b[k][q].v[i];
-#pragma unroll
-          for (int pc = 0; pc < IN; ++pc) {
-            Pack<__bf16, 4> o;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              o.v[i] = (__bf16)v[i];
-              v[i] -= (float)o.v[i];
-            }
-            *(Pack<__bf16, 4>*)((isC ? shC : shB) + pc * L::kPieceB + (j + q) * L::kRowB + at * 2) = o;
-          }
-        }
+      for (int pc = 0; pc < IN; ++pc) {
+        const u32x2 o = {lo[pc], hi[pc]};
+        *(u32x2*)(at + pc * piece + q * row) = o;
       }
     }
+  };
+  // four values' place in their 16: quarters 0, 2 | 1, 3
+  auto place = [](int i) { return (i & ~15) + ((i >> 2) & 1) * 8 + ((i >> 3) & 1) * 4; };
+  auto put_turned = [&](int id, const Raw4<T> (&b)[4]) {
+    const int n = id % (8 * NT) * 4, j = id / (8 * NT) * 4;
+    put(shT + n * L::kRowT + place(j) * 2, L::kRowT, L::kPieceT, b, true);
+  };
+
+  if (w.t0 < w.t1) fetch(w.t0);
+  for (int t = w.t0; t < w.t1; t += kQ) {
+    const int rows = min(kQ, w.t1 - t);
+    // B and C into LDS
+    if (!wide) fetch_narrow(t);
+    constexpr int kHeld = L::kShared && FULL ? kItems : 1;
+    Raw4<T> held[kHeld][4];  // B, where its transpose has to wait
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int first = wave * 64 + k * kThreads;
+      if (first >= (FULL ? 2 : 1) * kBlocks) break;
+      const bool isC = first >= kBlocks;
+      const int blk = tid + k * kThreads - (isC ? kBlocks : 0);
+      const int n = blk % (8 * NT) * 4, j = blk / (8 * NT) * 4;
+      if (FULL)
+        put((isC ? shC : shB) + j * L::kRowB + place(n) * 2, L::kRowB, L::kPieceB, nb[k], false);
+      if (L::kShared && FULL) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) held[k][q] = nb[k][q];
+      } else if (!isC) {
+        put_turned(blk, nb[k]);
+      }
+    }
+    float x[16];
+    if (!FULL)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = raw_f32<T>(nx[r]);
     // the chunk's exponents, by lane li (both halves alike)
+    const float d = li < rows ? step_of(a, raw_f32<T>(ndt), bias) : 0.0f;
     double cum = (double)A * (double)d * 1.4426950408889634;
     cum = cum < -256.0 ? -256.0 : (cum > 256.0 ? 256.0 : cum);
-#pragma unroll
-    for (int m = 1; m < kQ; m <<= 1) {
-      const double o = __shfl_up(cum, m, kQ);
-      if (li >= m) cum += o;
-    }
-    const double whole = __shfl(cum, kQ - 1, kQ);
+    cum = half_scan(cum);
+    const double whole = lane_f64(cum, kQ - 1);
     total += whole;
-    const float eall = __builtin_amdgcn_exp2f((float)whole);
+    float eall = __builtin_amdgcn_exp2f((float)whole);
     if (half == 0) {
       const float hi = (float)cum;
       shHi[li] = hi;
@@ -641,32 +773,50 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
       shE[li] = __builtin_amdgcn_exp2f(hi);
       shW[li] = __builtin_amdgcn_exp2f((float)(whole - cum)) * d;
     }
+    uint32_t z[16];
+    if (FULL) {
+      fetch_x(t);
+      const auto bz = rows_of<T>(a.z, t, a.zs, a.z ? rows : 0);
+      const uint32_t zo = here(zoff);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = load_raw<T>(bz, zo + acc_row(r, 0) * zs);
+    }
+    if (t + kQ < w.t1) fetch(t + kQ);
     __syncthreads();
 
-    v16f Y;
     if constexpr (FULL) {
       // C B^T of the chunk: three 16x16 tiles on and below the diagonal
       if (wave < 3) {
         const int jt = wave == 2 ? 16 : 0, it = wave == 0 ? 0 : 16;
         const int lr = lane & 15, lg = lane >> 4;
         v4f cb = {0.0f, 0.0f, 0.0f, 0.0f};
+        // operands of kAhead steps of 32 are read before the first is used
+        constexpr int kAhead = IN == 1 ? (NT < 4 ? NT : 4) : 1;
 #pragma unroll
-        for (int k = 0; k < NT; ++k) {
-          v8bf pb[IN], pc[IN];
+        for (int k0 = 0; k0 < NT; k0 += kAhead) {
+          v8bf pb[kAhead][IN], pc[kAhead][IN];
 #pragma unroll
-          for (int i = 0; i < IN; ++i) {
-            pb[i] = *(const v8bf*)(shB + i * L::kPieceB + (jt + lr) * L::kRowB + (32 * k + 8 * lg) * 2);
-            pc[i] = *(const v8bf*)(shC + i * L::kPieceB + (it + lr) * L::kRowB + (32 * k + 8 * lg) * 2);
-          }
+          for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-          for (int i = 0; i < IN; ++i)
+            for (int i = 0; i < IN; ++i) {
+              const int at = (32 * (k0 + k) + 8 * lg) * 2;
+              pb[k][i] = *(const v8bf*)(shB + i * L::kPieceB + (jt + lr) * L::kRowB + at);
+              pc[k][i] = *(const v8bf*)(shC + i * L::kPieceB + (it + lr) * L::kRowB + at);
+            }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < IN; ++j)
-              if (i + j < YP) cb = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pb[i], pc[j], cb, 0, 0, 0);
+          for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (int i = 0; i < IN; ++i)
+#pragma unroll
+              for (int j = 0; j < IN; ++j)
+                if (i + j < YP)
+                  cb = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pb[k][i], pc[k][j], cb, 0, 0, 0);
         }
         *(v4f*)(shCb + (it + lr) * L::kRowCb + jt + 4 * lg) = cb;
       }
       // C S, scaled by e^{c_i}
+      v16f Y;
 #pragma unroll
       for (int r = 0; r < 16; ++r) Y[r] = 0.0f;
 #pragma unroll
@@ -691,54 +841,24 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
         Y[4 * q + 2] *= e.z;
         Y[4 * q + 3] *= e.w;
       }
-      __syncthreads();  // C B^T is whole, B by rows is done with
-    }
-    // B^T into its place
+      __syncthreads();  // C B^T is whole
+      __builtin_amdgcn_sched_barrier(0);  // nothing that waits for x moves up
+      if (L::kShared) {
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const int id = tid + k * kThreads;
-      if (id >= kBlocks) continue;  // C's
-      const int n = id % (8 * NT) * 4, j = id / (8 * NT) * 4;
-      const int at = (j & ~15) + ((j >> 2) & 1) * 8 + ((j >> 3) & 1) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = (float)b[k][q].v[i];
-#pragma unroll
-        for (int pc = 0; pc < IN; ++pc) {
-          Pack<__bf16, 4> o;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            o.v[q] = (__bf16)v[q];
-            v[q] -= (float)o.v[q];
-          }
-          *(Pack<__bf16, 4>*)(shB + pc * L::kPieceT + (n + i) * L::kRowT + at * 2) = o;
-        }
+        for (int k = 0; k < kHeld; ++k)
+          if (tid + k * kThreads < kBlocks) put_turned(tid + k * kThreads, held[k]);
       }
-    }
-    // the weighted x, for the state
-    v8bf xw[2][kStatePieces];
-    {
-      float v[16];
+      // M x within the chunk; a column with an infinite x or NaN is NaN from
+      // that row on, and so is its state
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 e = *(const float4*)(shW + 8 * q + 4 * half);
-        v[4 * q] = x[4 * q] * e.x;
-        v[4 * q + 1] = x[4 * q + 1] * e.y;
-        v[4 * q + 2] = x[4 * q + 2] * e.z;
-        v[4 * q + 3] = x[4 * q + 3] * e.w;
-      }
-      split8<kStatePieces>(xw[0], v);
-      split8<kStatePieces>(xw[1], v + 8);
-    }
-    if constexpr (FULL) {
-      // M x within the chunk
-      bool odd = false;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) odd |= !(__builtin_fabsf(x[r]) < __builtin_inff());
+      for (int r = 0; r < 16; ++r) x[r] = raw_f32<T>(nx[r]);
       int first = kQ;
-      if (__ballot(odd)) {
+      float probe = 0.0f;  // NaN once any x is not finite
+#pragma unroll
+      for (int r = 0; r < 16; ++r) probe = __builtin_fmaf(x[r], 0.0f, probe);
+      const bool odd = __ballot(probe != probe) != 0;
+      if (odd) {
+        asm volatile("");  // a branch, not selects
 #pragma unroll
         for (int r = 15; r >= 0; --r)
           if (!(__builtin_fabsf(x[r]) < __builtin_inff())) {
@@ -746,8 +866,10 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
             x[r] = 0.0f;
           }
         first = min(first, __shfl_xor(first, 32));
+        if (first < kQ) eall = __builtin_nanf("");
       }
-      const float hi = shHi[li], lo = shLo[li];
+      const float hi = shHi[li], lo = kExact ? shLo[li] : 0.0f;
+      const int diag = (int)here((uint32_t)(li - 4 * half));
       float m[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -759,8 +881,12 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
                     l4[4] = {jl.x, jl.y, jl.z, jl.w}, d4[4] = {jd.x, jd.y, jd.z, jd.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f((hi - h4[i]) + (lo - l4[i]));
-          m[4 * q + i] = j0 + i <= li ? cbv[i] * (e * d4[i]) : 0.0f;
+          // for a bf16 y the first parts' difference is exact enough: sums of
+          // up to 2^13, off by 2^-12 each
+          const float e = __builtin_amdgcn_exp2f(kExact ? (hi - h4[i]) + (lo - l4[i]) : hi - h4[i]);
+          float v = cbv[i] * (e * d4[i]);
+          asm volatile("" : "+v"(v));  // a select, not a branch around the exponential
+          m[4 * q + i] = 8 * q + i <= diag ? v : 0.0f;
         }
       }
 #pragma unroll
@@ -770,27 +896,52 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
         split8<IN>(px, x + 8 * s);
         Y = mfma32<YP>(pm, px, Y);
       }
+      const auto by = rows_of<T>(a.y, t, a.ys, rows);
+      const uint32_t yo = here(yoff);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) Y[r] = __builtin_fmaf(Dp, x[r], Y[r]);
+      if (odd) {
+        asm volatile("");
+#pragma unroll
+        for (int r = 0; r < 16; ++r) Y[r] = acc_row(r, half) < first ? Y[r] : __builtin_nanf("");
+      }
+      if (a.z)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          Y[r] *= kExact ? silu_f32(raw_f32<T>(z[r])) : silu_short(raw_f32<T>(z[r]));
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int i = acc_row(r, half);
-        float v = i < first ? Y[r] : __builtin_nanf("");
-        v = __builtin_fmaf(Dp, x[r], v);
-        if (a.z) v *= silu_f32(z[r]);
-        if (on && t + i < w.t1) ((T*)a.y)[(int64_t)(t + i) * a.ys + c] = (T)v;
+        const float out[1] = {Y[r]};
+        store_row<T, 1>(by, yo + acc_row(r, 0) * ys, out);
       }
+      if (L::kShared) __syncthreads();  // B^T is whole
     }
-    __syncthreads();  // B^T is whole
+    // the state
+    {
+      v8bf xw[2][kStatePieces];
+      float v[16];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+      for (int q = 0; q < 4; ++q) {
+        const float4 e = *(const float4*)(shW + 8 * q + 4 * half);
+        v[4 * q] = x[4 * q] * e.x;
+        v[4 * q + 1] = x[4 * q + 1] * e.y;
+        v[4 * q + 2] = x[4 * q + 2] * e.z;
+        v[4 * q + 3] = x[4 * q + 3] * e.w;
+      }
+      split8<kStatePieces>(xw[0], v);
+      split8<kStatePieces>(xw[1], v + 8);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) S[nt][r] *= eall;
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        v8bf pb[IN];
+        for (int r = 0; r < 16; ++r) S[nt][r] *= eall;
 #pragma unroll
-        for (int i = 0; i < IN; ++i)
-          pb[i] = *(const v8bf*)(shB + i * L::kPieceT + (32 * nt + li) * L::kRowT + (16 * s + 8 * half) * 2);
-        S[nt] = mfma32<kStatePieces>(pb, xw[s], S[nt]);
+        for (int s = 0; s < 2; ++s) {
+          v8bf pb[IN];
+#pragma unroll
+          for (int i = 0; i < IN; ++i)
+            pb[i] = *(const v8bf*)(shT + i * L::kPieceT + (32 * nt + li) * L::kRowT + (16 * s + 8 * half) * 2);
+          S[nt] = mfma32<kStatePieces>(pb, xw[s], S[nt]);
+        }
       }
     }
     __syncthreads();  // the next chunk may overwrite LDS
@@ -799,20 +950,16 @@ __global__ __launch_bounds__(64 * NW) void k_scan_mm(SsmArgs a, ScanPlan pl, int
   if constexpr (!FULL) {
     if (!active) return;
     float* e = pl.ends + (int64_t)blockIdx.x * unit_floats + tile_at;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) e[(nt * 16 + r) * 64] = S[nt][r];
+    put_tile(e, S);
     if (pt == 0 && lane == 0)
       pl.decays[(int64_t)blockIdx.x * a.heads + h] = __builtin_amdgcn_exp2f((float)total);
-  } else if (on && w.slot >= 0 && w.u.k == w.last) {
-    float* st = a.state + (int64_t)w.slot * a.ss + c * a.n;
+  } else if (w.slot >= 0 && w.u.k == w.last) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int n = nt * 32 + acc_row(r, half);
-        if (n < a.n) st[n] = S[nt][r];
+        const float out[1] = {S[nt][r]};
+        store_row<float, 1>(bst, state_off(nt, r), out);
       }
   }
 }
@@ -821,7 +968,7 @@ static int mm_ptiles(int hd) { return (hd + 31) / 32; }
 static int mm_nt(int n) { return n <= 32 ? 1 : (n <= 64 ? 2 : (n <= 128 ? 4 : 8)); }
 // waves per block: eight where a group has that many tiles and the state
 // leaves room for two waves per SIMD
-static int mm_waves(int tiles, int nt) { return tiles > 4 && nt < 8 ? 8 : 4; }
+static int mm_waves(int tiles, int nt) { return 4; }
 
 template <typename T, int NT, int NW>
 static hipError_t launch_mm(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
@@ -840,9 +987,12 @@ static hipError_t launch_mm(const SsmArgs& a, const ScanPlan& pl, hipStream_t s)
     if (raised[0] != hipSuccess) return raised[0];
     if (raised[1] != hipSuccess) return raised[1];
   }
-  if (pl.split)
+  if (pl.split) {
     hipLaunchKernelGGL((k_scan_mm<T, NT, NW, false>), grid, dim3(64 * NW), bytes, s, a, pl, tiles,
                        wide);
+    const int head = mm_ptiles(a.hd) * NT * 1024;
+    launch_join<4>(a, pl, (int64_t)a.heads * head, head, s);
+  }
   hipLaunchKernelGGL((k_scan_mm<T, NT, NW, true>), grid, dim3(64 * NW), bytes, s, a, pl, tiles,
                      wide);
   return hipGetLastError();
@@ -862,9 +1012,10 @@ static hipError_t launch_mm_t(const SsmArgs& a, const ScanPlan& pl, hipStream_t 
 
 // ---- the cut into units ----------------------------------------------------
 // Units as short as the chip needs to be filled (kFillWaves waves over all of
-// them), but no shorter than what the first pass and the walk over a
+// them: a little less than the 2048 that the second pass's registers let it
+// hold, since one workgroup that finds no place doubles the whole time), but no shorter than what the first pass and the walk over a
 // sequence's units are worth, and no more than 32 (64) of them in a sequence.
-constexpr int kFillWaves = 2048;
+constexpr int kFillWaves = 1920;
 
 static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
   ScanPlan pl{};
@@ -875,9 +1026,9 @@ static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
   const int step = small ? 32 : kQ, least = small ? 32 : 4 * kQ, most_units = small ? 64 : 32;
   const int64_t T = op->n_tokens;
   const int64_t want = kFillWaves / waves > 1 ? kFillWaves / waves : 1;
-  int64_t len = (T / want + step) / step * step;
-  const int64_t floor_len = (T / most_units + step) / step * step;
-  if (len > 512) len = 512;  // uneven lengths: the longest sequence is cut too
+  int64_t len = ((T + want - 1) / want + step - 1) / step * step;
+  const int64_t floor_len = ((T + most_units - 1) / most_units + step - 1) / step * step;
+  if (len > 512 && op->n_seqs > 1) len = 512;  // uneven lengths: the longest is cut too
   if (len < floor_len) len = floor_len;
   if (len < least) len = least;
   pl.len = (int)len;

@@ -319,14 +319,11 @@ def test_offsets_past_32_bits(hip):
     H, P, N, far = 2, 16, 16, 3
     stride = (1 << 31) + 64
     pool = torch.empty(far * stride, dtype=torch.float32, device="cuda")
-    xs = (1 << 29) + 16
-    rows = torch.empty(9 * xs + 64, dtype=torch.float32, device="cuda")
+    xs, n = (1 << 24) - 16, 270
+    rows = torch.empty(n * xs + 64, dtype=torch.float32, device="cuda")
     for step in (False, True):
-        c = SsmCase("f32", H, P, 1, N, [1] * 9 if step else [9], step=step, slots=None, spare=0)
-        if step:
-            c.slots = [2] + [-1] * 8
-        else:
-            c.slots = [2]
+        c = SsmCase("f32", H, P, 1, N, [1] * n if step else [n], step=step, slots=None, spare=0)
+        c.slots = [-1] * (n - 1) + [2] if step else [2]
         c.n_slots = 3
         state = torch.randn(H * P * N, device="cuda")
         pool[2 * stride:2 * stride + H * P * N] = state
@@ -335,7 +332,7 @@ def test_offsets_past_32_bits(hip):
         want, tols, new, stol = c.want()
         d = c.descriptor()
         d.state, d.state_stride = at(pool), stride
-        wide = rows[:9 * xs].view(9, xs)
+        wide = rows[:n * xs].view(n, xs)
         wide[:, :H * P] = c.x
         d.x, d.x_stride = at(rows), xs
         d.y, d.y_stride = at(rows) + 4 * H * P, xs

@@ -39,7 +39,7 @@ def refused(rc, word):
 SHARED = [("type", dict(type=3)), ("type", dict(type=-1)), ("n_seqs", dict(n_seqs=-1)),
           ("x needs", dict(x=None)), ("x needs", dict(x=P + 2)), ("y needs", dict(y=None)),
           ("y needs", dict(y_stride=63)), ("x needs", dict(x_stride=63)),
-          ("x needs", dict(x_stride=(1 << 30) + 1)), ("slots", dict(n_slots=0)),
+          ("x needs", dict(x_stride=1 << 24)), ("slots", dict(n_slots=0)),
           ("slots", dict(slots=None, n_slots=1)), ("addresses", dict(slots=P + 1)),
           ("addresses", dict(state=P + 2)), ("y overlaps x", dict(y=P + 8)),
           ("y overlaps x", dict(y=P + 4 * 64 * 3))]
