@@ -60,11 +60,12 @@ struct ConvArgs {
 
 template <typename T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
+  const int slots = first_slots(a.q);
   const Unit u = find_unit(a.q, blockIdx.x, kConvRows);
   if (u.b < 0) return;
   const int t0 = u.s + u.k * kConvRows, t1 = min(u.e, t0 + kConvRows);
   if (u.k > 0 && t0 >= t1) return;
-  const int slot = find_slot(a.q, u.b);
+  const int slot = find_slot(a.q, u.b, slots);
   if (slot == kNoSlot) return;
   const int c = (blockIdx.y * 256 + threadIdx.x) * V;
   if (c >= a.channels) return;
@@ -131,7 +132,7 @@ template <typename T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs a) {
   const int b = blockIdx.x;
   const int c = (blockIdx.y * 256 + threadIdx.x) * V;
-  const int slot = find_slot(a.q, b);
+  const int slot = find_slot(a.q, b, first_slots(a.q));
   if (slot == kNoSlot || c >= a.channels) return;
   const Taps<W, V> taps(a.w, a.bias, a.channels, c, a.silu);
   float r[V], o[V], win[W - 1][V];

@@ -184,38 +184,47 @@ struct Unit {
   int k;     // unit of it
   int s, e;  // its rows
 };
-// The unit's sequence by a search in steps of 64 (one load and ballot per
-// level).  All lanes of the wave must call it with the same u.
+// The unit's sequence by a search in steps of 63 (one load and ballot per
+// level, the last of which also has the sequence's rows).  All lanes of the
+// wave must call it with the same u.
 __device__ __forceinline__ Unit find_unit(const SeqView& q, int u, int len) {
   if (!q.seq_start) return Unit{0, u, 0, q.n_tokens};
   const int lane = threadIdx.x & 63;
   int lo = 0, hi = q.n_seqs;
-  do {
-    const int step = (hi - lo + 63) / 64;
-    const int i = lo + lane * step;
-    const bool below = i < hi && seq_row(q, i) / len + i <= u;
-    const int c = __popcll(__ballot(below));
+  for (;;) {
+    const int step = (hi - lo + 62) / 63;
+    const int i = min(lo + lane * step, hi);
+    const int row = seq_row(q, i);
+    const int c = __popcll(__ballot(i < hi && row / len + i <= u));
     if (c == 0) return Unit{-1, 0, 0, 0};  // rows before the first sequence
+    if (step == 1) {
+      const int s = __builtin_amdgcn_readlane(row, c - 1), e = __builtin_amdgcn_readlane(row, c);
+      const int b = lo + c - 1;
+      return Unit{b, u - (s / len + b), s, e < s ? s : e};
+    }
     lo += (c - 1) * step;
     hi = min(hi, lo + step);
-  } while (hi - lo > 1);
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  const int s = __builtin_amdgcn_readfirstlane(seq_row(q, lo));
-  const int e = __builtin_amdgcn_readfirstlane(seq_row(q, lo + 1));
-  return Unit{lo, u - (s / len + lo), s, e < s ? s : e};
+  }
 }
 
 constexpr int kNoSlot = -1, kNoPool = -2;
+// The slots of the first 64 sequences, one per lane: a load that waits for
+// nothing, issued before the sequence is known.
+__device__ __forceinline__ int first_slots(const SeqView& q) {
+  const int lane = threadIdx.x & 63;
+  return q.n_slots != 0 && q.slots ? q.slots[min(lane, q.n_seqs - 1)] : 0;
+}
 // The slot of sequence b; kNoSlot: padding.  All lanes of the wave must call
-// it with the same b.
-__device__ __forceinline__ int find_slot(const SeqView& q, int b) {
+// it with the same b; first: first_slots().
+__device__ __forceinline__ int find_slot(const SeqView& q, int b, int first) {
   if (q.n_slots == 0) return kNoPool;
   if (!q.slots) return b;  // checked by the host: n_seqs <= n_slots
   const int lane = threadIdx.x & 63;
-  const int slot = __builtin_amdgcn_readfirstlane(q.slots[b]);
+  const int slot = b < 64 ? __builtin_amdgcn_readlane(first, b)
+                          : __builtin_amdgcn_readfirstlane(q.slots[b]);
   if (slot < 0 || slot >= q.n_slots) return kNoSlot;
-  bool taken = false;
-  for (int j = lane; j < b; j += 64) taken |= q.slots[j] == slot;
+  bool taken = lane < b && first == slot;
+  for (int j = lane + 64; j < b; j += 64) taken |= q.slots[j] == slot;
   return __ballot(taken) ? kNoSlot : slot;
 }
 

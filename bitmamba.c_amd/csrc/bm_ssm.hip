@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs a) {
   const int nw = blockDim.x >> 6;
   const int p0 = (blockIdx.z * nw + wave) * (kRows * U) + lane / TEAM;
   const int nl = (lane % TEAM) * V;
-  const int slot = find_slot(a.q, b);
+  const int slot = find_slot(a.q, b, first_slots(a.q));
   if (slot == kNoSlot) return;
   const int g = h / (a.heads / a.groups);
   const float d = step_of(a, (float)((const T*)a.dt)[(int64_t)b * a.dts + h], bias_of(a, h));
@@ -177,15 +177,235 @@ struct ScanUnit {
 };
 // false: nothing to do (no such unit, or padding)
 __device__ __forceinline__ bool scan_unit(const SeqView& q, int index, int len, ScanUnit& w) {
+  const int slots = first_slots(q);
   w.u = find_unit(q, index, len);
   if (w.u.b < 0) return false;
   w.t0 = w.u.s + w.u.k * len;
   w.last = w.u.e > w.u.s ? (w.u.e - w.u.s - 1) / len : 0;
   if (w.u.k > w.last) return false;
   w.t1 = w.u.e - w.t0 < len ? w.u.e : w.t0 + len;
-  w.slot = find_slot(q, w.u.b);
+  w.slot = find_slot(q, w.u.b, slots);
   w.keep = w.slot >= 0 && !(q.fresh && q.fresh[w.u.b]);
   return w.slot != kNoSlot;
+}
+
+// ---- up to 8 state values per channel -------------------------------------
+// A lane owns VC neighbouring channels with their state in registers and
+// walks the unit's rows; a block is one wave.  What the channels of a head
+// share per row -- decay, d B[n], C[n] -- is worked out once per row and head
+// into LDS.  2-4 operations per state value and row against 12 bytes per
+// channel and row: bound by memory, and in one short prompt by the round
+// trips to it, so that a tile's loads are all issued before any is used.
+constexpr int kSmallState = 8;
+constexpr int kSmallRows = 16;  // rows per tile
+__host__ __device__ constexpr int small_entry(int ns) { return (1 + 2 * ns + 3) / 4 * 4; }
+
+template <typename T, int NS, int VC, bool FULL>
+__global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int heads_max) {
+  constexpr int tile = kSmallRows, EW = small_entry(NS);
+  extern __shared__ float4 sh4[];
+  float* sh = (float*)sh4;  // [tile][heads_max][EW]
+  ScanUnit w;
+  if (!scan_unit(a.q, blockIdx.x, pl.len, w)) return;
+  if (!FULL && w.u.k == w.last) return;
+  const int lane = threadIdx.x, channels = a.heads * a.hd;
+  const int c0 = blockIdx.y * 64 * VC;
+  const int c = c0 + lane * VC;
+  const bool on = c < channels;  // VC divides head_dim where it is more than 1
+  const int h0 = c0 / a.hd;
+  const int h1 = (min(c0 + 64 * VC, channels) - 1) / a.hd;
+  const int nh = h1 - h0 + 1;
+  const int h = on ? c / a.hd : h0;
+  const int per = a.heads / a.groups;
+  const int64_t unit0 = (int64_t)blockIdx.x - w.u.k;
+  const int64_t unit_floats = (int64_t)channels * a.n;
+
+  const uint32_t col = on ? (uint32_t)(c * sizeof(T)) : kNoColumn;
+  const uint32_t xs = (uint32_t)(a.xs * sizeof(T)), zs = (uint32_t)(a.zs * sizeof(T)),
+                 ys = (uint32_t)(a.ys * sizeof(T));
+  Pack<T, VC> xr[kSmallRows], zr[kSmallRows];
+  auto fetch = [&](int t) {
+    const int rows = min(tile, w.t1 - t);
+    const auto bx = rows_of<T>(a.x, t, a.xs, rows);
+    const auto bz = rows_of<T>(a.z, t, a.zs, FULL && a.z ? rows : 0);
+#pragma unroll
+    for (int r = 0; r < kSmallRows; ++r) {
+      xr[r] = load_row<T, VC>(bx, col + r * xs);
+      if (FULL) zr[r] = load_row<T, VC>(bz, col + r * zs);
+    }
+  };
+  if (w.t0 < w.t1) fetch(w.t0);
+
+  float S[NS][VC];
+#pragma unroll
+  for (int n = 0; n < NS; ++n)
+#pragma unroll
+    for (int i = 0; i < VC; ++i) S[n][i] = 0.0f;
+  // from the slot, or from the copy that the first pass made of it
+  if (on && w.keep && (FULL ? w.last == 0 : w.u.k == 0)) {
+    const float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < VC; ++i)
+        if (n < a.n) S[n][i] = st[i * a.n + n];
+  }
+  if constexpr (!FULL) {
+    if (w.u.k == 0) {
+      if (on) {
+        float* e = pl.ends + (unit0 + w.last) * unit_floats;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+          if (n < a.n) store_f32<float, VC>(e + (int64_t)n * channels + c, S[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int i = 0; i < VC; ++i) S[n][i] = 0.0f;
+    }
+  } else if (w.last > 0 && on) {
+    // the join, a few floats of each unit before this one: cheaper here than
+    // a launch of its own (4.7 us and its gap against 3 us)
+    constexpr int kAhead = NS == 1 ? 16 : 4;
+    const float* e = pl.ends + unit0 * unit_floats + c;
+    const float* dec = pl.decays + unit0 * a.heads + h;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+      if (n < a.n) load_f32<float, VC>(S[n], e + w.last * unit_floats + (int64_t)n * channels);
+    for (int j0 = 0; j0 < w.u.k; j0 += kAhead) {
+      float v[kAhead][NS][VC], d[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int j = min(j0 + i, w.u.k - 1);
+        d[i] = dec[(int64_t)j * a.heads];
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+          load_f32<float, VC>(v[i][n], e + j * unit_floats + (int64_t)min(n, a.n - 1) * channels);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (j0 + i >= w.u.k) break;
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int k = 0; k < VC; ++k)
+            S[n][k] = n < a.n ? __builtin_fmaf(S[n][k], d[i], v[i][n][k]) : 0.0f;
+      }
+    }
+  }
+
+  float D[VC], all = 1.0f;
+#pragma unroll
+  for (int i = 0; i < VC; ++i) D[i] = FULL && on && a.D ? a.D[c + i] : 0.0f;
+  for (int t = w.t0; t < w.t1; t += tile) {
+    const int rows = min(tile, w.t1 - t);
+    for (int i = lane; i < tile * nh; i += 64) {
+      const int r = i / nh, hh = i - r * nh;
+      float* s = sh + (r * heads_max + hh) * EW;
+      if (r >= rows) {  // past the unit: leaves the state as it is
+        s[0] = 1.0f;
+#pragma unroll
+        for (int n = 1; n < EW; ++n) s[n] = 0.0f;
+        continue;
+      }
+      const int64_t row = t + r;
+      const int g = (h0 + hh) / per;
+      const float d = step_of(a, (float)((const T*)a.dt)[row * a.dts + h0 + hh],
+                              bias_of(a, h0 + hh));
+      s[0] = exp_f32(a.A[h0 + hh] * d);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const bool have = n < a.n;
+        s[1 + n] = have ? d * (float)((const T*)a.B)[row * a.Bs + (int64_t)g * a.n + n] : 0.0f;
+        if (FULL)
+          s[1 + NS + n] = have ? (float)((const T*)a.C)[row * a.Cs + (int64_t)g * a.n + n] : 0.0f;
+      }
+    }
+    __syncthreads();
+    float x[kSmallRows][VC], z[kSmallRows][VC];
+#pragma unroll
+    for (int r = 0; r < kSmallRows; ++r)
+#pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        x[r][i] = (float)xr[r].v[i];
+        z[r][i] = FULL && a.z ? silu_f32((float)zr[r].v[i]) : 1.0f;
+      }
+    if (t + tile < w.t1) fetch(t + tile);
+    const auto by = rows_of<T>(a.y, t, a.ys, rows);
+#pragma unroll
+    for (int r = 0; r < kSmallRows; ++r) {
+      float e[EW];
+      const float4* s = (const float4*)(sh + (r * heads_max + (h - h0)) * EW);
+#pragma unroll
+      for (int k = 0; k < EW / 4; ++k) *(float4*)(e + 4 * k) = s[k];
+      float y[VC];
+#pragma unroll
+      for (int i = 0; i < VC; ++i) y[i] = FULL ? D[i] * x[r][i] : 0.0f;
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+          S[n][i] = __builtin_fmaf(S[n][i], e[0], x[r][i] * e[1 + n]);
+          // a value beyond d_state stays zero even where the decay is infinite
+          if (NS > 2) S[n][i] = n < a.n ? S[n][i] : 0.0f;
+          if (FULL) y[i] = __builtin_fmaf(S[n][i], e[1 + NS + n], y[i]);
+        }
+      all *= e[0];
+      if (FULL) {
+#pragma unroll
+        for (int i = 0; i < VC; ++i) y[i] *= z[r][i];
+        store_row<T, VC>(by, col + r * ys, y);
+      }
+    }
+    __syncthreads();
+  }
+  if (!on) return;
+  if constexpr (!FULL) {
+    float* e = pl.ends + (int64_t)blockIdx.x * unit_floats;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+      if (n < a.n) store_f32<float, VC>(e + (int64_t)n * channels + c, S[n]);
+    if (c % a.hd == 0) pl.decays[(int64_t)blockIdx.x * a.heads + h] = all;
+  } else if (w.slot >= 0 && w.u.k == w.last) {
+    float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < VC; ++i)
+        if (n < a.n) st[i * a.n + n] = S[n][i];
+  }
+}
+
+template <typename T, int NS, int VC>
+static hipError_t launch_small(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
+  const int span = 64 * VC, channels = a.heads * a.hd;
+  const int by = (channels + span - 1) / span;
+  const int hm = (span + a.hd - 2) / a.hd + 1;
+  const int heads_max = hm < a.heads ? hm : a.heads;
+  const int bytes = kSmallRows * heads_max * small_entry(NS) * 4;
+  if (bytes > 64 * 1024) {  // heads of one channel; once per process
+    static const hipError_t raised[2] = {
+        hipFuncSetAttribute((const void*)k_scan_small<T, NS, VC, false>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024),
+        hipFuncSetAttribute((const void*)k_scan_small<T, NS, VC, true>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)};
+    if (raised[0] != hipSuccess) return raised[0];
+    if (raised[1] != hipSuccess) return raised[1];
+  }
+  if (pl.split)
+    hipLaunchKernelGGL((k_scan_small<T, NS, VC, false>), dim3((unsigned)pl.units, by), dim3(64),
+                       bytes, s, a, pl, heads_max);
+  hipLaunchKernelGGL((k_scan_small<T, NS, VC, true>), dim3((unsigned)pl.units, by), dim3(64),
+                     bytes, s, a, pl, heads_max);
+  return hipGetLastError();
+}
+
+template <typename T, int VC>
+static hipError_t launch_small_n(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
+  if (a.n == 1) return launch_small<T, 1, VC>(a, pl, s);
+  if (a.n == 2) return launch_small<T, 2, VC>(a, pl, s);
+  if (a.n <= 4) return launch_small<T, 4, VC>(a, pl, s);
+  return launch_small<T, 8, VC>(a, pl, s);
 }
 
 // The join: a thread takes V neighbouring floats of a sequence's units in
@@ -227,182 +447,6 @@ static void launch_join(const SsmArgs& a, const ScanPlan& pl, int64_t unit_float
   hipLaunchKernelGGL((k_scan_join<V>),
                      dim3((unsigned)pl.units, (unsigned)((unit_floats / V + 255) / 256)), dim3(256),
                      0, s, a.q, pl, unit_floats, head_stride, a.heads);
-}
-
-// ---- up to 8 state values per channel -------------------------------------
-// A lane owns VC neighbouring channels with their state in registers and
-// walks the unit's rows; a block is one wave.  What the channels of a head
-// share per row -- decay, d B[n], C[n] -- is worked out once per row and head
-// into LDS.  2-4 operations per state value and row against 12 bytes per
-// channel and row: bound by memory.
-constexpr int kSmallState = 8;
-__host__ __device__ constexpr int small_entry(int ns) { return (1 + 2 * ns + 3) / 4 * 4; }
-constexpr int kSmallRows = 16;  // rows of x and z in flight per lane
-
-template <typename T, int NS, int VC, bool FULL>
-__global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int tile, int heads_max) {
-  constexpr int EW = small_entry(NS);
-  extern __shared__ float4 sh4[];
-  float* sh = (float*)sh4;  // [tile][heads_max][EW]
-  ScanUnit w;
-  if (!scan_unit(a.q, blockIdx.x, pl.len, w)) return;
-  if (!FULL && w.u.k == w.last) return;
-  const int lane = threadIdx.x, channels = a.heads * a.hd;
-  const int c0 = blockIdx.y * 64 * VC;
-  const int c = c0 + lane * VC;
-  const bool on = c < channels;  // VC divides head_dim where it is more than 1
-  const int h0 = c0 / a.hd;
-  const int h1 = (min(c0 + 64 * VC, channels) - 1) / a.hd;
-  const int nh = h1 - h0 + 1;
-  const int h = on ? c / a.hd : h0;
-  const int per = a.heads / a.groups;
-  const int64_t unit0 = (int64_t)blockIdx.x - w.u.k;
-
-  float S[NS][VC];
-#pragma unroll
-  for (int n = 0; n < NS; ++n)
-#pragma unroll
-    for (int i = 0; i < VC; ++i) S[n][i] = 0.0f;
-  // from the slot, or from the copy that the first pass made of it
-  if (on && w.keep && (FULL ? w.last == 0 : w.u.k == 0)) {
-    const float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int i = 0; i < VC; ++i)
-        if (n < a.n) S[n][i] = st[i * a.n + n];
-  }
-  if constexpr (!FULL) {
-    if (w.u.k == 0) {
-      if (on) {
-        float* e = pl.ends + (unit0 + w.last) * channels * a.n;
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-          if (n < a.n) store_f32<float, VC>(e + (int64_t)n * channels + c, S[n]);
-      }
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < VC; ++i) S[n][i] = 0.0f;
-    }
-  } else if (w.last > 0 && on) {
-    const float* e = pl.ends + (int64_t)blockIdx.x * channels * a.n;
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-      if (n < a.n) load_f32<float, VC>(S[n], e + (int64_t)n * channels + c);
-  }
-
-  float D[VC], all = 1.0f;
-#pragma unroll
-  for (int i = 0; i < VC; ++i) D[i] = FULL && on && a.D ? a.D[c + i] : 0.0f;
-  const uint32_t col = on ? (uint32_t)(c * sizeof(T)) : kNoColumn;
-  const uint32_t xs = (uint32_t)(a.xs * sizeof(T)), zs = (uint32_t)(a.zs * sizeof(T)),
-                 ys = (uint32_t)(a.ys * sizeof(T));
-  for (int t = w.t0; t < w.t1; t += tile) {
-    const int rows = min(tile, w.t1 - t);
-    const auto bx = rows_of<T>(a.x, t, a.xs, rows);
-    const auto bz = rows_of<T>(a.z, t, a.zs, FULL && a.z ? rows : 0);
-    const auto by = rows_of<T>(a.y, t, a.ys, rows);
-    for (int i = lane; i < rows * nh; i += 64) {
-      const int r = i / nh, hh = i - r * nh;
-      const int64_t row = t + r;
-      const int g = (h0 + hh) / per;
-      const float d = step_of(a, (float)((const T*)a.dt)[row * a.dts + h0 + hh],
-                              bias_of(a, h0 + hh));
-      float* s = sh + (r * heads_max + hh) * EW;
-      s[0] = exp_f32(a.A[h0 + hh] * d);
-#pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        const bool have = n < a.n;
-        s[1 + n] = have ? d * (float)((const T*)a.B)[row * a.Bs + (int64_t)g * a.n + n] : 0.0f;
-        if (FULL)
-          s[1 + NS + n] = have ? (float)((const T*)a.C)[row * a.Cs + (int64_t)g * a.n + n] : 0.0f;
-      }
-    }
-    __syncthreads();
-    for (int r0 = 0; r0 < rows; r0 += kSmallRows) {
-      Pack<T, VC> xr[kSmallRows], zr[kSmallRows];
-#pragma unroll
-      for (int r = 0; r < kSmallRows; ++r) {
-        xr[r] = load_row<T, VC>(bx, col + (r0 + r) * xs);
-        if (FULL) zr[r] = load_row<T, VC>(bz, col + (r0 + r) * zs);
-      }
-#pragma unroll
-      for (int r = 0; r < kSmallRows; ++r) {
-        if (r0 + r >= rows) break;
-        float e[EW];
-        const float4* s = (const float4*)(sh + ((r0 + r) * heads_max + (h - h0)) * EW);
-#pragma unroll
-        for (int k = 0; k < EW / 4; ++k) *(float4*)(e + 4 * k) = s[k];
-        float x[VC], y[VC];
-#pragma unroll
-        for (int i = 0; i < VC; ++i) {
-          x[i] = (float)xr[r].v[i];
-          y[i] = FULL ? D[i] * x[i] : 0.0f;
-        }
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-          for (int i = 0; i < VC; ++i) {
-            S[n][i] = __builtin_fmaf(S[n][i], e[0], x[i] * e[1 + n]);
-            // a value beyond d_state stays zero even where the decay is infinite
-            if (NS > 2) S[n][i] = n < a.n ? S[n][i] : 0.0f;
-            if (FULL) y[i] = __builtin_fmaf(S[n][i], e[1 + NS + n], y[i]);
-          }
-        all *= e[0];
-        if (FULL) {
-          if (a.z)
-#pragma unroll
-            for (int i = 0; i < VC; ++i) y[i] *= silu_f32((float)zr[r].v[i]);
-          store_row<T, VC>(by, col + (r0 + r) * ys, y);
-        }
-      }
-    }
-    __syncthreads();
-  }
-  if (!on) return;
-  if constexpr (!FULL) {
-    float* e = pl.ends + (int64_t)blockIdx.x * channels * a.n;
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-      if (n < a.n) store_f32<float, VC>(e + (int64_t)n * channels + c, S[n]);
-    if (c % a.hd == 0) pl.decays[(int64_t)blockIdx.x * a.heads + h] = all;
-  } else if (w.slot >= 0 && w.u.k == w.last) {
-    float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int i = 0; i < VC; ++i)
-        if (n < a.n) st[i * a.n + n] = S[n][i];
-  }
-}
-
-template <typename T, int NS, int VC>
-static hipError_t launch_small(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
-  const int span = 64 * VC, channels = a.heads * a.hd;
-  const int by = (channels + span - 1) / span;
-  const int hm = (span + a.hd - 2) / a.hd + 1;
-  const int heads_max = hm < a.heads ? hm : a.heads;
-  // rows per tile: 32, or what fits 32 KB (a row is at most 64 heads of 80 bytes)
-  const int row = heads_max * small_entry(NS) * 4;
-  int tile = 32;
-  while (tile * row > 32768) tile /= 2;
-  if (pl.split) {
-    hipLaunchKernelGGL((k_scan_small<T, NS, VC, false>), dim3((unsigned)pl.units, by), dim3(64),
-                       tile * row, s, a, pl, tile, heads_max);
-    launch_join<1>(a, pl, (int64_t)channels * a.n, a.hd, s);
-  }
-  hipLaunchKernelGGL((k_scan_small<T, NS, VC, true>), dim3((unsigned)pl.units, by), dim3(64),
-                     tile * row, s, a, pl, tile, heads_max);
-  return hipGetLastError();
-}
-
-template <typename T, int VC>
-static hipError_t launch_small_n(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
-  if (a.n == 1) return launch_small<T, 1, VC>(a, pl, s);
-  if (a.n == 2) return launch_small<T, 2, VC>(a, pl, s);
-  if (a.n <= 4) return launch_small<T, 4, VC>(a, pl, s);
-  return launch_small<T, 8, VC>(a, pl, s);
 }
 
 // ---- more state values: chunks of kQ rows on the matrix cores --------------
@@ -1015,7 +1059,7 @@ static hipError_t launch_mm_t(const SsmArgs& a, const ScanPlan& pl, hipStream_t 
 // them: a little less than the 2048 that the second pass's registers let it
 // hold, since one workgroup that finds no place doubles the whole time), but no shorter than what the first pass and the walk over a
 // sequence's units are worth, and no more than 32 (64) of them in a sequence.
-constexpr int kFillWaves = 1920;
+constexpr int kFillWaves = 1920, kSmallFillWaves = 2048;
 
 static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
   ScanPlan pl{};
@@ -1025,7 +1069,8 @@ static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
                               : (int64_t)op->n_heads * mm_ptiles(op->head_dim);
   const int step = small ? 32 : kQ, least = small ? 32 : 4 * kQ, most_units = small ? 64 : 32;
   const int64_t T = op->n_tokens;
-  const int64_t want = kFillWaves / waves > 1 ? kFillWaves / waves : 1;
+  const int64_t fill = small ? kSmallFillWaves : kFillWaves;
+  const int64_t want = fill / waves > 1 ? fill / waves : 1;
   int64_t len = ((T + want - 1) / want + step - 1) / step * step;
   const int64_t floor_len = ((T + most_units - 1) / most_units + step - 1) / step * step;
   if (len > 512 && op->n_seqs > 1) len = 512;  // uneven lengths: the longest is cut too
