@@ -14,6 +14,8 @@
 namespace bm {
 
 constexpr int kConvRows = 32;  // rows per unit
+constexpr int kConvBatch = 8;  // rows loaded together
+constexpr int kConvSeqs = 4;   // single tokens per thread where there are many
 
 template <int W, int V>
 struct Taps {
@@ -21,12 +23,11 @@ struct Taps {
   bool silu;
   __device__ __forceinline__ Taps(const float* wp, const float* bp, int channels, int c, bool act)
       : silu(act) {
+    const auto rw = rows_at(wp, (uint32_t)(W * channels * 4));
+    const auto rb = rows_at(bp, bp ? (uint32_t)(channels * 4) : 0);  // none: zeros
 #pragma unroll
-    for (int k = 0; k < W; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[k][i] = wp[(size_t)k * channels + c + i];
-#pragma unroll
-    for (int i = 0; i < V; ++i) b[i] = bp ? bp[c + i] : 0.0f;
+    for (int k = 0; k < W; ++k) load_floats<V>(w[k], rw, (uint32_t)((k * channels + c) * 4));
+    load_floats<V>(b, rb, (uint32_t)(c * 4));
   }
   // win: the W - 1 rows before x; moves x into it
   __device__ __forceinline__ void push(float (&win)[W - 1][V], const float (&x)[V],
@@ -36,12 +37,14 @@ struct Taps {
       float a = b[i];
 #pragma unroll
       for (int k = 0; k < W - 1; ++k) a = __builtin_fmaf(win[k][i], w[k][i], a);
-      a = __builtin_fmaf(x[i], w[W - 1][i], a);
-      y[i] = silu ? silu_f32(a) : a;
+      y[i] = __builtin_fmaf(x[i], w[W - 1][i], a);
 #pragma unroll
       for (int k = 0; k + 1 < W - 1; ++k) win[k][i] = win[k + 1][i];
       win[W - 2][i] = x[i];
     }
+    if (silu)
+#pragma unroll
+      for (int i = 0; i < V; ++i) y[i] = silu_f32(y[i]);
   }
 };
 
@@ -56,106 +59,139 @@ struct ConvArgs {
   int64_t ss;
   void* y;
   int64_t ys;
+  // the slot's rows; without one nothing is read (zeros) or written
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t slot_rows(int slot, int rows) const {
+    return rows_at(state + (slot >= 0 ? (int64_t)slot * ss : 0),
+                   slot >= 0 ? (uint32_t)(rows * channels * 4) : 0);
+  }
 };
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(float (&o)[V], const Pack<T, V>& p) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = (float)p.v[i];
+}
 
 template <typename T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
+  const int c = (blockIdx.y * 256 + threadIdx.x) * V;
   const int slots = first_slots(a.q);
   const Unit u = find_unit(a.q, blockIdx.x, kConvRows);
   if (u.b < 0) return;
-  const int t0 = u.s + u.k * kConvRows, t1 = min(u.e, t0 + kConvRows);
+  const int t0 = u.s + u.k * kConvRows, t1 = u.e - t0 < kConvRows ? u.e : t0 + kConvRows;
   if (u.k > 0 && t0 >= t1) return;
   const int slot = find_slot(a.q, u.b, slots);
-  if (slot == kNoSlot) return;
-  const int c = (blockIdx.y * 256 + threadIdx.x) * V;
-  if (c >= a.channels) return;
-  const T* x = (const T*)a.x + c;
-  T* y = (T*)a.y + c;
-  float win[W - 1][V];
-  if (u.k > 0) {
+  if (slot == kNoSlot || c >= a.channels) return;
+  const uint32_t col = (uint32_t)(c * sizeof(T)), xs = (uint32_t)(a.xs * sizeof(T)),
+                 ys = (uint32_t)(a.ys * sizeof(T)), row = (uint32_t)(a.channels * 4);
+  const int rows = t1 - t0;
+  const auto bx = rows_of<T>(a.x, t0, a.xs, rows);
+  const auto by = rows_of<T>(a.y, t0, a.ys, rows);
+  Pack<T, V> next[kConvBatch];
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k)
-      load_f32<T, V>(win[k], x + (int64_t)(t0 - (W - 1) + k) * a.xs);
+  for (int j = 0; j < kConvBatch; ++j) next[j] = load_row<T, V>(bx, col + j * xs);
+
+  float win[W - 1][V], old[W - 1][V];
+  Pack<T, V> end[W - 1];
+  const auto st = a.slot_rows(slot, W - 1);
+  if (u.k > 0) {
+    const auto bw = rows_of<T>(a.x, t0 - (W - 1), a.xs, W - 1);
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) unpack(win[k], load_row<T, V>(bw, col + k * xs));
   } else {
     // the sequence's first unit also replaces the state: the same thread has
     // read the old rows before it writes the new ones
-    float* st = slot >= 0 ? a.state + (int64_t)slot * a.ss + c : nullptr;
     const bool keep = slot >= 0 && !(a.q.fresh && a.q.fresh[u.b]);
+    const int n = u.e - u.s;
+    const auto be = rows_of<T>(a.x, u.e - min(n, W - 1), a.xs, min(n, W - 1));
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+      load_floats<V>(old[k], st, keep ? (uint32_t)(c * 4) + k * row : kNoColumn);
+      const int back = n - (W - 1) < 0 ? n - (W - 1) : 0;  // rows that the old state keeps
+      end[k] = load_row<T, V>(be, k + back >= 0 ? col + (k + back) * xs : kNoColumn);
+    }
 #pragma unroll
     for (int k = 0; k < W - 1; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[k][i] = keep ? st[(size_t)k * a.channels + i] : 0.0f;
-    if (st) {
-      const int n = u.e - u.s;
-#pragma unroll
-      for (int k = 0; k < W - 1; ++k) {
-        const int pos = n - (W - 1) + k;  // of the new row; negative: an old one
-        float r[V];
-        if (pos >= 0) {
-          load_f32<T, V>(r, x + (int64_t)(u.s + pos) * a.xs);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            r[i] = 0.0f;
-#pragma unroll
-            for (int o = 0; o < W - 1; ++o) r[i] = o == W - 1 + pos ? win[o][i] : r[i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) st[(size_t)k * a.channels + i] = r[i];
-      }
-    }
+      for (int i = 0; i < V; ++i) win[k][i] = old[k][i];
   }
   const Taps<W, V> taps(a.w, a.bias, a.channels, c, a.silu);
-  int t = t0;
-  for (; t + 8 <= t1; t += 8) {
-    float r[8][V], o[V];
+  for (int t = 0; t < rows; t += kConvBatch) {
+    Pack<T, V> now[kConvBatch];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) load_f32<T, V>(r[j], x + (int64_t)(t + j) * a.xs);
+    for (int j = 0; j < kConvBatch; ++j) now[j] = next[j];
+    if (t + kConvBatch < rows)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      taps.push(win, r[j], o);
-      store_f32<T, V>(y + (int64_t)(t + j) * a.ys, o);
+      for (int j = 0; j < kConvBatch; ++j)
+        next[j] = load_row<T, V>(bx, col + (t + kConvBatch + j) * xs);
+#pragma unroll
+    for (int j = 0; j < kConvBatch; ++j) {
+      float x[V], o[V];
+      unpack(x, now[j]);
+      taps.push(win, x, o);
+      store_row<T, V>(by, col + (t + j) * ys, o);
     }
   }
-  for (; t < t1; ++t) {
-    float r[V], o[V];
-    load_f32<T, V>(r, x + (int64_t)t * a.xs);
-    taps.push(win, r, o);
-    store_f32<T, V>(y + (int64_t)t * a.ys, o);
+  if (u.k == 0) {
+    const int n = u.e - u.s;
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+      float r[V];
+      unpack(r, end[k]);
+      // with fewer than W - 1 rows the first of the new state are old ones
+#pragma unroll
+      for (int o = k; o < W - 1; ++o)
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] = n + k == o ? old[o][i] : r[i];
+      store_floats<V>(st, (uint32_t)(c * 4) + k * row, r);
+    }
   }
 }
 
 // One token of each sequence: bound by its state rows, read and written; at
-// few sequences by one launch and the round trips slot -> rows.
-template <typename T, int W, int V>
+// few sequences by one launch and the round trips slot -> rows.  A thread
+// takes SEQS sequences, so that its taps are loaded once for them.
+template <typename T, int W, int V, int SEQS>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs a) {
-  const int b = blockIdx.x;
   const int c = (blockIdx.y * 256 + threadIdx.x) * V;
-  const int slot = find_slot(a.q, b, first_slots(a.q));
-  if (slot == kNoSlot || c >= a.channels) return;
+  const int first = first_slots(a.q);
+  const uint32_t row = (uint32_t)(a.channels * 4), col = c < a.channels ? (uint32_t)(c * 4) : kNoColumn;
+  const uint32_t at = c < a.channels ? (uint32_t)(c * sizeof(T)) : kNoColumn;
+  int slot[SEQS];
+  float win[SEQS][W - 1][V];
+  Pack<T, V> x[SEQS];
+#pragma unroll
+  for (int q = 0; q < SEQS; ++q) {
+    const int b = blockIdx.x * SEQS + q;
+    slot[q] = b < a.q.n_seqs ? find_slot(a.q, b, first) : kNoSlot;
+    const auto st = a.slot_rows(slot[q], W - 1);
+    x[q] = load_row<T, V>(rows_of<T>(a.x, b, a.xs, slot[q] != kNoSlot), at);
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) load_floats<V>(win[q][k], st, col + k * row);
+  }
+  if (c >= a.channels) return;
   const Taps<W, V> taps(a.w, a.bias, a.channels, c, a.silu);
-  float r[V], o[V], win[W - 1][V];
-  load_f32<T, V>(r, (const T*)a.x + (int64_t)b * a.xs + c);
-  float* st = slot >= 0 ? a.state + (int64_t)slot * a.ss + c : nullptr;
 #pragma unroll
-  for (int k = 0; k < W - 1; ++k)
+  for (int q = 0; q < SEQS; ++q) {
+    const int b = blockIdx.x * SEQS + q;
+    float r[V], o[V];
+    unpack(r, x[q]);
+    taps.push(win[q], r, o);
+    const auto st = a.slot_rows(slot[q], W - 1);
 #pragma unroll
-    for (int i = 0; i < V; ++i) win[k][i] = st ? st[(size_t)k * a.channels + i] : 0.0f;
-  taps.push(win, r, o);
-  if (st)
-#pragma unroll
-    for (int k = 0; k < W - 1; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) st[(size_t)k * a.channels + i] = win[k][i];
-  store_f32<T, V>((T*)a.y + (int64_t)b * a.ys + c, o);
+    for (int k = 0; k < W - 1; ++k) store_floats<V>(st, col + k * row, win[q][k]);
+    store_row<T, V>(rows_of<T>(a.y, b, a.ys, slot[q] != kNoSlot), at, o);
+  }
 }
 
 template <typename T, int W, int V>
 static hipError_t launch_conv(const ConvArgs& a, bool step, hipStream_t s) {
   const unsigned gy = (unsigned)((a.channels + 256 * V - 1) / (256 * V));
-  if (step)
-    hipLaunchKernelGGL((k_conv_step<T, W, V>), dim3(a.q.n_seqs, gy), dim3(256), 0, s, a);
+  if (step && (int64_t)a.q.n_seqs * gy >= 1024)  // one thread's work for four still fills the chip
+    hipLaunchKernelGGL((k_conv_step<T, W, V, kConvSeqs>),
+                       dim3((a.q.n_seqs + kConvSeqs - 1) / kConvSeqs, gy), dim3(256), 0, s, a);
+  else if (step)
+    hipLaunchKernelGGL((k_conv_step<T, W, V, 1>), dim3(a.q.n_seqs, gy), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((k_conv<T, W, V>),
                        dim3((unsigned)unit_count(a.q.n_seqs, a.q.n_tokens, kConvRows), gy),

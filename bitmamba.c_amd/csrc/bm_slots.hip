@@ -24,8 +24,8 @@ __device__ __forceinline__ uint8_t zero_of(const uint8_t*) { return 0; }
 // say, in one pass and without a second buffer.
 //
 // Several pairs with one dst: the first that moves anything counts.  The
-// block finds it in a hash table of the destinations in LDS (at most 1024 of
-// 2048 places taken).
+// block finds it in a hash table of the destinations in LDS (at most half of
+// its places taken).
 // ---------------------------------------------------------------------------
 constexpr int kHash = 2 * kMaxPairs;
 
@@ -33,58 +33,61 @@ template <typename W, int E>
 __global__ __launch_bounds__(256) void k_slots_copy(PoolView pool, int n_slots,
                                                     const int32_t* __restrict__ src,
                                                     const int32_t* __restrict__ dst, int n,
-                                                    int log_cols) {
-  __shared__ int key[kHash], first[kHash], from[kMaxPairs];
-  const int tid = threadIdx.x;
-  for (int i = tid; i < kHash; i += 256) {
+                                                    int log_cols, int log_hash) {
+  __shared__ int key[kHash], first[kHash], from[kMaxPairs], into[kMaxPairs];
+  const int tid = threadIdx.x, places = 1 << log_hash;
+  for (int i = tid; i < places; i += 256) {
     key[i] = -1;
     first[i] = kMaxPairs;
   }
   __syncthreads();
-  auto place = [](int d) { return (int)(((uint32_t)d * 2654435761u) >> 21); };  // 11 bits
   for (int i = tid; i < n; i += 256) {
     const int s = src[i], d = dst[i];
     const bool moves = s >= -1 && s < n_slots && d >= 0 && d < n_slots;
-    from[i] = moves ? d : -1;
+    from[i] = s;
+    into[i] = -1;
     if (!moves) continue;
-    int at = place(d);
-    for (int tries = 0; tries < kHash; ++tries) {  // at most n places are taken
+    int at = (int)(((uint32_t)d * 2654435761u) >> (32 - log_hash));
+    for (int tries = 0; tries < places; ++tries) {  // at most n places are taken
       const int was = atomicCAS(&key[at], -1, d);
       if (was == -1 || was == d) break;
-      at = (at + 1) & (kHash - 1);
+      at = (at + 1) & (places - 1);
     }
     atomicMin(&first[at], i);
   }
+  __syncthreads();
+  for (int i = tid; i < places; i += 256)
+    if (key[i] >= 0) into[first[i]] = key[i];
   __syncthreads();
 
   const int64_t words = pool.slot_bytes / (int64_t)sizeof(W);
   const int64_t col0 = (int64_t)blockIdx.x << log_cols;
   uint8_t* layer = pool.base + (int64_t)blockIdx.y * pool.layer_stride;
   W v[E];
-  W* to[E];
+  int to[E];
+  const int64_t col = col0 + (tid & ((1 << log_cols) - 1));  // 256 is a multiple of the columns,
+  const int first_pair = tid >> log_cols;                     // or one pair has them all
+  const bool many = log_cols > 8;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int item = tid + 256 * e;
-    const int i = item >> log_cols;
-    const int64_t col = col0 + (item & ((1 << log_cols) - 1));
-    to[e] = nullptr;
-    if (i >= n || col >= words) continue;
-    const int d = from[i];
-    if (d < 0) continue;
-    int at = place(d);
-    for (int tries = 0; tries < kHash && key[at] != d; ++tries) at = (at + 1) & (kHash - 1);
-    if (first[at] != i) continue;
-    to[e] = (W*)(layer + (int64_t)d * pool.slot_stride) + col;
-    const int s = src[i];
+    const int i = many ? item >> log_cols : first_pair + (e << (8 - log_cols));
+    const int64_t at = many ? col0 + (item & ((1 << log_cols) - 1)) : col;
+    to[e] = i < n && at < words ? into[i] : -1;
+    if (to[e] < 0) continue;
+    const int s = from[i];
     v[e] = s < 0 ? zero_of((const W*)nullptr)
-                 : ((const W*)(layer + (int64_t)s * pool.slot_stride))[col];
+                 : ((const W*)(layer + (int64_t)s * pool.slot_stride))[at];
   }
   // every load of the block has returned before its first store
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (to[e]) *to[e] = v[e];
+  for (int e = 0; e < E; ++e) {
+    if (to[e] < 0) continue;
+    const int64_t at = many ? col0 + ((tid + 256 * e) & ((1 << log_cols) - 1)) : col;
+    ((W*)(layer + (int64_t)to[e] * pool.slot_stride))[at] = v[e];
+  }
 }
 
 template <typename W, int E>
@@ -92,19 +95,27 @@ static hipError_t launch_copy_e(const PoolView& p, int n_layers, int n_slots, co
                                 const int32_t* dst, int n, hipStream_t s) {
   // the columns of a block: a power of two, all pairs' words in its registers
   const int64_t words = p.slot_bytes / (int64_t)sizeof(W);
-  int lc = 0;
+  int lc = 0, lh = 6;
   while ((2 << lc) * n <= 256 * E && ((int64_t)1 << lc) < words) ++lc;
+  while ((1 << lh) < 2 * n) ++lh;
   const int64_t blocks = (words + ((int64_t)1 << lc) - 1) >> lc;
   if (blocks > 0x7fffffff) return hipErrorInvalidValue;
   hipLaunchKernelGGL((k_slots_copy<W, E>), dim3((unsigned)blocks, n_layers), dim3(256), 0, s, p,
-                     n_slots, src, dst, n, lc);
+                     n_slots, src, dst, n, lc, lh);
   return hipGetLastError();
 }
 
+// Words per thread: as many as leave the chip at least two workgroups per CU,
+// since each of them works the lists out for itself.
 template <typename W>
 static hipError_t launch_copy_w(const PoolView& p, int n_layers, int n_slots, const int32_t* src,
                                 const int32_t* dst, int n, hipStream_t s) {
-  return launch_copy_e<W, 16>(p, n_layers, n_slots, src, dst, n, s);
+  const int64_t items = p.slot_bytes / (int64_t)sizeof(W) * n * n_layers;
+  if (n > 512 || items >= 512 * 256 * 16)
+    return launch_copy_e<W, 16>(p, n_layers, n_slots, src, dst, n, s);
+  if (n > 128 || items >= 512 * 256 * 4)
+    return launch_copy_e<W, 4>(p, n_layers, n_slots, src, dst, n, s);
+  return launch_copy_e<W, 1>(p, n_layers, n_slots, src, dst, n, s);
 }
 
 // the widest word that every slot's start and size fit

@@ -62,62 +62,71 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs a) {
   const int g = h / (a.heads / a.groups);
   const float d = step_of(a, (float)((const T*)a.dt)[(int64_t)b * a.dts + h], bias_of(a, h));
   const float decay = exp_f32(a.A[h] * d);
-  float* st = slot >= 0 ? a.state + (int64_t)slot * a.ss + (int64_t)h * a.hd * a.n : nullptr;
-  const T* Bp = (const T*)a.B + (int64_t)b * a.Bs + (int64_t)g * a.n;
-  const T* Cp = (const T*)a.C + (int64_t)b * a.Cs + (int64_t)g * a.n;
-  const T* xp = (const T*)a.x + (int64_t)b * a.xs + (int64_t)h * a.hd;
-  float s[U][E][V], x[U], Bv[E][V], Cv[E][V];
+  // the head's part of the slot, of x, z and y; what lies past them reads as
+  // zeros and is not written
+  const auto st = rows_at(a.state + (slot >= 0 ? (int64_t)slot * a.ss : 0) + (int64_t)h * a.hd * a.n,
+                          slot >= 0 ? (uint32_t)(a.hd * a.n * 4) : 0);
+  const uint32_t head = (uint32_t)(a.hd * sizeof(T));
+  const auto bx = rows_at((const T*)a.x + (int64_t)b * a.xs + (int64_t)h * a.hd, head);
+  const auto bz = rows_at((const T*)a.z + (int64_t)b * a.zs + (int64_t)h * a.hd, a.z ? head : 0);
+  const auto by = rows_at((const T*)a.y + (int64_t)b * a.ys + (int64_t)h * a.hd, head);
+  const auto bD = rows_at(a.D + (int64_t)h * a.hd, a.D ? (uint32_t)(a.hd * 4) : 0);
+  const uint32_t gn = (uint32_t)(a.n * sizeof(T));
+  const auto bB = rows_at((const T*)a.B + (int64_t)b * a.Bs + (int64_t)g * a.n, gn);
+  const auto bC = rows_at((const T*)a.C + (int64_t)b * a.Cs + (int64_t)g * a.n, gn);
+  float s[U][E][V], Bv[E][V], Cv[E][V];
+  uint32_t x[U], z[U];
+  float D[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int p = p0 + u * kRows;
-    x[u] = p < a.hd ? (float)xp[p] : 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int n = nl + e * TEAM * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[u][e][i] = 0.0f;
-      if (st && p < a.hd && n < a.n) load_f32<float, V>(s[u][e], st + (int64_t)p * a.n + n);
+      load_floats<V>(s[u][e], st, n < a.n ? (uint32_t)((p * a.n + n) * 4) : kNoColumn);
     }
+    x[u] = load_raw<T>(bx, (uint32_t)(p * sizeof(T)));
+    z[u] = load_raw<T>(bz, (uint32_t)(p * sizeof(T)));
+    D[u] = __uint_as_float(load_raw<float>(bD, (uint32_t)(p * 4)));
   }
 #pragma unroll
   for (int e = 0; e < E; ++e)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = nl + e * TEAM * V + i;
-      Bv[e][i] = n < a.n ? d * (float)Bp[n] : 0.0f;
-      Cv[e][i] = n < a.n ? (float)Cp[n] : 0.0f;
+      const uint32_t n = (uint32_t)((nl + e * TEAM * V + i) * sizeof(T));
+      Bv[e][i] = d * raw_f32<T>(load_raw<T>(bB, n));
+      Cv[e][i] = raw_f32<T>(load_raw<T>(bC, n));
+      // beyond d_state: zeros, whatever d is
+      if (n >= gn) Bv[e][i] = 0.0f;
     }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int p = p0 + u * kRows;
+    const float xf = raw_f32<T>(x[u]);
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
+    for (int e = 0; e < E; ++e) {
+      const int n = nl + e * TEAM * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[u][e][i] = __builtin_fmaf(s[u][e][i], decay, x[u] * Bv[e][i]);
+        s[u][e][i] = __builtin_fmaf(s[u][e][i], decay, xf * Bv[e][i]);
+        // beyond d_state nothing counts, even where x or the decay is infinite
+        if (E * TEAM * V > 1 && (V == 1 || E > 1)) s[u][e][i] = n + i < a.n ? s[u][e][i] : 0.0f;
         sum = __builtin_fmaf(s[u][e][i], Cv[e][i], sum);
       }
-    sum = team_sum<TEAM>(sum);
-    if (p < a.hd) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int n = nl + e * TEAM * V;
-        if (st && n < a.n) store_f32<float, V>(st + (int64_t)p * a.n + n, s[u][e]);
-      }
-      if (lane % TEAM == 0) {
-        const int64_t c = (int64_t)h * a.hd + p;
-        if (a.D) sum = __builtin_fmaf(a.D[c], x[u], sum);
-        if (a.z) sum *= silu_f32((float)((const T*)a.z)[(int64_t)b * a.zs + c]);
-        ((T*)a.y)[(int64_t)b * a.ys + c] = (T)sum;
-      }
+      if (V > 1) sum = n < a.n ? sum : 0.0f;
+      store_floats<V>(st, n < a.n ? (uint32_t)((p * a.n + n) * 4) : kNoColumn, s[u][e]);
     }
+    sum = __builtin_fmaf(D[u], xf, team_sum<TEAM>(sum));
+    if (a.z) sum *= silu_f32(raw_f32<T>(z[u]));
+    const float out[1] = {sum};
+    store_row<T, 1>(by, lane % TEAM == 0 ? (uint32_t)(p * sizeof(T)) : kNoColumn, out);
   }
 }
 
 template <typename T, int TEAM, int V, int E>
 static hipError_t launch_step(const SsmArgs& a, hipStream_t s) {
-  constexpr int U = TEAM >= 4 ? 4 : 1;
+  constexpr int U = TEAM >= 16 ? 8 : (TEAM >= 4 ? 4 : 1);
   constexpr int kRows = 64 / TEAM * U;  // channels per wave
   const int waves = (a.hd + kRows - 1) / kRows;
   const int nw = waves < 4 ? waves : 4;
@@ -128,7 +137,7 @@ static hipError_t launch_step(const SsmArgs& a, hipStream_t s) {
 
 template <typename T>
 static hipError_t launch_step_t(const SsmArgs& a, hipStream_t s) {
-  if (a.n % 4 == 0 && a.ss % 4 == 0 && (uintptr_t)a.state % 16 == 0) {
+  if (a.n % 4 == 0) {  // a row's loads of four floats need no more than a float's alignment
     if (a.n <= 4) return launch_step<T, 1, 4, 1>(a, s);
     if (a.n <= 8) return launch_step<T, 2, 4, 1>(a, s);
     if (a.n <= 16) return launch_step<T, 4, 4, 1>(a, s);
