@@ -13,7 +13,7 @@
 
 namespace bm {
 
-constexpr int kConvRows = 32;  // rows per unit
+constexpr int kConvRows = 16;  // rows per unit
 constexpr int kConvBatch = 8;  // rows loaded together
 constexpr int kConvSeqs = 4;   // single tokens per thread where there are many
 

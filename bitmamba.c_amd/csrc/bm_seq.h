@@ -118,32 +118,35 @@ __device__ __forceinline__ void store_row(__amdgpu_buffer_rsrc_t r, uint32_t off
   }
 }
 
-// V neighbouring floats (1, 4 or 8) on a multiple of 4 bytes
-template <int V>
+// V neighbouring floats (1, 4 or 8) on a multiple of 4 bytes; STREAM: past the caches, for what is
+// read and written once and does not fit them
+template <int V, bool STREAM = false>
 __device__ __forceinline__ void load_floats(float (&o)[V], __amdgpu_buffer_rsrc_t r, uint32_t off) {
+  constexpr int kAux = STREAM ? 2 : 0;  // the nt bit
   if constexpr (V == 1) {
-    o[0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    o[0] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kAux));
   } else {
 #pragma unroll
     for (int k = 0; k < V; k += 4) {
-      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * k, 0, 0);
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * k, 0, kAux);
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[k + i] = __uint_as_float(v[i]);
     }
   }
 }
-template <int V>
+template <int V, bool STREAM = false>
 __device__ __forceinline__ void store_floats(__amdgpu_buffer_rsrc_t r, uint32_t off,
                                              const float (&o)[V]) {
+  constexpr int kAux = STREAM ? 2 : 0;
   if constexpr (V == 1) {
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[0]), r, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[0]), r, off, 0, kAux);
   } else {
 #pragma unroll
     for (int k = 0; k < V; k += 4) {
       u32x4 v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(o[k + i]);
-      __builtin_amdgcn_raw_buffer_store_b128(v, r, off + 4 * k, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(v, r, off + 4 * k, 0, kAux);
     }
   }
 }
