@@ -743,13 +743,13 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
   };
   auto fetch = [&](int t) {
     const int rows = min(kQ, w.t1 - t);
+    const auto bdt = rows_of<T>(a.dt, t, a.dts, rows);
+    ndt = load_raw<T>(bdt, li * (uint32_t)(a.dts * sizeof(T)) + h * (uint32_t)sizeof(T));
     if (wide)
       fetch_bc(t, [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
         return load_raw4<T>(r, n < a.n ? off : kNoColumn);
       });
     if (!FULL) fetch_x(t);
-    const auto bdt = rows_of<T>(a.dt, t, a.dts, rows);
-    ndt = load_raw<T>(bdt, li * (uint32_t)(a.dts * sizeof(T)) + h * (uint32_t)sizeof(T));
   };
   // value by value, where four do not lie on one load's alignment: not ahead
   auto fetch_narrow = [&](int t) {
@@ -790,7 +790,32 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
     put(shT + n * L::kRowT + place(j) * 2, L::kRowT, L::kPieceT, b, true);
   };
 
-  if (w.t0 < w.t1) fetch(w.t0);
+  // A chunk's exponents, by lane li (both halves alike), and what is made of
+  // them, in the wave's own part of LDS; out of dt fetched before.  Done ahead
+  // of the chunk, in the shadow of the products before it.
+  float eall = 1.0f;
+  auto exponents = [&](int rows) {
+    const float d = li < rows ? step_of(a, raw_f32<T>(ndt), bias) : 0.0f;
+    double cum = (double)A * (double)d * 1.4426950408889634;
+    cum = cum < -256.0 ? -256.0 : (cum > 256.0 ? 256.0 : cum);
+    cum = half_scan(cum);
+    const double whole = lane_f64(cum, kQ - 1);
+    total += whole;
+    eall = __builtin_amdgcn_exp2f((float)whole);
+    if (half == 0) {
+      const float hi = (float)cum;
+      shHi[li] = hi;
+      shLo[li] = (float)(cum - (double)hi);
+      shD[li] = d;
+      shE[li] = __builtin_amdgcn_exp2f(hi);
+      shW[li] = __builtin_amdgcn_exp2f((float)(whole - cum)) * d;
+    }
+  };
+
+  if (w.t0 < w.t1) {
+    fetch(w.t0);
+    exponents(min(kQ, w.t1 - w.t0));
+  }
   for (int t = w.t0; t < w.t1; t += kQ) {
     const int rows = min(kQ, w.t1 - t);
     // B and C into LDS
@@ -817,22 +842,6 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
     if (!FULL)
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = raw_f32<T>(nx[r]);
-    // the chunk's exponents, by lane li (both halves alike)
-    const float d = li < rows ? step_of(a, raw_f32<T>(ndt), bias) : 0.0f;
-    double cum = (double)A * (double)d * 1.4426950408889634;
-    cum = cum < -256.0 ? -256.0 : (cum > 256.0 ? 256.0 : cum);
-    cum = half_scan(cum);
-    const double whole = lane_f64(cum, kQ - 1);
-    total += whole;
-    float eall = __builtin_amdgcn_exp2f((float)whole);
-    if (half == 0) {
-      const float hi = (float)cum;
-      shHi[li] = hi;
-      shLo[li] = (float)(cum - (double)hi);
-      shD[li] = d;
-      shE[li] = __builtin_amdgcn_exp2f(hi);
-      shW[li] = __builtin_amdgcn_exp2f((float)(whole - cum)) * d;
-    }
     uint32_t z[16];
     if (FULL) {
       fetch_x(t);
@@ -1003,6 +1012,7 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
           S[nt] = mfma32<kStatePieces>(pb, xw[s], S[nt]);
         }
       }
+      if (t + kQ < w.t1) exponents(min(kQ, w.t1 - t - kQ));
     }
     __syncthreads();  // the next chunk may overwrite LDS
   }
