@@ -78,8 +78,8 @@ __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
   const int slots = first_slots(a.q);
   const Unit u = find_unit(a.q, blockIdx.x, kConvRows);
   if (u.b < 0) return;
+  if (u.k > (u.e > u.s ? (u.e - u.s - 1) / kConvRows : 0)) return;  // past its rows
   const int t0 = u.s + u.k * kConvRows, t1 = u.e - t0 < kConvRows ? u.e : t0 + kConvRows;
-  if (u.k > 0 && t0 >= t1) return;
   const int slot = find_slot(a.q, u.b, slots);
   if (slot == kNoSlot || c >= a.channels) return;
   const uint32_t col = (uint32_t)(c * sizeof(T)), xs = (uint32_t)(a.xs * sizeof(T)),

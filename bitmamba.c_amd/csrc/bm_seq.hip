@@ -40,8 +40,8 @@ bool check_apart(const char* op, const char* name, const void* p, int64_t stride
 bool check_seqs(const char* op, int n_seqs, int n_tokens, const int32_t* seq_start,
                 const int32_t* slots, const float* state, int64_t state_stride, int n_slots,
                 int64_t slot_floats, bool step) {
-  if (n_seqs < 0 || (!step && n_tokens < 0)) {
-    bm_set_error("%s: n_seqs=%d n_tokens=%d", op, n_seqs, n_tokens);
+  if (n_seqs < 0 || n_seqs > (1 << 20) || (!step && (n_tokens < 0 || n_tokens >= (1 << 30)))) {
+    bm_set_error("%s: n_seqs=%d n_tokens=%d (up to 2^20 and below 2^30)", op, n_seqs, n_tokens);
     return false;
   }
   if (!step && !seq_start && n_seqs > 1) {

@@ -181,6 +181,8 @@ struct ScanPlan {
   int len;         // rows per unit
   int64_t units;
   bool split;      // a sequence may have more than one unit
+  bool by_rows;    // where a sequence's units lie in the workspace (ScanUnit)
+  bool fits;       // a grid
   float* ends;
   float* decays;
 };
@@ -190,16 +192,22 @@ struct ScanUnit {
   int slot, t0, t1;
   int last;       // the sequence's last unit, counted from u.k's unit 0
   bool keep;      // starts from its slot's state
+  // The place of the sequence's unit 0 in the workspace: its unit's index, or
+  // 2 row / len.  The second leaves a sequence of two or more units the places
+  // up to its end's, which are at least as many, and needs none for the others.
+  int64_t place0;
 };
 // false: nothing to do (no such unit, or padding)
-__device__ __forceinline__ bool scan_unit(const SeqView& q, int index, int len, ScanUnit& w) {
-  const int slots = first_slots(q);
+__device__ __forceinline__ bool scan_unit(const SeqView& q, int index, const ScanPlan& pl,
+                                          ScanUnit& w) {
+  const int len = pl.len, slots = first_slots(q);
   w.u = find_unit(q, index, len);
   if (w.u.b < 0) return false;
   w.t0 = w.u.s + w.u.k * len;
   w.last = w.u.e > w.u.s ? (w.u.e - w.u.s - 1) / len : 0;
   if (w.u.k > w.last) return false;
   w.t1 = w.u.e - w.t0 < len ? w.u.e : w.t0 + len;
+  w.place0 = pl.by_rows ? 2 * (int64_t)(w.u.s / len) : (int64_t)index - w.u.k;
   w.slot = find_slot(q, w.u.b, slots);
   w.keep = w.slot >= 0 && !(q.fresh && q.fresh[w.u.b]);
   return w.slot != kNoSlot;
@@ -222,7 +230,7 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
   extern __shared__ float4 sh4[];
   float* sh = (float*)sh4;  // [tile][heads_max][EW]
   ScanUnit w;
-  if (!scan_unit(a.q, blockIdx.x, pl.len, w)) return;
+  if (!scan_unit(a.q, blockIdx.x, pl, w)) return;
   if (!FULL && w.u.k == w.last) return;
   const int lane = threadIdx.x, channels = a.heads * a.hd;
   const int c0 = blockIdx.y * 64 * VC;
@@ -233,7 +241,7 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
   const int nh = h1 - h0 + 1;
   const int h = on ? c / a.hd : h0;
   const int per = a.heads / a.groups;
-  const int64_t unit0 = (int64_t)blockIdx.x - w.u.k;
+  const int64_t unit0 = w.place0, unit = unit0 + w.u.k;
   const int64_t unit_floats = (int64_t)channels * a.n;
 
   const uint32_t col = on ? (uint32_t)(c * sizeof(T)) : kNoColumn;
@@ -377,11 +385,11 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
   }
   if (!on) return;
   if constexpr (!FULL) {
-    float* e = pl.ends + (int64_t)blockIdx.x * unit_floats;
+    float* e = pl.ends + unit * unit_floats;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
       if (n < a.n) store_f32<float, VC>(e + (int64_t)n * channels + c, S[n]);
-    if (c % a.hd == 0) pl.decays[(int64_t)blockIdx.x * a.heads + h] = all;
+    if (c % a.hd == 0) pl.decays[unit * a.heads + h] = all;
   } else if (w.slot >= 0 && w.u.k == w.last) {
     float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
 #pragma unroll
@@ -429,14 +437,14 @@ static hipError_t launch_small_n(const SsmArgs& a, const ScanPlan& pl, hipStream
 // head lies: (float / head_stride) % heads.
 template <int V>
 __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64_t unit_floats,
-                                                   int head_stride, int heads) {
+                                                   int blocks, int head_stride, int heads) {
   constexpr int kAhead = 8;
   ScanUnit w;
-  if (!scan_unit(q, blockIdx.x, pl.len, w) || w.u.k != 0 || w.last == 0) return;
-  const int64_t at = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V;
+  if (!scan_unit(q, blockIdx.x / blocks, pl, w) || w.u.k != 0 || w.last == 0) return;
+  const int64_t at = ((int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x) * V;
   if (at >= unit_floats) return;
-  float* e = pl.ends + (int64_t)blockIdx.x * unit_floats + at;
-  const float* dec = pl.decays + (int64_t)blockIdx.x * heads + at / head_stride % heads;
+  float* e = pl.ends + w.place0 * unit_floats + at;
+  const float* dec = pl.decays + w.place0 * heads + at / head_stride % heads;
   float S[V];
   load_f32<float, V>(S, e + w.last * unit_floats);
   for (int j0 = 0; j0 < w.last; j0 += kAhead) {
@@ -456,13 +464,6 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
     }
   }
   store_f32<float, V>(e + w.last * unit_floats, S);
-}
-template <int V>
-static void launch_join(const SsmArgs& a, const ScanPlan& pl, int64_t unit_floats, int head_stride,
-                        hipStream_t s) {
-  hipLaunchKernelGGL((k_scan_join<V>),
-                     dim3((unsigned)pl.units, (unsigned)((unit_floats / V + 255) / 256)), dim3(256),
-                     0, s, a.q, pl, unit_floats, head_stride, a.heads);
 }
 
 // ---- more state values: chunks of kQ rows on the matrix cores --------------
@@ -655,7 +656,7 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
         *shW = scal + 4 * kQ;
 
   ScanUnit w;
-  if (!scan_unit(a.q, blockIdx.x, pl.len, w)) return;
+  if (!scan_unit(a.q, blockIdx.x, pl, w)) return;
   if (!FULL && w.u.k == w.last) return;
   const int g = blockIdx.y, per = a.heads / a.groups;
   const int ptiles = (a.hd + 31) / 32;
@@ -666,7 +667,7 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
   const int p = pt * 32 + li;
   const bool on = active && p < a.hd;
   const int64_t c = (int64_t)h * a.hd + p;
-  const int64_t unit0 = (int64_t)blockIdx.x - w.u.k;
+  const int64_t unit0 = w.place0, unit = unit0 + w.u.k;
   constexpr int kTile = NT * 16 * 64;  // floats of a state tile in `ends`: [nt][r / 4][lane][4]
   const int64_t tile_at = ((int64_t)h * ptiles + pt) * kTile + 4 * lane;
   const int64_t unit_floats = (int64_t)a.heads * ptiles * kTile;
@@ -701,7 +702,7 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
       }
     }
   } else if (w.last > 0 && active) {
-    get_tile(S, pl.ends + (int64_t)blockIdx.x * unit_floats + tile_at);
+    get_tile(S, pl.ends + unit * unit_floats + tile_at);
   }
 
   const float A = a.A[h], bias = bias_of(a, h);
@@ -1019,10 +1020,10 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
 
   if constexpr (!FULL) {
     if (!active) return;
-    float* e = pl.ends + (int64_t)blockIdx.x * unit_floats + tile_at;
+    float* e = pl.ends + unit * unit_floats + tile_at;
     put_tile(e, S);
     if (pt == 0 && lane == 0)
-      pl.decays[(int64_t)blockIdx.x * a.heads + h] = __builtin_amdgcn_exp2f((float)total);
+      pl.decays[unit * a.heads + h] = __builtin_amdgcn_exp2f((float)total);
   } else if (w.slot >= 0 && w.u.k == w.last) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -1061,7 +1062,10 @@ static hipError_t launch_mm(const SsmArgs& a, const ScanPlan& pl, hipStream_t s)
     hipLaunchKernelGGL((k_scan_mm<T, NT, NW, false>), grid, dim3(64 * NW), bytes, s, a, pl, tiles,
                        wide);
     const int head = mm_ptiles(a.hd) * NT * 1024;
-    launch_join<4>(a, pl, (int64_t)a.heads * head, head, s);
+    const int64_t floats = (int64_t)a.heads * head;
+    const int blocks = (int)((floats / 4 + 255) / 256);
+    hipLaunchKernelGGL((k_scan_join<4>), dim3((unsigned)(pl.units * blocks)), dim3(256), 0, s, a.q,
+                       pl, floats, blocks, head, a.heads);
   }
   hipLaunchKernelGGL((k_scan_mm<T, NT, NW, true>), grid, dim3(64 * NW), bytes, s, a, pl, tiles,
                      wide);
@@ -1108,8 +1112,14 @@ static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
   const int64_t floats =
       small ? channels * op->d_state
             : (int64_t)op->n_heads * mm_ptiles(op->head_dim) * mm_nt(op->d_state) * 1024;
-  const size_t ends = align_up((size_t)pl.units * floats * 4, 256);
-  *bytes = pl.split ? ends + (size_t)pl.units * op->n_heads * 4 : 0;
+  // no more places than sequences of two units can take
+  const int64_t by_rows = 2 * (T / pl.len) + 2;
+  pl.by_rows = by_rows < pl.units;
+  const int64_t places = pl.by_rows ? by_rows : pl.units;
+  const size_t ends = align_up((size_t)places * floats * 4, 256);
+  *bytes = pl.split ? ends + (size_t)places * op->n_heads * 4 : 0;
+  // the join's grid, the largest, has to fit
+  pl.fits = pl.units <= 0x7fffffff && (small || pl.units * ((floats + 1023) / 1024) <= 0x7fffffff);
   pl.decays = (float*)ends;  // its offset, until the workspace is known
   return pl;
 }
@@ -1132,7 +1142,7 @@ static bool shape_fits(const char* name, const bm_hip_ssm_t* op) {
   if (op->type < BM_HIP_F32 || op->type > BM_HIP_F16 || op->n_heads < 1 || op->n_heads > 65535 ||
       op->head_dim < 1 || op->head_dim > 65535 || op->n_groups < 1 ||
       op->n_heads % op->n_groups || op->d_state < 1 || op->d_state > 256 ||
-      (int64_t)op->n_heads * op->head_dim > (1 << 22)) {
+      (int64_t)op->n_heads * op->head_dim > (1 << 21)) {
     bm_set_error("%s: invalid arguments (type=%d n_heads=%d head_dim=%d n_groups=%d d_state=%d)",
                  name, op->type, op->n_heads, op->head_dim, op->n_groups, op->d_state);
     return false;
@@ -1187,7 +1197,7 @@ static int ssm_call(const bm_hip_ssm_t* op, void* workspace, void* stream, bool 
       bm_set_error("%s: a workspace of %zu bytes on 256 bytes is required", name, bytes);
       return -2;
     }
-    if (pl.units > 0x7fffffff) {
+    if (!pl.fits) {
       bm_set_error("%s: too many rows for one call", name);
       return -2;
     }

@@ -204,6 +204,16 @@ def test_scan_long(hip, type_name, N, lens):
 
 
 @pytest.mark.parametrize("N", [1, 24])
+def test_scan_long_sequences_among_many_short_ones(hip, N):
+    """More sequences than rows make units: the long ones' parts keep apart."""
+    r = np.random.default_rng(12)
+    lens = [int(v) for v in r.integers(0, 4, 150)]
+    for at_ in (0, 40, 41, 120, 149):
+        lens[at_] = int(r.integers(520, 700))
+    SsmCase("f32", 2, 32, 2 if N == 1 else 1, N, lens, seed=N, front=1).check(hip, "many")
+
+
+@pytest.mark.parametrize("N", [1, 24])
 def test_scan_steps_given(hip, N):
     """Without softplus, and without bias: dt is the step itself."""
     for bias in (True, False):

@@ -37,6 +37,7 @@ def refused(rc, word):
 
 
 SHARED = [("type", dict(type=3)), ("type", dict(type=-1)), ("n_seqs", dict(n_seqs=-1)),
+          ("n_seqs", dict(n_seqs=(1 << 20) + 1, n_slots=1 << 21)),
           ("x needs", dict(x=None)), ("x needs", dict(x=P + 2)), ("y needs", dict(y=None)),
           ("y needs", dict(y_stride=63)), ("x needs", dict(x_stride=63)),
           ("x needs", dict(x_stride=1 << 24)), ("slots", dict(n_slots=0)),
@@ -44,6 +45,7 @@ SHARED = [("type", dict(type=3)), ("type", dict(type=-1)), ("n_seqs", dict(n_seq
           ("addresses", dict(state=P + 2)), ("y overlaps x", dict(y=P + 8)),
           ("y overlaps x", dict(y=P + 4 * 64 * 3))]
 PROMPTS = [("seq_start", dict(seq_start=None)), ("n_tokens", dict(n_tokens=-1)),
+           ("n_tokens", dict(n_tokens=1 << 30)),
            ("y overlaps x", dict(y=P))]
 
 
@@ -95,6 +97,9 @@ def test_workspace_is_required():
     bare = bh.Ssm(type=d.type, n_heads=64, head_dim=64, n_groups=1, d_state=128, n_seqs=1,
                   n_tokens=16384)
     assert L.bm_hip_ssm_workspace_bytes(C.byref(bare)) == n
+    # many short sequences: no more than the rows of long ones could need
+    bare.n_seqs = 4096
+    assert L.bm_hip_ssm_workspace_bytes(C.byref(bare)) < 8 * n + (1 << 30)
     if n:
         refused(L.bm_hip_ssm_dev(C.byref(d), None, None), "workspace")
         refused(L.bm_hip_ssm_dev(C.byref(d), C.c_void_p(P + 64), None), "workspace")
