@@ -214,17 +214,21 @@ __device__ __forceinline__ bool scan_unit(const SeqView& q, int index, const Sca
 }
 
 // ---- up to 8 state values per channel -------------------------------------
-// A lane owns VC neighbouring channels with their state in registers and
-// walks the unit's rows; a block is one wave.  What the channels of a head
-// share per row -- decay, d B[n], C[n] -- is worked out once per row and head
-// into LDS.  2-4 operations per state value and row against 12 bytes per
-// channel and row: bound by memory, and in one short prompt by the round
-// trips to it, so that a tile's loads are all issued before any is used.
+// A lane owns a channel with its state in registers and walks the unit's
+// rows; a block is one wave.  What the channels of a head share per row --
+// decay, d B[n], C[n] -- is worked out once per row and head into LDS.  2-4
+// operations per state value and row against 12 bytes per channel and row:
+// bound by memory, and in one short prompt by the round trips to it, so that
+// the loads of a tile of kSmallRows rows are all issued before any is used,
+// and the next tile's while one is worked on.  At 64 heads of 64 channels and
+// one value, fp32, 1024 rows: 8 and 16 us for the two passes, 51 MB at 2.2
+// TB/s; 6001 rows of 32 heads 54 us, 2.8 TB/s (tiles of 8 and 32 rows: 73 and
+// 69 us; two or four channels per lane: 72 and 103).
 constexpr int kSmallState = 8;
-constexpr int kSmallRows = 16;  // rows per tile
+constexpr int kSmallRows = 16;
 __host__ __device__ constexpr int small_entry(int ns) { return (1 + 2 * ns + 3) / 4 * 4; }
 
-template <typename T, int NS, int VC, bool FULL>
+template <typename T, int NS, bool FULL>
 __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int heads_max) {
   constexpr int tile = kSmallRows, EW = small_entry(NS);
   extern __shared__ float4 sh4[];
@@ -233,11 +237,11 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
   if (!scan_unit(a.q, blockIdx.x, pl, w)) return;
   if (!FULL && w.u.k == w.last) return;
   const int lane = threadIdx.x, channels = a.heads * a.hd;
-  const int c0 = blockIdx.y * 64 * VC;
-  const int c = c0 + lane * VC;
-  const bool on = c < channels;  // VC divides head_dim where it is more than 1
+  const int c0 = blockIdx.y * 64;
+  const int c = c0 + lane;
+  const bool on = c < channels;
   const int h0 = c0 / a.hd;
-  const int h1 = (min(c0 + 64 * VC, channels) - 1) / a.hd;
+  const int h1 = (min(c0 + 64, channels) - 1) / a.hd;
   const int nh = h1 - h0 + 1;
   const int h = on ? c / a.hd : h0;
   const int per = a.heads / a.groups;
@@ -247,80 +251,69 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
   const uint32_t col = on ? (uint32_t)(c * sizeof(T)) : kNoColumn;
   const uint32_t xs = (uint32_t)(a.xs * sizeof(T)), zs = (uint32_t)(a.zs * sizeof(T)),
                  ys = (uint32_t)(a.ys * sizeof(T));
-  Pack<T, VC> xr[kSmallRows], zr[kSmallRows];
+  uint32_t xr[tile], zr[tile];
   auto fetch = [&](int t) {
     const int rows = min(tile, w.t1 - t);
     const auto bx = rows_of<T>(a.x, t, a.xs, rows);
     const auto bz = rows_of<T>(a.z, t, a.zs, FULL && a.z ? rows : 0);
 #pragma unroll
-    for (int r = 0; r < kSmallRows; ++r) {
-      xr[r] = load_row<T, VC>(bx, col + r * xs);
-      if (FULL) zr[r] = load_row<T, VC>(bz, col + r * zs);
+    for (int r = 0; r < tile; ++r) {
+      xr[r] = load_raw<T>(bx, col + r * xs);
+      if (FULL) zr[r] = load_raw<T>(bz, col + r * zs);
     }
   };
   if (w.t0 < w.t1) fetch(w.t0);
 
-  float S[NS][VC];
+  float S[NS];
 #pragma unroll
-  for (int n = 0; n < NS; ++n)
-#pragma unroll
-    for (int i = 0; i < VC; ++i) S[n][i] = 0.0f;
+  for (int n = 0; n < NS; ++n) S[n] = 0.0f;
   // from the slot, or from the copy that the first pass made of it
   if (on && w.keep && (FULL ? w.last == 0 : w.u.k == 0)) {
     const float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int i = 0; i < VC; ++i)
-        if (n < a.n) S[n][i] = st[i * a.n + n];
+      if (n < a.n) S[n] = st[n];
   }
   if constexpr (!FULL) {
     if (w.u.k == 0) {
-      if (on) {
-        float* e = pl.ends + (unit0 + w.last) * unit_floats;
+      float* e = pl.ends + (unit0 + w.last) * unit_floats + c;
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-          if (n < a.n) store_f32<float, VC>(e + (int64_t)n * channels + c, S[n]);
+      for (int n = 0; n < NS; ++n) {
+        if (on && n < a.n) e[(int64_t)n * channels] = S[n];
+        S[n] = 0.0f;
       }
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < VC; ++i) S[n][i] = 0.0f;
     }
   } else if (w.last > 0 && on) {
     // the join, a few floats of each unit before this one: cheaper here than
-    // a launch of its own (4.7 us and its gap against 3 us)
+    // a launch of its own (3 us against 4.7 and its gap)
     constexpr int kAhead = NS == 1 ? 16 : 4;
     const float* e = pl.ends + unit0 * unit_floats + c;
     const float* dec = pl.decays + unit0 * a.heads + h;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-      if (n < a.n) load_f32<float, VC>(S[n], e + w.last * unit_floats + (int64_t)n * channels);
+      if (n < a.n) S[n] = e[w.last * unit_floats + (int64_t)n * channels];
     for (int j0 = 0; j0 < w.u.k; j0 += kAhead) {
-      float v[kAhead][NS][VC], d[kAhead];
+      float v[kAhead][NS], d[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int j = min(j0 + i, w.u.k - 1);
         d[i] = dec[(int64_t)j * a.heads];
 #pragma unroll
         for (int n = 0; n < NS; ++n)
-          load_f32<float, VC>(v[i][n], e + j * unit_floats + (int64_t)min(n, a.n - 1) * channels);
+          v[i][n] = e[j * unit_floats + (int64_t)min(n, a.n - 1) * channels];
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (j0 + i >= w.u.k) break;
 #pragma unroll
         for (int n = 0; n < NS; ++n)
-#pragma unroll
-          for (int k = 0; k < VC; ++k)
-            S[n][k] = n < a.n ? __builtin_fmaf(S[n][k], d[i], v[i][n][k]) : 0.0f;
+          S[n] = n < a.n ? __builtin_fmaf(S[n], d[i], v[i][n]) : 0.0f;
       }
     }
   }
 
-  float D[VC], all = 1.0f;
-#pragma unroll
-  for (int i = 0; i < VC; ++i) D[i] = FULL && on && a.D ? a.D[c + i] : 0.0f;
+  const float D = FULL && on && a.D ? a.D[c] : 0.0f;
+  float all = 1.0f;  // the unit's decay
   for (int t = w.t0; t < w.t1; t += tile) {
     const int rows = min(tile, w.t1 - t);
     for (int i = lane; i < tile * nh; i += 64) {
@@ -346,105 +339,94 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
       }
     }
     __syncthreads();
-    float x[kSmallRows][VC], z[kSmallRows][VC];
+    float x[tile], z[tile];
 #pragma unroll
-    for (int r = 0; r < kSmallRows; ++r)
-#pragma unroll
-      for (int i = 0; i < VC; ++i) {
-        x[r][i] = (float)xr[r].v[i];
-        z[r][i] = FULL && a.z ? silu_f32((float)zr[r].v[i]) : 1.0f;
-      }
+    for (int r = 0; r < tile; ++r) {
+      x[r] = raw_f32<T>(xr[r]);
+      z[r] = FULL && a.z ? silu_f32(raw_f32<T>(zr[r])) : 1.0f;
+    }
     if (t + tile < w.t1) fetch(t + tile);
     const auto by = rows_of<T>(a.y, t, a.ys, rows);
 #pragma unroll
-    for (int r = 0; r < kSmallRows; ++r) {
+    for (int r = 0; r < tile; ++r) {
       float e[EW];
       const float4* s = (const float4*)(sh + (r * heads_max + (h - h0)) * EW);
 #pragma unroll
       for (int k = 0; k < EW / 4; ++k) *(float4*)(e + 4 * k) = s[k];
-      float y[VC];
+      float y = FULL ? D * x[r] : 0.0f;
 #pragma unroll
-      for (int i = 0; i < VC; ++i) y[i] = FULL ? D[i] * x[r][i] : 0.0f;
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int i = 0; i < VC; ++i) {
-          S[n][i] = __builtin_fmaf(S[n][i], e[0], x[r][i] * e[1 + n]);
-          // a value beyond d_state stays zero even where the decay is infinite
-          if (NS > 2) S[n][i] = n < a.n ? S[n][i] : 0.0f;
-          if (FULL) y[i] = __builtin_fmaf(S[n][i], e[1 + NS + n], y[i]);
-        }
+      for (int n = 0; n < NS; ++n) {
+        S[n] = __builtin_fmaf(S[n], e[0], x[r] * e[1 + n]);
+        // a value beyond d_state stays zero even where the decay is infinite
+        if (NS > 2) S[n] = n < a.n ? S[n] : 0.0f;
+        if (FULL) y = __builtin_fmaf(S[n], e[1 + NS + n], y);
+      }
       all *= e[0];
       if (FULL) {
-#pragma unroll
-        for (int i = 0; i < VC; ++i) y[i] *= z[r][i];
-        store_row<T, VC>(by, col + r * ys, y);
+        const float out[1] = {y * z[r]};
+        store_row<T, 1>(by, col + r * ys, out);
       }
     }
     __syncthreads();
   }
   if (!on) return;
   if constexpr (!FULL) {
-    float* e = pl.ends + unit * unit_floats;
+    float* e = pl.ends + unit * unit_floats + c;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-      if (n < a.n) store_f32<float, VC>(e + (int64_t)n * channels + c, S[n]);
+      if (n < a.n) e[(int64_t)n * channels] = S[n];
     if (c % a.hd == 0) pl.decays[unit * a.heads + h] = all;
   } else if (w.slot >= 0 && w.u.k == w.last) {
     float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int i = 0; i < VC; ++i)
-        if (n < a.n) st[i * a.n + n] = S[n][i];
+      if (n < a.n) st[n] = S[n];
   }
 }
 
-template <typename T, int NS, int VC>
+template <typename T, int NS>
 static hipError_t launch_small(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
-  const int span = 64 * VC, channels = a.heads * a.hd;
-  const int by = (channels + span - 1) / span;
-  const int hm = (span + a.hd - 2) / a.hd + 1;
+  const int channels = a.heads * a.hd;
+  const int by = (channels + 63) / 64;
+  const int hm = (64 + a.hd - 2) / a.hd + 1;
   const int heads_max = hm < a.heads ? hm : a.heads;
-  const int bytes = kSmallRows * heads_max * small_entry(NS) * 4;
+  const int bytes = kSmallRows * heads_max * small_entry(NS) * 4;  // at most 80 KB
   if (bytes > 64 * 1024) {  // heads of one channel; once per process
     static const hipError_t raised[2] = {
-        hipFuncSetAttribute((const void*)k_scan_small<T, NS, VC, false>,
+        hipFuncSetAttribute((const void*)k_scan_small<T, NS, false>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024),
-        hipFuncSetAttribute((const void*)k_scan_small<T, NS, VC, true>,
+        hipFuncSetAttribute((const void*)k_scan_small<T, NS, true>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)};
     if (raised[0] != hipSuccess) return raised[0];
     if (raised[1] != hipSuccess) return raised[1];
   }
+  const dim3 grid((unsigned)pl.units, by);
   if (pl.split)
-    hipLaunchKernelGGL((k_scan_small<T, NS, VC, false>), dim3((unsigned)pl.units, by), dim3(64),
-                       bytes, s, a, pl, heads_max);
-  hipLaunchKernelGGL((k_scan_small<T, NS, VC, true>), dim3((unsigned)pl.units, by), dim3(64),
-                     bytes, s, a, pl, heads_max);
+    hipLaunchKernelGGL((k_scan_small<T, NS, false>), grid, dim3(64), bytes, s, a, pl, heads_max);
+  hipLaunchKernelGGL((k_scan_small<T, NS, true>), grid, dim3(64), bytes, s, a, pl, heads_max);
   return hipGetLastError();
 }
 
-template <typename T, int VC>
+template <typename T>
 static hipError_t launch_small_n(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
-  if (a.n == 1) return launch_small<T, 1, VC>(a, pl, s);
-  if (a.n == 2) return launch_small<T, 2, VC>(a, pl, s);
-  if (a.n <= 4) return launch_small<T, 4, VC>(a, pl, s);
-  return launch_small<T, 8, VC>(a, pl, s);
+  if (a.n == 1) return launch_small<T, 1>(a, pl, s);
+  if (a.n == 2) return launch_small<T, 2>(a, pl, s);
+  if (a.n <= 4) return launch_small<T, 4>(a, pl, s);
+  return launch_small<T, 8>(a, pl, s);
 }
 
-// The join: a thread takes V neighbouring floats of a sequence's units in
-// turn, kAhead of them loaded before the first is used.  Where the floats'
-// head lies: (float / head_stride) % heads.
-template <int V>
+// The join: a thread takes four neighbouring floats of a sequence's units in
+// turn, kAhead of them loaded before the first is used.  A head's floats are
+// head_floats.  Bound by reading and writing the states once: 4 TB/s at 31 MB.
 __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64_t unit_floats,
-                                                   int blocks, int head_stride, int heads) {
-  constexpr int kAhead = 8;
+                                                   int blocks, int head_floats, int heads) {
+  constexpr int kAhead = 8, V = 4;
   ScanUnit w;
   if (!scan_unit(q, blockIdx.x / blocks, pl, w) || w.u.k != 0 || w.last == 0) return;
   const int64_t at = ((int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x) * V;
   if (at >= unit_floats) return;
   float* e = pl.ends + w.place0 * unit_floats + at;
-  const float* dec = pl.decays + w.place0 * heads + at / head_stride % heads;
+  const float* dec = pl.decays + w.place0 * heads + at / head_floats;
   float S[V];
   load_f32<float, V>(S, e + w.last * unit_floats);
   for (int j0 = 0; j0 < w.last; j0 += kAhead) {
@@ -471,9 +453,21 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
 // With c_i the sum of A d over the chunk's rows up to i,
 //   y_i = sum_{j<=i} (C_i . B_j) e^{c_i - c_j} d_j x_j + e^{c_i} C_i . S
 //   S'  = e^{c_Q} S + sum_j B_j (e^{c_Q - c_j} d_j x_j)
-// A block takes one unit and up to NW tiles of 32 channels of one group; a
+// A block takes one unit and up to four tiles of 32 channels of one group; a
 // wave keeps its tile's state S [d_state][32] in accumulators over the whole
-// unit.  B and C go through LDS once per chunk for all tiles.
+// unit.  B and C go through LDS once per chunk for all tiles.  Four waves and
+// two blocks per CU beat one block of eight, whose waves all wait for the same
+// barriers (second pass at d_state 128, bf16: 319 against 335 us then).
+//
+// What bounds it: per 32 rows and channels at d_state 128, bf16, about 1050
+// vector instructions (splitting S, the decays, gates) and 46 MFMAs.  With two
+// waves per SIMD (214 registers) the vector pipe is busy about 60 % of the
+// time; leaving out all memory accesses takes 228 us to 177.  Tried without
+// gain: x and z a chunk ahead, a third wave per SIMD (spills), dot products in
+// place of subtractions in the split, uniform row offsets, one exponential per
+// row in place of one per pair.  64 heads of 64, d_state 128, one group, bf16,
+// 16384 rows: 100 + 16 + 220 us for the passes and the join, 417 MB (82 us);
+// 32 heads, d_state 64, fp32, 3001 rows: 22 + 10 + 38 us, 84 MB (16 us).
 //
 // Precision.  MFMA operands are bf16.  An fp32 value is carried as the sum of
 // three bf16 pieces (8 bits each, the remainder of the piece before), fp16 as
@@ -497,7 +491,7 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
 // Causality holds for infinities and NaN too: a product takes 0 for M above
 // the diagonal, and 0 times such an x would reach earlier rows, so x enters
 // that product as 0 and the rows from it on become NaN.
-constexpr int kQ = 32;
+constexpr int kQ = 32, kWaves = 4;
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -571,16 +565,14 @@ struct MmLds {
   static constexpr int kRowCb = kQ + 4;  // floats
   static constexpr int kCb = kQ * kRowCb * 4;
   static constexpr int kScal = 5 * kQ * 4;  // per wave: c (two parts), d, e^c, e^{c_Q - c} d
-  static constexpr int whole(int nw) {
-    return Pieces<T>::IN * (2 * kPieceB + kPieceT) + kCb + nw * kScal;
-  }
-  // B by rows and B^T share a place where they do not both fit: the first is
-  // done with when C B^T is
-  static constexpr bool kShared = whole(4) > 80 * 1024;
+  static constexpr int kApart = Pieces<T>::IN * (2 * kPieceB + kPieceT) + kCb + kWaves * kScal;
+  // B by rows and B^T share a place where two blocks do not fit a CU
+  // otherwise: the first is done with when C B^T is
+  static constexpr bool kShared = kApart > 80 * 1024;
   static constexpr int kC = Pieces<T>::IN * (kShared && kPieceT > kPieceB ? kPieceT : kPieceB);
   static constexpr int kT = kShared ? 0 : kC + Pieces<T>::IN * kPieceB;
   static constexpr int kAfter = kC + Pieces<T>::IN * (kPieceB + (kShared ? 0 : kPieceT));
-  static constexpr int bytes(int nw) { return kAfter + kCb + nw * kScal; }
+  static constexpr int kBytes = kAfter + kCb + kWaves * kScal;
 };
 
 // running sums over each half of the wave
@@ -636,12 +628,12 @@ __device__ __forceinline__ void get_tile(v16f (&S)[NT], const float* e) {
     }
 }
 
-template <typename T, int NT, int NW, bool FULL>
-__global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, ScanPlan pl, int tiles, int wide) {
+template <typename T, int NT, bool FULL>
+__global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, ScanPlan pl, int tiles, int wide) {
   using L = MmLds<T, NT>;
   constexpr int IN = Pieces<T>::IN, YP = Pieces<T>::Y;
   constexpr bool kExact = YP == 3;  // y to better than bf16
-  constexpr int kThreads = 64 * NW;
+  constexpr int kThreads = 64 * kWaves;
   constexpr int kBlocks = 64 * NT;  // 4x4 blocks of B (or C) in a chunk
   constexpr int kItems = ((FULL ? 2 : 1) * kBlocks + kThreads - 1) / kThreads;
   extern __shared__ float4 sh4[];
@@ -660,7 +652,7 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
   if (!FULL && w.u.k == w.last) return;
   const int g = blockIdx.y, per = a.heads / a.groups;
   const int ptiles = (a.hd + 31) / 32;
-  const int item = blockIdx.z * NW + wave;  // tile of the group
+  const int item = blockIdx.z * kWaves + wave;  // tile of the group
   const bool active = item < tiles;
   const int h = g * per + (active ? item / ptiles : 0);
   const int pt = active ? item % ptiles : 0;
@@ -1037,58 +1029,56 @@ __global__ __launch_bounds__(64 * NW, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs a, 
 
 static int mm_ptiles(int hd) { return (hd + 31) / 32; }
 static int mm_nt(int n) { return n <= 32 ? 1 : (n <= 64 ? 2 : (n <= 128 ? 4 : 8)); }
-// waves per block: eight where a group has that many tiles and the state
-// leaves room for two waves per SIMD
-static int mm_waves(int tiles, int nt) { return 4; }
-
-template <typename T, int NT, int NW>
+template <typename T, int NT>
 static hipError_t launch_mm(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
   const int tiles = a.heads / a.groups * mm_ptiles(a.hd);
-  constexpr int bytes = MmLds<T, NT>::bytes(NW);
+  constexpr int bytes = MmLds<T, NT>::kBytes;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   const int wide = a.n % 4 == 0 && a.Bs % 4 == 0 && a.Cs % 4 == 0 &&
                    ((uintptr_t)a.B | (uintptr_t)a.C) % (4 * sizeof(T)) == 0;
-  const dim3 grid((unsigned)pl.units, a.groups, (tiles + NW - 1) / NW);
+  const dim3 grid((unsigned)pl.units, a.groups, (tiles + kWaves - 1) / kWaves);
   if (bytes > 64 * 1024) {  // once per process: a kernel's limit above the default
     static const hipError_t raised[2] = {
-        hipFuncSetAttribute((const void*)k_scan_mm<T, NT, NW, false>,
+        hipFuncSetAttribute((const void*)k_scan_mm<T, NT, false>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
-        hipFuncSetAttribute((const void*)k_scan_mm<T, NT, NW, true>,
+        hipFuncSetAttribute((const void*)k_scan_mm<T, NT, true>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes)};
     if (raised[0] != hipSuccess) return raised[0];
     if (raised[1] != hipSuccess) return raised[1];
   }
   if (pl.split) {
-    hipLaunchKernelGGL((k_scan_mm<T, NT, NW, false>), grid, dim3(64 * NW), bytes, s, a, pl, tiles,
+    hipLaunchKernelGGL((k_scan_mm<T, NT, false>), grid, dim3(64 * kWaves), bytes, s, a, pl, tiles,
                        wide);
     const int head = mm_ptiles(a.hd) * NT * 1024;
     const int64_t floats = (int64_t)a.heads * head;
     const int blocks = (int)((floats / 4 + 255) / 256);
-    hipLaunchKernelGGL((k_scan_join<4>), dim3((unsigned)(pl.units * blocks)), dim3(256), 0, s, a.q,
+    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(pl.units * blocks)), dim3(256), 0, s, a.q,
                        pl, floats, blocks, head, a.heads);
   }
-  hipLaunchKernelGGL((k_scan_mm<T, NT, NW, true>), grid, dim3(64 * NW), bytes, s, a, pl, tiles,
+  hipLaunchKernelGGL((k_scan_mm<T, NT, true>), grid, dim3(64 * kWaves), bytes, s, a, pl, tiles,
                      wide);
   return hipGetLastError();
 }
 
 template <typename T>
 static hipError_t launch_mm_t(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
-  const int nt = mm_nt(a.n);
-  const bool w8 = mm_waves(a.heads / a.groups * mm_ptiles(a.hd), nt) == 8;
-  switch (nt) {
-    case 1: return w8 ? launch_mm<T, 1, 8>(a, pl, s) : launch_mm<T, 1, 4>(a, pl, s);
-    case 2: return w8 ? launch_mm<T, 2, 8>(a, pl, s) : launch_mm<T, 2, 4>(a, pl, s);
-    case 4: return w8 ? launch_mm<T, 4, 8>(a, pl, s) : launch_mm<T, 4, 4>(a, pl, s);
-    default: return launch_mm<T, 8, 4>(a, pl, s);
+  switch (mm_nt(a.n)) {
+    case 1: return launch_mm<T, 1>(a, pl, s);
+    case 2: return launch_mm<T, 2>(a, pl, s);
+    case 4: return launch_mm<T, 4>(a, pl, s);
+    default: return launch_mm<T, 8>(a, pl, s);
   }
 }
 
 // ---- the cut into units ----------------------------------------------------
-// Units as short as the chip needs to be filled (kFillWaves waves over all of
-// them: a little less than the 2048 that the second pass's registers let it
-// hold, since one workgroup that finds no place doubles the whole time), but no shorter than what the first pass and the walk over a
-// sequence's units are worth, and no more than 32 (64) of them in a sequence.
+// Units as short as it takes to fill the chip, no shorter than what a unit's
+// prologue and the first pass are worth (32 rows; 128 on the matrix cores), at
+// most 64 (32) of them in the longest sequence, and, where there are several
+// sequences of which one may have almost all rows, no longer than 512 rows.
+// The matrix kernel's fill stays a little below the 2048 waves that its second
+// pass's registers let the chip hold, since one workgroup that finds no place
+// then doubles the whole time: 219 against 330 us with 15 and 16 units of
+// 16384 rows.
 constexpr int kFillWaves = 1920, kSmallFillWaves = 2048;
 
 static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
@@ -1127,11 +1117,7 @@ static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
 template <typename T>
 static hipError_t launch_scan_t(const SsmArgs& a, const ScanPlan& pl, hipStream_t s) {
   if (a.n > kSmallState) return launch_mm_t<T>(a, pl, s);
-  constexpr int V = 4;
-  const bool wide = a.hd % V == 0 && a.xs % V == 0 && a.ys % V == 0 && (!a.z || a.zs % V == 0) &&
-                    ((uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.z) % (V * sizeof(T)) == 0;
-  (void)wide;
-  return launch_small_n<T, 1>(a, pl, s);
+  return launch_small_n<T>(a, pl, s);
 }
 
 static bool shape_fits(const char* name, const bm_hip_ssm_t* op) {
