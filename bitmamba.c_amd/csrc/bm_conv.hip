@@ -76,7 +76,7 @@ template <typename T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
   const int c = (blockIdx.y * 256 + threadIdx.x) * V;
   const int slots = first_slots(a.q);
-  const Unit u = find_unit(a.q, blockIdx.x, kConvRows);
+  const Unit u = find_unit(a.q, (int)wide_block(), kConvRows);
   if (u.b < 0) return;
   if (u.k > (u.e > u.s ? (u.e - u.s - 1) / kConvRows : 0)) return;  // past its rows
   const int t0 = u.s + u.k * kConvRows, t1 = u.e - t0 < kConvRows ? u.e : t0 + kConvRows;
@@ -194,8 +194,8 @@ static hipError_t launch_conv(const ConvArgs& a, bool step, hipStream_t s) {
     hipLaunchKernelGGL((k_conv_step<T, W, V, 1>), dim3(a.q.n_seqs, gy), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((k_conv<T, W, V>),
-                       dim3((unsigned)unit_count(a.q.n_seqs, a.q.n_tokens, kConvRows), gy),
-                       dim3(256), 0, s, a);
+                       wide_grid(unit_count(a.q.n_seqs, a.q.n_tokens, kConvRows), gy), dim3(256), 0,
+                       s, a);
   return hipGetLastError();
 }
 
@@ -242,10 +242,6 @@ static int conv_call(const bm_hip_conv_t* op, void* stream, bool step) {
                        op->channels, rows, elem, step))
     return -2;
   if (op->n_seqs == 0) return 0;
-  if (bm::unit_count(op->n_seqs, step ? 0 : op->n_tokens, bm::kConvRows) > 0x7fffffff) {
-    bm_set_error("%s: too many rows for one call", name);
-    return -2;
-  }
   if (!bm_hip_init()) return -1;
   bm::OnDevice dev;
   bm::ConvArgs a;

@@ -212,6 +212,16 @@ __device__ __forceinline__ int seq_row(const SeqView& q, int i) {
 __host__ __device__ inline int64_t unit_count(int n_seqs, int n_tokens, int len) {
   return (int64_t)n_tokens / len + n_seqs;
 }
+// A grid of any number of blocks: x and z, since a launch has less than 2^32
+// threads along x.  The last row of z may have blocks past the number.
+constexpr int64_t kGridX = 1 << 20;
+inline dim3 wide_grid(int64_t blocks, unsigned y) {
+  return dim3((unsigned)(blocks < kGridX ? blocks : kGridX), y,
+              (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ int64_t wide_block() {
+  return (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
+}
 struct Unit {
   int b;     // sequence, -1: none
   int k;     // unit of it
@@ -232,6 +242,8 @@ __device__ __forceinline__ Unit find_unit(const SeqView& q, int u, int len) {
     if (c == 0) return Unit{-1, 0, 0, 0};  // rows before the first sequence
     if (step == 1) {
       const int s = __builtin_amdgcn_readlane(row, c - 1), e = __builtin_amdgcn_readlane(row, c);
+      // every counted start has i <= u, so b <= u and the unit's first row,
+      // s + k len = s % len + (u - b) len, is not below 0 even where starts descend
       const int b = lo + c - 1;
       return Unit{b, u - (s / len + b), s, e < s ? s : e};
     }

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void k_slots_copy(PoolView pool, int n_slots,
   __syncthreads();
 
   const int64_t words = pool.slot_bytes / (int64_t)sizeof(W);
-  const int64_t col0 = (int64_t)blockIdx.x << log_cols;
+  const int64_t col0 = wide_block() << log_cols;
   uint8_t* layer = pool.base + (int64_t)blockIdx.y * pool.layer_stride;
   W v[E];
   int to[E];
@@ -99,9 +99,9 @@ static hipError_t launch_copy_e(const PoolView& p, int n_layers, int n_slots, co
   while ((2 << lc) * n <= 256 * E && ((int64_t)1 << lc) < words) ++lc;
   while ((1 << lh) < 2 * n) ++lh;
   const int64_t blocks = (words + ((int64_t)1 << lc) - 1) >> lc;
-  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_slots_copy<W, E>), dim3((unsigned)blocks, n_layers), dim3(256), 0, s, p,
-                     n_slots, src, dst, n, lc, lh);
+  if (blocks > kGridX * 65535) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((k_slots_copy<W, E>), wide_grid(blocks, n_layers), dim3(256), 0, s, p, n_slots,
+                     src, dst, n, lc, lh);
   return hipGetLastError();
 }
 
@@ -320,6 +320,11 @@ extern "C" int bm_hip_slots_compact_dev(const bm_hip_slots_t* pools, int n_pools
       (uintptr_t)workspace % 16 ||
       ((uintptr_t)slots | (uintptr_t)new_slots | (uintptr_t)n_live) % 4) {
     bm_set_error("slots_compact: invalid arguments (n=%d n_slots=%d)", n, n_slots);
+    return -2;
+  }
+  const uintptr_t t0 = (uintptr_t)slots, t1 = (uintptr_t)new_slots, len = (uintptr_t)n * 4;
+  if (t0 != t1 && t0 < t1 + len && t1 < t0 + len) {
+    bm_set_error("slots_compact: new_slots overlaps slots in part");
     return -2;
   }
   if (!bm_hip_init()) return -1;

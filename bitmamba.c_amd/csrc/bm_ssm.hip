@@ -182,7 +182,6 @@ struct ScanPlan {
   int64_t units;
   bool split;      // a sequence may have more than one unit
   bool by_rows;    // where a sequence's units lie in the workspace (ScanUnit)
-  bool fits;       // a grid
   float* ends;
   float* decays;
 };
@@ -422,8 +421,10 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
                                                    int blocks, int head_floats, int heads) {
   constexpr int kAhead = 8, V = 4;
   ScanUnit w;
-  if (!scan_unit(q, blockIdx.x / blocks, pl, w) || w.u.k != 0 || w.last == 0) return;
-  const int64_t at = ((int64_t)(blockIdx.x % blocks) * 256 + threadIdx.x) * V;
+  const int64_t block = wide_block();
+  if (block >= pl.units * blocks) return;
+  if (!scan_unit(q, (int)(block / blocks), pl, w) || w.u.k != 0 || w.last == 0) return;
+  const int64_t at = (block % blocks * 256 + threadIdx.x) * V;
   if (at >= unit_floats) return;
   float* e = pl.ends + w.place0 * unit_floats + at;
   const float* dec = pl.decays + w.place0 * heads + at / head_floats;
@@ -1052,8 +1053,8 @@ static hipError_t launch_mm(const SsmArgs& a, const ScanPlan& pl, hipStream_t s)
     const int head = mm_ptiles(a.hd) * NT * 1024;
     const int64_t floats = (int64_t)a.heads * head;
     const int blocks = (int)((floats / 4 + 255) / 256);
-    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(pl.units * blocks)), dim3(256), 0, s, a.q,
-                       pl, floats, blocks, head, a.heads);
+    hipLaunchKernelGGL(k_scan_join, wide_grid(pl.units * blocks, 1), dim3(256), 0, s, a.q, pl,
+                       floats, blocks, head, a.heads);
   }
   hipLaunchKernelGGL((k_scan_mm<T, NT, true>), grid, dim3(64 * kWaves), bytes, s, a, pl, tiles,
                      wide);
@@ -1108,8 +1109,6 @@ static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
   const int64_t places = pl.by_rows ? by_rows : pl.units;
   const size_t ends = align_up((size_t)places * floats * 4, 256);
   *bytes = pl.split ? ends + (size_t)places * op->n_heads * 4 : 0;
-  // the join's grid, the largest, has to fit
-  pl.fits = pl.units <= 0x7fffffff && (small || pl.units * ((floats + 1023) / 1024) <= 0x7fffffff);
   pl.decays = (float*)ends;  // its offset, until the workspace is known
   return pl;
 }
@@ -1168,7 +1167,7 @@ static int ssm_call(const bm_hip_ssm_t* op, void* workspace, void* stream, bool 
     if (!op->z && &t == &in[4]) continue;  // no gate
     if (!bm::check_rows(name, t.name, t.p, t.stride, t.width, elem) ||
         !bm::check_apart(name, t.name, t.p, t.stride, t.width, op->y, op->y_stride, hp, rows, elem,
-                         step && t.p == op->x))
+                         step && (&t == &in[0] || (&t == &in[4] && op->z == op->x))))
       return -2;
   }
   if (!op->A || ((uintptr_t)op->A | (uintptr_t)op->dt_bias | (uintptr_t)op->D) % 4) {
@@ -1181,10 +1180,6 @@ static int ssm_call(const bm_hip_ssm_t* op, void* workspace, void* stream, bool 
     pl = bm::scan_plan(op, &bytes);
     if (bytes && (!workspace || (uintptr_t)workspace % 256)) {
       bm_set_error("%s: a workspace of %zu bytes on 256 bytes is required", name, bytes);
-      return -2;
-    }
-    if (!pl.fits) {
-      bm_set_error("%s: too many rows for one call", name);
       return -2;
     }
     pl.ends = (float*)workspace;

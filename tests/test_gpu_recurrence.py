@@ -356,3 +356,68 @@ def test_offsets_past_32_bits(hip):
             close(got[t].reshape(H, P), want[t], tols[t], "f32", "row %d" % t)
         close(f64(pool[2 * stride:2 * stride + H * P * N]).reshape(H, P, N), new[2], stol[2],
               "f32", "state")
+
+
+def test_more_rows_than_a_grid_row_of_units(hip):
+    """2^28 + 21 rows of one channel: more units than a launch has blocks of
+    256 threads along x.  Two taps of 1 on integers: every sum is exact."""
+    n = (1 << 28) + 21
+    x = (torch.arange(n, device="cuda", dtype=torch.int32) % 101).to(torch.bfloat16)
+    y = torch.full((n + 8,), -1.0, dtype=torch.bfloat16, device="cuda")
+    w = torch.ones(2, device="cuda")
+    d = bh.Conv(type=bh.BF16, channels=1, width=2, silu=0, n_seqs=1, n_tokens=n, x=at(x),
+                x_stride=1, w=at(w), y=at(y), y_stride=1)
+    note("conv of %d rows" % n)
+    torch.cuda.synchronize()
+    bh.check(hip.bm_hip_conv_dev(C.byref(d), None))
+    torch.cuda.synchronize()
+    assert y[0] == x[0] and torch.equal(y[1:n], x[1:] + x[:-1])
+    assert (y[n:] == -1).all()
+
+
+def test_join_of_more_blocks_than_a_grid_row(hip):
+    """Many prompts, one of which is cut, with states of 512 blocks each: the
+    join's grid is longer than a launch along x."""
+    H, P, N, n = 64, 64, 128, 40000
+    lens = [1] * (n - 1) + [3000]
+    r = torch.Generator().manual_seed(3)
+    T = sum(lens)
+    x = torch.randn((T, H * P), generator=r).cuda().to(torch.bfloat16)
+    BC = torch.randn((T, 2 * N), generator=r).cuda().to(torch.bfloat16)
+    dt = torch.randn((T, H), generator=r).cuda().to(torch.bfloat16)
+    A = -torch.rand(H, generator=r).cuda() - 0.1
+    starts = gpu(np.concatenate([[0], np.cumsum(lens)]), torch.int32)
+
+    def run(first, count, start, y):
+        o = lambda t: at(t) + first * t.shape[1] * 2
+        d = bh.Ssm(type=bh.BF16, n_heads=H, head_dim=P, n_groups=1, d_state=N, dt_softplus=1,
+                   n_seqs=n if start is not None else 1, n_tokens=count, seq_start=at(start),
+                   x=o(x), x_stride=H * P, B=o(BC), B_stride=2 * N, C=o(BC) + 2 * N,
+                   C_stride=2 * N, dt=o(dt), dt_stride=H, A=at(A), y=at(y), y_stride=H * P)
+        size = hip.bm_hip_ssm_workspace_bytes(C.byref(d))
+        work = torch.empty(size + 256, dtype=torch.uint8, device="cuda")
+        base = (work.data_ptr() + 255) // 256 * 256
+        note("scan of %d rows, workspace %d MB" % (count, size >> 20))
+        torch.cuda.synchronize()
+        bh.check(hip.bm_hip_ssm_dev(C.byref(d), C.c_void_p(base) if size else None, None))
+        torch.cuda.synchronize()
+
+    y = torch.zeros((T, H * P), dtype=torch.bfloat16, device="cuda")
+    run(0, T, starts, y)
+    # 3000 rows in units of 1344: three units to join
+    # the cut prompt by itself: the same sums in another cut, each y within a
+    # few roundings of the largest term; both are rounded to bf16
+    alone = torch.zeros((3000, H * P), dtype=torch.bfloat16, device="cuda")
+    run(n - 1, 3000, None, alone)
+    a, b = y[n - 1:].float(), alone.float()
+    scale = b.abs().amax(0, keepdim=True)
+    assert ((a - b).abs() <= 2 * 2.0 ** -8 * b.abs() + 2.0 ** -8 * scale).all()
+    # a prompt of one token: y = (C . B) softplus(dt) x, three factors in bf16
+    k = 17
+    want = ((BC[k, N:].double() @ BC[k, :N].double()) * torch.nn.functional.softplus(dt[k].double())
+            ).repeat_interleave(P) * x[k].double()
+    size = ((BC[k, N:].double().abs() @ BC[k, :N].double().abs())
+            * torch.nn.functional.softplus(dt[k].double())).repeat_interleave(P) * x[k].double().abs()
+    # the matrix operand M = C.B d has two bf16 pieces (2^-17 of it), sums of
+    # 128 fp32 products (2^-17 of the absolute sum), one rounding to bf16
+    assert ((y[k].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * size).all()

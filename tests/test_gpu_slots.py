@@ -155,3 +155,18 @@ def test_compact_of_an_empty_table(hip):
                                           at(work), None))
     torch.cuda.synchronize()
     assert t.tolist() == [0]
+
+
+def test_copy_of_more_blocks_than_a_grid_row(hip):
+    """1024 pairs leave a block four bytes of a slot: slots of 2^26 + 21 bytes
+    need more blocks than a launch has along x.  Two slots change places."""
+    n = (1 << 26) + 21
+    buf = torch.randint(0, 256, (2, n), dtype=torch.uint8, device="cuda")
+    want = buf.flip(0).clone()
+    src, dst = gpu(np.array([0, 1] + [-1] * 1022), torch.int32), gpu(np.array([1, 0] + [-1] * 1022), torch.int32)
+    d = bh.Slots(base=at(buf), n_slots=2, n_layers=1, slot_bytes=n, slot_stride=n, layer_stride=0)
+    note("copy of 2 x %d bytes" % n)
+    torch.cuda.synchronize()
+    bh.check(hip.bm_hip_slots_copy_dev(C.byref(d), 1, at(src), at(dst), 1024, None))
+    torch.cuda.synchronize()
+    assert torch.equal(buf, want)

@@ -164,3 +164,22 @@ def test_slot_lists_refused():
     assert L.bm_hip_slots_compact_workspace_bytes(0) == 0
     assert L.bm_hip_slots_compact_workspace_bytes(65537) == 0
     assert L.bm_hip_slots_compact_workspace_bytes(65536) > 0
+
+
+def test_new_table_overlapping_in_part_is_refused():
+    L = bh.lib()
+    p, d = C.c_void_p(P), C.byref(slots())
+    for shift in (-4, 4, 12):
+        refused(L.bm_hip_slots_compact_dev(d, 1, p, C.c_void_p(P + shift), 4, None, p, None),
+                "overlaps")
+
+
+@pytest.mark.parametrize("name", ["B", "C", "dt"])
+def test_step_over_an_input_that_other_channels_read_is_refused(name):
+    """y over x is allowed, but not where x is also B, C or dt."""
+    L = bh.lib()
+    p = C.c_void_p(P)
+    apart = {k: C.c_void_p(3 * P) for k in ("B", "C", "dt", "z")}  # the others' rows
+    d = ssm(n_heads=4, head_dim=1, n_groups=4, d_state=1, y=p, x_stride=64, y_stride=64,
+            **dict(apart, **{"x": p, name: p, name + "_stride": 64}))
+    refused(L.bm_hip_ssm_step_dev(C.byref(d), None), "overlaps " + name)
