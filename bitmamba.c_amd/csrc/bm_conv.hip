@@ -8,7 +8,10 @@
 // thread owns V neighbouring channels (16 bytes where the rows allow it) and
 // walks a unit of kConvRows rows with the window in registers; the rows of a
 // block's lanes are read whole, and each row is read 1 + (W - 1) / kConvRows
-// times, the repeats out of L2.
+// times, the repeats out of L2.  4096 rows of 4096 channels, fp32: 32 us, 135
+// MB at 4.2 TB/s; 1999 rows of 2307 channels, bf16, one channel per lane: 10
+// us.  Stores of y past the caches take 26 us for the first, but the call and
+// the scan that reads y then take 108 us together and not 105.
 #include "bm_seq.h"
 
 namespace bm {
@@ -150,7 +153,9 @@ __global__ __launch_bounds__(256) void k_conv(ConvArgs a) {
 
 // One token of each sequence: bound by its state rows, read and written; at
 // few sequences by one launch and the round trips slot -> rows.  A thread
-// takes SEQS sequences, so that its taps are loaded once for them.
+// takes SEQS sequences, so that its taps are loaded once for them.  4096
+// channels fp32, one sequence: 2.4 us; 4352 channels bf16, 512 sequences: 14.7
+// us, 62 MB at 4.3 TB/s.
 template <typename T, int W, int V, int SEQS>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs a) {
   const int c = (blockIdx.y * 256 + threadIdx.x) * V;

@@ -269,7 +269,17 @@ __device__ __forceinline__ int find_slot(const SeqView& q, int b, int first) {
                           : __builtin_amdgcn_readfirstlane(q.slots[b]);
   if (slot < 0 || slot >= q.n_slots) return kNoSlot;
   bool taken = lane < b && first == slot;
-  for (int j = lane + 64; j < b; j += 64) taken |= q.slots[j] == slot;
+  // Each block looks for itself, eight loads to a round trip: a step of the
+  // scan with 64 heads of 64 and one value takes 18 us with a list and 15
+  // without at 512 sequences, 180 and 94 at 4096 (272 by one load each).
+  constexpr int kAhead = 8;
+  for (int j = lane + 64; j < b; j += 64 * kAhead) {
+    int v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) v[k] = q.slots[min(j + 64 * k, b)];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) taken |= j + 64 * k < b && v[k] == slot;
+  }
   return __ballot(taken) ? kNoSlot : slot;
 }
 

@@ -48,6 +48,10 @@ bool check_seqs(const char* op, int n_seqs, int n_tokens, const int32_t* seq_sta
     bm_set_error("%s: %d sequences need seq_start", op, n_seqs);
     return false;
   }
+  if (state && slots && n_seqs > (1 << 16)) {  // each looks for its slot among those before it
+    bm_set_error("%s: a list of %d slots (up to 2^16)", op, n_seqs);
+    return false;
+  }
   if (((uintptr_t)seq_start | (uintptr_t)slots | (uintptr_t)state) % 4) {
     bm_set_error("%s: seq_start, slots and state need addresses on 4 bytes", op);
     return false;

@@ -346,7 +346,9 @@ int bm_hip_ternary_gemm_i32_dev(const int8_t *xq,
 /* - Tensors of the descriptor's `type` are read and written at any     */
 /*   row stride (in elements, below 2^24) and any element alignment;    */
 /*   everything is computed in fp32 or more, y is rounded once.         */
-/* - At most 2^20 sequences and 2^30 - 1 rows.                          */
+/* - At most 2^20 sequences and 2^30 - 1 rows; 2^16 sequences with a    */
+/*   list of slots, whose search for repeated entries grows with their  */
+/*   square (it is small up to about a thousand).                       */
 /* - Prompts are joined rows: sequence b has rows seq_start[b] ..       */
 /*   seq_start[b + 1] - 1 (device, n_seqs + 1 ascending entries;        */
 /*   NULL for one sequence of n_tokens rows).  Entries are clamped to   */

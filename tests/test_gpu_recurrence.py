@@ -421,3 +421,17 @@ def test_join_of_more_blocks_than_a_grid_row(hip):
     # the matrix operand M = C.B d has two bf16 pieces (2^-17 of it), sums of
     # 128 fp32 products (2^-17 of the absolute sum), one rounding to bf16
     assert ((y[k].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * size).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_repeated_slots_far_apart(hip, kind):
+    """Repeats at every distance that the search for them treats apart: below
+    64 entries, above, and past eight times 64."""
+    n = 1300
+    c = make(kind, [1] * n, step=True, seed=6)
+    for first, again in ((0, 63), (1, 64), (2, 65), (70, 575), (71, 576), (64, 577), (130, 1299),
+                         (1150, 1151), (640, 1200), (3, 1298)):
+        c.slots[again] = c.slots[first]
+    c.slots[5] = c.slots[900] = -1
+    note("%s, %d slots with repeats" % (kind, n))
+    c.check(hip, "repeats")

@@ -183,3 +183,12 @@ def test_step_over_an_input_that_other_channels_read_is_refused(name):
     d = ssm(n_heads=4, head_dim=1, n_groups=4, d_state=1, y=p, x_stride=64, y_stride=64,
             **dict(apart, **{"x": p, name: p, name + "_stride": 64}))
     refused(L.bm_hip_ssm_step_dev(C.byref(d), None), "overlaps " + name)
+
+
+def test_long_slot_lists_are_refused():
+    L = bh.lib()
+    n = (1 << 16) + 1
+    refused(L.bm_hip_conv_step_dev(C.byref(conv(n_seqs=n, n_slots=n)), None), "list")
+    refused(L.bm_hip_ssm_step_dev(C.byref(ssm(n_seqs=n, n_slots=n)), None), "list")
+    refused(L.bm_hip_conv_dev(C.byref(conv(n_seqs=n, n_slots=n)), None), "list")
+    refused(L.bm_hip_ssm_dev(C.byref(ssm(n_seqs=n, n_slots=n)), C.c_void_p(P), None), "list")
