@@ -1108,10 +1108,25 @@ static ScanPlan scan_plan(const bm_hip_ssm_t* op, size_t* bytes) {
   // no more places than sequences of two units can take
   const int64_t by_rows = 2 * (T / pl.len) + 2;
   pl.by_rows = by_rows < pl.units;
-  const int64_t places = pl.by_rows ? by_rows : pl.units;
-  const size_t ends = align_up((size_t)places * floats * 4, 256);
-  *bytes = pl.split ? ends + (size_t)places * op->n_heads * 4 : 0;
+  auto size_of = [&](int64_t places, size_t* ends) {
+    *ends = align_up((size_t)places * floats * 4, 256);
+    return *ends + (size_t)places * op->n_heads * 4;
+  };
+  size_t ends;
+  (void)size_of(pl.by_rows ? by_rows : pl.units, &ends);
   pl.decays = (float*)ends;  // its offset, until the workspace is known
+  // The size asked for is enough for any call of no more rows and sequences,
+  // of which shorter ones can take more places: len does not grow evenly.
+  // From its lines above T / len is at most `parts`, which, like the rule for
+  // whether a sequence can be cut, never falls as T or n_seqs grows.
+  const bool several = op->n_seqs > 1;
+  int64_t parts = several && T / 512 > want ? T / 512 : want;
+  if (parts > most_units) parts = most_units;
+  if (parts > T / least) parts = T / least;
+  const bool cut = T > least && (want > 1 || (several && T > 512));
+  const int64_t places = parts + op->n_seqs < 2 * parts + 2 ? parts + op->n_seqs : 2 * parts + 2;
+  size_t unused;
+  *bytes = cut ? size_of(places, &unused) : 0;
   return pl;
 }
 
@@ -1180,7 +1195,7 @@ static int ssm_call(const bm_hip_ssm_t* op, void* workspace, void* stream, bool 
   if (!step) {
     size_t bytes = 0;
     pl = bm::scan_plan(op, &bytes);
-    if (bytes && (!workspace || (uintptr_t)workspace % 256)) {
+    if (pl.split && (!workspace || (uintptr_t)workspace % 256)) {
       bm_set_error("%s: a workspace of %zu bytes on 256 bytes is required", name, bytes);
       return -2;
     }

@@ -1,0 +1,42 @@
+"""The batched recurrence where a call is at the edge of what it is documented
+to take: workspaces shared by calls of several sizes, kernels that only large
+calls reach, values at the end of a type's range.  The oracle is the definition
+in 64 bits with the bounds of tests/recurrence.py."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import native
+from native import bh
+from recurrence import ConvCase, SsmCase, at, check_rows, close, f64, gpu
+
+pytestmark = pytest.mark.gpu
+
+
+def note(msg):
+    print("[case] " + msg, flush=True)
+
+
+@pytest.mark.parametrize("shape,rows,most", [((64, 64, 64, 1), 1024, 2049),
+                                             ((2, 32, 1, 24), 4096, 4097)])
+def test_a_workspace_serves_shorter_prompts(hip, shape, rows, most):
+    """A workspace of the longest prompt's size, and a shorter one whose units
+    are more: right, and nothing behind the workspace is written."""
+    note("scan %s: %d rows in the workspace of %d" % (shape, rows, most))
+    c = SsmCase("f32", *shape, [rows], seed=2)
+    want, tols, pool, stol = c.want()
+    d = c.descriptor()
+    d.n_tokens = most
+    n = hip.bm_hip_ssm_workspace_bytes(C.byref(d))
+    d.n_tokens = rows
+    assert hip.bm_hip_ssm_workspace_bytes(C.byref(d)) <= n
+    work = torch.full((n + (1 << 20),), 0xFF, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    bh.check(hip.bm_hip_ssm_dev(C.byref(d), at(work), None))
+    torch.cuda.synchronize()
+    assert (work[n:] == 0xFF).all()
+    check_rows(c.ybuf, c.y, want, tols, "f32", (c.H, c.P), "shorter")
+    k = c.slots[0]
+    close(c.pool()[k], pool[k], stol[k], "f32", "state")
