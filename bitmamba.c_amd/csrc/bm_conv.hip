@@ -241,8 +241,8 @@ static int conv_call(const bm_hip_conv_t* op, void* stream, bool step) {
   if (!bm::check_seqs(name, op->n_seqs, op->n_tokens, op->seq_start, op->slots, op->state,
                       op->state_stride, op->n_slots, (int64_t)(op->width - 1) * op->channels,
                       step) ||
-      !bm::check_rows(name, "x", op->x, op->x_stride, op->channels, elem) ||
-      !bm::check_rows(name, "y", op->y, op->y_stride, op->channels, elem) ||
+      !bm::check_rows(name, "x", op->x, op->x_stride, op->channels, rows, elem) ||
+      !bm::check_rows(name, "y", op->y, op->y_stride, op->channels, rows, elem) ||
       !bm::check_apart(name, "x", op->x, op->x_stride, op->channels, op->y, op->y_stride,
                        op->channels, rows, elem, step))
     return -2;

@@ -303,7 +303,7 @@ class OnDevice {
 // Host checks shared by the descriptors; each sets the error and returns false.
 inline size_t type_bytes(int type) { return type == BM_HIP_F32 ? 4 : 2; }
 bool check_rows(const char* op, const char* name, const void* p, int64_t stride, int64_t width,
-                size_t elem);
+                int64_t rows, size_t elem);
 bool check_apart(const char* op, const char* name, const void* p, int64_t stride, int64_t width,
                  const void* y, int64_t y_stride, int64_t y_width, int64_t rows, size_t elem,
                  bool same_ok);

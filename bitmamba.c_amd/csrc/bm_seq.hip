@@ -8,8 +8,9 @@ hipStream_t stream_of(void* stream) {
 }
 
 bool check_rows(const char* op, const char* name, const void* p, int64_t stride, int64_t width,
-                size_t elem) {
-  if (!p || (uintptr_t)p % elem || stride < width || stride >= (1 << 24)) {
+                int64_t rows, size_t elem) {
+  // without rows nothing is read or written: an empty tensor's address may be null
+  if ((!p && rows > 0) || (uintptr_t)p % elem || stride < width || stride >= (1 << 24)) {
     bm_set_error("%s: %s needs an address on %zu bytes and a row stride of %lld to 2^24 - 1 (%lld)", op,
                  name, elem, (long long)width, (long long)stride);
     return false;

@@ -1179,10 +1179,10 @@ static int ssm_call(const bm_hip_ssm_t* op, void* workspace, void* stream, bool 
             {"C", op->C, op->C_stride, gn},
             {"dt", op->dt, op->dt_stride, op->n_heads},
             {"z", op->z, op->z_stride, hp}};
-  if (!bm::check_rows(name, "y", op->y, op->y_stride, hp, elem)) return -2;
+  if (!bm::check_rows(name, "y", op->y, op->y_stride, hp, rows, elem)) return -2;
   for (const auto& t : in) {
     if (!op->z && &t == &in[4]) continue;  // no gate
-    if (!bm::check_rows(name, t.name, t.p, t.stride, t.width, elem) ||
+    if (!bm::check_rows(name, t.name, t.p, t.stride, t.width, rows, elem) ||
         !bm::check_apart(name, t.name, t.p, t.stride, t.width, op->y, op->y_stride, hp, rows, elem,
                          step && (&t == &in[0] || (&t == &in[4] && op->z == op->x))))
       return -2;

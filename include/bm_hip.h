@@ -353,6 +353,8 @@ int bm_hip_ternary_gemm_i32_dev(const int8_t *xq,
 /*   seq_start[b + 1] - 1 (device, n_seqs + 1 ascending entries;        */
 /*   NULL for one sequence of n_tokens rows).  Entries are clamped to   */
 /*   0..n_tokens.  Rows that belong to no sequence are not touched.     */
+/*   A call without rows still starts fresh sequences' slots; x, y and  */
+/*   the other tensors with a row per token may then be NULL.           */
 /* - Single tokens (_step): row b is the next token of sequence b;      */
 /*   seq_start, fresh and n_tokens are not read.                        */
 /* - The state of sequence b is slot slots[b] of the pool (device;      */

@@ -40,3 +40,21 @@ def test_a_workspace_serves_shorter_prompts(hip, shape, rows, most):
     check_rows(c.ybuf, c.y, want, tols, "f32", (c.H, c.P), "shorter")
     k = c.slots[0]
     close(c.pool()[k], pool[k], stol[k], "f32", "state")
+
+
+@pytest.mark.parametrize("N", [0, 1, 24])
+def test_calls_without_rows(hip, N):
+    """Prompts without a row and tensors without an address: a fresh
+    sequence's slot becomes zero, the others stay (N 0: the convolution)."""
+    note("no rows, N=%d" % N)
+    c = SsmCase("f32", 4, 40, 2, N, [0] * 3, seed=1) if N else ConvCase("f32", 130, 4, [0] * 3, seed=1)
+    c.fresh = [0, 1, 0]
+    d = c.descriptor()
+    for f in ["x", "y"] + (["B", "C", "dt", "z"] if N else []):
+        setattr(d, f, None)
+    want = c.pool_buf.clone()
+    want[c.slots[1]] = 0.0
+    torch.cuda.synchronize()
+    bh.check(hip.bm_hip_ssm_dev(C.byref(d), None, None) if N else hip.bm_hip_conv_dev(C.byref(d), None))
+    torch.cuda.synchronize()
+    assert torch.equal(c.pool_buf, want)

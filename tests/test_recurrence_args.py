@@ -192,3 +192,20 @@ def test_long_slot_lists_are_refused():
     refused(L.bm_hip_ssm_step_dev(C.byref(ssm(n_seqs=n, n_slots=n)), None), "list")
     refused(L.bm_hip_conv_dev(C.byref(conv(n_seqs=n, n_slots=n)), None), "list")
     refused(L.bm_hip_ssm_dev(C.byref(ssm(n_seqs=n, n_slots=n)), C.c_void_p(P), None), "list")
+
+
+def test_calls_without_rows_need_no_addresses():
+    """An empty tensor's address may be null: no prompt rows, no sequences.
+    Alignment and strides are still looked at."""
+    L = bh.lib()
+    none = dict(x=None, y=None)
+    more = dict(none, B=None, C=None, dt=None, z=None)
+    assert L.bm_hip_conv_step_dev(C.byref(conv(n_seqs=0, **none)), None) == 0
+    assert L.bm_hip_ssm_step_dev(C.byref(ssm(n_seqs=0, **more)), None) == 0
+    assert L.bm_hip_conv_dev(C.byref(conv(n_seqs=0, n_tokens=0, **none)), None) == 0
+    assert L.bm_hip_ssm_dev(C.byref(ssm(n_seqs=0, n_tokens=0, **more)), None, None) == 0
+    refused(L.bm_hip_conv_dev(C.byref(conv(n_tokens=0, x=None, y=P + 2)), None), "y needs")
+    refused(L.bm_hip_ssm_dev(C.byref(ssm(n_tokens=0, **dict(more, B_stride=15))), None, None), "B needs")
+    if not L.bm_hip_available():  # past the checks: no GPU here
+        assert L.bm_hip_conv_dev(C.byref(conv(n_tokens=0, **none)), None) == -1
+        assert L.bm_hip_ssm_dev(C.byref(ssm(n_tokens=0, **more)), None, None) == -1
