@@ -193,15 +193,11 @@ template <typename T, int W, int V>
 static hipError_t launch_conv(const ConvArgs& a, bool step, hipStream_t s) {
   const unsigned gy = (unsigned)((a.channels + 256 * V - 1) / (256 * V));
   if (step && (int64_t)a.q.n_seqs * gy >= 1024)  // one thread's work for four still fills the chip
-    hipLaunchKernelGGL((k_conv_step<T, W, V, kConvSeqs>),
-                       dim3((a.q.n_seqs + kConvSeqs - 1) / kConvSeqs, gy), dim3(256), 0, s, a);
-  else if (step)
-    hipLaunchKernelGGL((k_conv_step<T, W, V, 1>), dim3(a.q.n_seqs, gy), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_conv<T, W, V>),
-                       wide_grid(unit_count(a.q.n_seqs, a.q.n_tokens, kConvRows), gy), dim3(256), 0,
-                       s, a);
-  return hipGetLastError();
+    return launch(k_conv_step<T, W, V, kConvSeqs>,
+                  dim3((a.q.n_seqs + kConvSeqs - 1) / kConvSeqs, gy), dim3(256), 0, s, a);
+  if (step) return launch(k_conv_step<T, W, V, 1>, dim3(a.q.n_seqs, gy), dim3(256), 0, s, a);
+  return launch(k_conv<T, W, V>, wide_grid(unit_count(a.q.n_seqs, a.q.n_tokens, kConvRows), gy),
+                dim3(256), 0, s, a);
 }
 
 template <typename T, int V>

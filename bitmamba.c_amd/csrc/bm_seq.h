@@ -2,6 +2,8 @@
 // of a call, the sequences' state slots, and the fp32 functions of the block.
 #pragma once
 
+#include <tuple>
+
 #include "bm_common.h"
 #include "bm_hip.h"
 
@@ -299,6 +301,18 @@ class OnDevice {
  private:
   int was_ = 0;
 };
+
+// A launch by its own status: an error that an earlier call of the caller's
+// left in this thread is not this one's.  The arguments are converted to the
+// kernel's parameters.
+template <typename... P, typename... A>
+inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s,
+                         const A&... args) {
+  std::tuple<P...> v(static_cast<P>(args)...);
+  void* p[sizeof...(P)];
+  std::apply([&](auto&... e) { size_t i = 0; ((p[i++] = (void*)&e), ...); }, v);
+  return hipLaunchKernel((const void*)kernel, grid, block, p, lds, s);
+}
 
 // Host checks shared by the descriptors; each sets the error and returns false.
 inline size_t type_bytes(int type) { return type == BM_HIP_F32 ? 4 : 2; }

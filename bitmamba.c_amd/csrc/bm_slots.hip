@@ -103,9 +103,8 @@ static hipError_t launch_copy_e(const PoolView& p, int n_layers, int n_slots, co
   while ((1 << lh) < 2 * n) ++lh;
   const int64_t blocks = (words + ((int64_t)1 << lc) - 1) >> lc;
   if (blocks > kGridX * 65535) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_slots_copy<W, E>), wide_grid(blocks, n_layers), dim3(256), 0, s, p, n_slots,
-                     src, dst, n, lc, lh);
-  return hipGetLastError();
+  return launch(k_slots_copy<W, E>, wide_grid(blocks, n_layers), dim3(256), 0, s, p, n_slots, src,
+                dst, n, lc, lh);
 }
 
 // Words per thread: as many as leave the chip at least two workgroups per CU,
@@ -249,9 +248,8 @@ static hipError_t launch_move(const PoolView& p, int n_layers, int n_slots, int 
   const int64_t words = p.slot_bytes / (int64_t)sizeof(W);
   const int64_t runs = (words + 1023) / 1024 * n_layers;
   const int64_t total = runs > 4096 ? 4096 : runs * most;
-  hipLaunchKernelGGL((k_slots_move<W>), dim3((unsigned)(total < 4096 ? total : 4096)), dim3(256),
-                     0, s, p, n_layers, n_slots, mv);
-  return hipGetLastError();
+  return launch(k_slots_move<W>, dim3((unsigned)(total < 4096 ? total : 4096)), dim3(256), 0, s, p,
+                n_layers, n_slots, mv);
 }
 
 static bool pools_fit(const char* name, const bm_hip_slots_t* pools, int n_pools) {
@@ -335,9 +333,9 @@ extern "C" int bm_hip_slots_compact_dev(const bm_hip_slots_t* pools, int n_pools
   bm::OnDevice dev;
   hipStream_t s = bm::stream_of(stream);
   bm::Moves* mv = (bm::Moves*)workspace;
-  hipLaunchKernelGGL(bm::k_slots_plan, dim3(1), dim3(1024), 0, s, slots, new_slots, n, n_slots,
-                     n_live, mv);
-  BM_HIP_CHECK_RET(hipGetLastError(), -1);
+  BM_HIP_CHECK_RET(bm::launch(bm::k_slots_plan, dim3(1), dim3(1024), 0, s, slots, new_slots, n,
+                              n_slots, n_live, mv),
+                   -1);
   const int most = n < n_slots / 2 ? n : n_slots / 2;  // moves: live ones above as many free ones
   if (most == 0) return 0;
   for (int i = 0; i < n_pools; ++i) {

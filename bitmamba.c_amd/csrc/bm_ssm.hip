@@ -138,10 +138,8 @@ static hipError_t launch_step(const SsmArgs& a, hipStream_t s) {
   // against 42.9 us at 100 MB, 16.5 against 13.6 us at 34 MB)
   constexpr bool kLarge = V == 4 && TEAM >= 4;
   if (kLarge && (int64_t)a.q.n_seqs * a.heads * a.hd * a.n >= (1 << 24))
-    hipLaunchKernelGGL((k_ssm_step<T, TEAM, V, E, U, kLarge>), grid, dim3(64 * nw), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_ssm_step<T, TEAM, V, E, U, false>), grid, dim3(64 * nw), 0, s, a);
-  return hipGetLastError();
+    return launch(k_ssm_step<T, TEAM, V, E, U, kLarge>, grid, dim3(64 * nw), 0, s, a);
+  return launch(k_ssm_step<T, TEAM, V, E, U, false>, grid, dim3(64 * nw), 0, s, a);
 }
 
 template <typename T>
@@ -402,10 +400,12 @@ static hipError_t launch_small(const SsmArgs& a, const ScanPlan& pl, hipStream_t
     if (raised[1] != hipSuccess) return raised[1];
   }
   const dim3 grid((unsigned)pl.units, by);
-  if (pl.split)
-    hipLaunchKernelGGL((k_scan_small<T, NS, false>), grid, dim3(64), bytes, s, a, pl, heads_max);
-  hipLaunchKernelGGL((k_scan_small<T, NS, true>), grid, dim3(64), bytes, s, a, pl, heads_max);
-  return hipGetLastError();
+  if (pl.split) {
+    const hipError_t e =
+        launch(k_scan_small<T, NS, false>, grid, dim3(64), bytes, s, a, pl, heads_max);
+    if (e != hipSuccess) return e;
+  }
+  return launch(k_scan_small<T, NS, true>, grid, dim3(64), bytes, s, a, pl, heads_max);
 }
 
 template <typename T>
@@ -1050,17 +1050,17 @@ static hipError_t launch_mm(const SsmArgs& a, const ScanPlan& pl, hipStream_t s)
     if (raised[1] != hipSuccess) return raised[1];
   }
   if (pl.split) {
-    hipLaunchKernelGGL((k_scan_mm<T, NT, false>), grid, dim3(64 * kWaves), bytes, s, a, pl, tiles,
-                       wide);
+    hipError_t e =
+        launch(k_scan_mm<T, NT, false>, grid, dim3(64 * kWaves), bytes, s, a, pl, tiles, wide);
+    if (e != hipSuccess) return e;
     const int head = mm_ptiles(a.hd) * NT * 1024;
     const int64_t floats = (int64_t)a.heads * head;
     const int blocks = (int)((floats / 4 + 255) / 256);
-    hipLaunchKernelGGL(k_scan_join, wide_grid(pl.units * blocks, 1), dim3(256), 0, s, a.q, pl,
-                       floats, blocks, head, a.heads);
+    e = launch(k_scan_join, wide_grid(pl.units * blocks, 1), dim3(256), 0, s, a.q, pl, floats,
+               blocks, head, a.heads);
+    if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((k_scan_mm<T, NT, true>), grid, dim3(64 * kWaves), bytes, s, a, pl, tiles,
-                     wide);
-  return hipGetLastError();
+  return launch(k_scan_mm<T, NT, true>, grid, dim3(64 * kWaves), bytes, s, a, pl, tiles, wide);
 }
 
 template <typename T>

@@ -58,3 +58,52 @@ def test_calls_without_rows(hip, N):
     bh.check(hip.bm_hip_ssm_dev(C.byref(d), None, None) if N else hip.bm_hip_conv_dev(C.byref(d), None))
     torch.cuda.synchronize()
     assert torch.equal(c.pool_buf, want)
+
+
+@pytest.mark.parametrize("kind", ["conv", "conv_step", "scan1", "scan24", "step", "slots"])
+def test_an_error_pending_is_not_the_calls(hip, kind):
+    """A call does not fail for an error that the caller's own earlier HIP call
+    left in the thread, and leaves it there."""
+    rt = C.CDLL("libamdhip64.so")
+    if kind == "slots":
+        pool = torch.arange(8 * 16, dtype=torch.float32, device="cuda").view(8, 16)
+        want = pool.clone()
+        want[2] = pool[5]
+        want[0], want[1] = want[2], want[7]
+        d = bh.Slots(base=at(pool), n_slots=8, n_layers=1, slot_bytes=64, slot_stride=64)
+        src, dst = gpu(np.array([5]), torch.int32), gpu(np.array([2]), torch.int32)
+        table = gpu(np.array([2, 7]), torch.int32)
+        work = torch.zeros(hip.bm_hip_slots_compact_workspace_bytes(8), dtype=torch.uint8,
+                           device="cuda")
+        f = lambda: (hip.bm_hip_slots_copy_dev(C.byref(d), 1, at(src), at(dst), 1, None) or
+                     hip.bm_hip_slots_compact_dev(C.byref(d), 1, at(table), at(table), 2, None,
+                                                  at(work), None))
+    else:
+        c = {"conv": lambda: ConvCase("f32", 64, 4, [40]),
+             "conv_step": lambda: ConvCase("f32", 64, 4, [1] * 3, step=True),
+             "scan1": lambda: SsmCase("f32", 2, 32, 2, 1, [300]),
+             "scan24": lambda: SsmCase("f32", 2, 32, 2, 24, [300]),
+             "step": lambda: SsmCase("f32", 2, 32, 2, 24, [1] * 3, step=True)}[kind]()
+        rows, tols = c.want()[:2]
+        d = c.descriptor()
+        if kind.startswith("conv"):
+            call = hip.bm_hip_conv_step_dev if c.step else hip.bm_hip_conv_dev
+            f = lambda: call(C.byref(d), None)
+        elif c.step:
+            f = lambda: hip.bm_hip_ssm_step_dev(C.byref(d), None)
+        else:
+            w = c.workspace(hip, d)
+            f = lambda: hip.bm_hip_ssm_dev(C.byref(d), w, None)
+    torch.cuda.synchronize()
+    note("%s with an error pending" % kind)
+    refused = rt.hipMalloc(None, C.c_size_t(16))  # on the host: no pointer to fill
+    assert refused != 0
+    rc = f()
+    assert rt.hipGetLastError() == refused
+    assert rc == 0, bh.last_error()
+    torch.cuda.synchronize()
+    if kind == "slots":
+        assert torch.equal(pool, want) and table.tolist() == [0, 1]
+    else:
+        shape = (64,) if kind.startswith("conv") else (c.H, c.P)
+        check_rows(c.ybuf, c.y, rows, tols, "f32", shape, kind)
