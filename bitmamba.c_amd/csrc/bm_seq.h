@@ -167,6 +167,27 @@ __device__ __forceinline__ float exp_f32(float x) {
   const float r = e * __builtin_fmaf(lo, 0x1.62e43p-1f, 1.0f);
   return __builtin_fabsf(hi) < 256.0f ? r : e;
 }
+// exp(p) as hi, the nearest float, and lo, what that leaves, for a state that is
+// multiplied by it row after row: the hardware's exponential is 0.12 units of
+// 2^-24 too small on average just below 1, and even a rounded one keeps
+// 2^-25 / (1 - a) of a steady state's value.  Below |p| = 1/16, where a decay's
+// error outlives a few rows, exp(p) - 1 = p + (p^2 / 2 + p^3 / 6 + p^4 / 24), off
+// by p^5 / 120 < 2^-26; above it lo is 0.
+struct Decay {
+  float hi, lo;
+};
+__device__ __forceinline__ Decay decay_of(float p) {
+  const float t = __builtin_fmaf(__builtin_fmaf(p, 1.0f / 24.0f, 1.0f / 6.0f), p, 0.5f);
+  const float s = p * p * t, m = p + s;  // |p| > |s| where neither is zero
+  const float near1 = 1.0f + m, far = exp_f32(p);
+  const bool near = __builtin_fabsf(p) < 0.0625f;
+  return Decay{near ? near1 : far, near ? (m - (near1 - 1.0f)) + (s - (m - p)) : 0.0f};
+}
+// add + s lo, an infinite s left to the product with hi
+__device__ __forceinline__ float with_low(float s, float lo, float add) {
+  constexpr float kMax = 0x1.fffffep127f;
+  return __builtin_fmaf(__builtin_amdgcn_fmed3f(s, -kMax, kMax), lo, add);
+}
 __device__ __forceinline__ float silu_f32(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + exp_f32(-x));
 }

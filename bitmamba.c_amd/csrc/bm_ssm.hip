@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs a) {
   if (slot == kNoSlot) return;
   const int g = h / (a.heads / a.groups);
   const float d = step_of(a, (float)((const T*)a.dt)[(int64_t)b * a.dts + h], bias_of(a, h));
-  const float decay = exp_f32(a.A[h] * d);
+  const Decay decay = decay_of(a.A[h] * d);
   // the head's part of the slot, of x, z and y; what lies past them reads as
   // zeros and is not written
   const auto st = rows_at(a.state + (slot >= 0 ? (int64_t)slot * a.ss : 0) + (int64_t)h * a.hd * a.n,
@@ -111,7 +111,8 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs a) {
       const int n = nl + e * TEAM * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        s[u][e][i] = __builtin_fmaf(s[u][e][i], decay, xf * Bv[e][i]);
+        s[u][e][i] = __builtin_fmaf(s[u][e][i], decay.hi,
+                                    with_low(s[u][e][i], decay.lo, xf * Bv[e][i]));
         // beyond d_state nothing counts, even where x or the decay is infinite
         if (E * TEAM * V > 1 && (V == 1 || E > 1)) s[u][e][i] = n + i < a.n ? s[u][e][i] : 0.0f;
         sum = __builtin_fmaf(s[u][e][i], Cv[e][i], sum);
@@ -221,11 +222,13 @@ __device__ __forceinline__ bool scan_unit(const SeqView& q, int index, const Sca
 // the loads of a tile of kSmallRows rows are all issued before any is used,
 // and the next tile's while one is worked on.  At 64 heads of 64 channels and
 // one value, fp32, 1024 rows: 8 and 16 us for the two passes, 51 MB at 2.2
-// TB/s; 6001 rows of 32 heads 54 us, 2.8 TB/s (tiles of 8 and 32 rows: 73 and
+// TB/s; 6001 rows of 32 heads 55 us, 2.7 TB/s (tiles of 8 and 32 rows: 73 and
 // 69 us; two or four channels per lane: 72 and 103).
 constexpr int kSmallState = 8;
 constexpr int kSmallRows = 16;
-__host__ __device__ constexpr int small_entry(int ns) { return (1 + 2 * ns + 3) / 4 * 4; }
+// of a row and head in LDS: decay, d B, C (in the first pass the exponent A d),
+// and last the decay's low part
+__host__ __device__ constexpr int small_entry(int ns) { return (2 + 2 * ns + 3) / 4 * 4; }
 
 template <typename T, int NS, bool FULL>
 __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int heads_max) {
@@ -312,7 +315,7 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
   }
 
   const float D = FULL && on && a.D ? a.D[c] : 0.0f;
-  float all = 1.0f;  // the unit's decay
+  double total = 0.0;  // of the unit's exponents: its decay is rounded once
   for (int t = w.t0; t < w.t1; t += tile) {
     const int rows = min(tile, w.t1 - t);
     for (int i = lane; i < tile * nh; i += 64) {
@@ -328,7 +331,11 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
       const int g = (h0 + hh) / per;
       const float d = step_of(a, (float)((const T*)a.dt)[row * a.dts + h0 + hh],
                               bias_of(a, h0 + hh));
-      s[0] = exp_f32(a.A[h0 + hh] * d);
+      const float Ad = a.A[h0 + hh] * d;
+      const Decay decay = decay_of(Ad);
+      s[0] = decay.hi;
+      s[EW - 1] = decay.lo;
+      if (!FULL) s[1 + NS] = Ad;
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         const bool have = n < a.n;
@@ -346,6 +353,7 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
     }
     if (t + tile < w.t1) fetch(t + tile);
     const auto by = rows_of<T>(a.y, t, a.ys, rows);
+    float exponents = 0.0f, low = 0.0f;  // the tile's sums
 #pragma unroll
     for (int r = 0; r < tile; ++r) {
       float e[EW];
@@ -360,12 +368,20 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
         if (NS > 2) S[n] = n < a.n ? S[n] : 0.0f;
         if (FULL) y = __builtin_fmaf(S[n], e[1 + NS + n], y);
       }
-      all *= e[0];
+      low += e[EW - 1];
+      if (!FULL) exponents += e[1 + NS];
       if (FULL) {
         const float out[1] = {y * z[r]};
         store_row<T, 1>(by, col + r * ys, out);
       }
     }
+    // The tile's decays were the nearest floats.  What that left of them: for
+    // the state from before the tile all of it, for what its rows added up to
+    // 16 halves of 2^-24 too much (a second product per row instead takes 57.5
+    // against 56.0 us at 4 values, fp16, 6000 rows of 32 heads of 64).
+#pragma unroll
+    for (int n = 0; n < NS; ++n) S[n] = with_low(S[n], low, S[n]);
+    if (!FULL) total += (double)exponents;
     __syncthreads();
   }
   if (!on) return;
@@ -374,7 +390,10 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
 #pragma unroll
     for (int n = 0; n < NS; ++n)
       if (n < a.n) e[(int64_t)n * channels] = S[n];
-    if (c % a.hd == 0) pl.decays[unit * a.heads + h] = all;
+    if (c % a.hd == 0) {
+      const Decay all = decay_of((float)total);
+      pl.decays[unit * a.heads + h] = all.hi + all.lo;
+    }
   } else if (w.slot >= 0 && w.u.k == w.last) {
     float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
 #pragma unroll

@@ -107,3 +107,80 @@ def test_an_error_pending_is_not_the_calls(hip, kind):
     else:
         shape = (64,) if kind.startswith("conv") else (c.H, c.P)
         check_rows(c.ybuf, c.y, rows, tols, "f32", shape, kind)
+
+
+# ---------------------------------------------------------------------------
+# a state that decays over thousands of tokens.  u = 2^-24.
+# ---------------------------------------------------------------------------
+def bare_state(H, N, T, rates, step):
+    """States of 1 and no input, one channel per head: what is left after T
+    tokens is the decays' product."""
+    c = SsmCase("f32", H, 1, 1, N, [1] if step else [T], gate=False, skip=False, bias=False,
+                soft=False, step=step, slots=None, spare=0)
+    c.x.zero_()
+    c.dt.fill_(1.0)
+    c.A = gpu(-rates, torch.float32)
+    c.pool_buf.fill_(1.0)
+    return c
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("N", [1, 2, 4, 5, 24])
+def test_one_decay(hip, N, step):
+    """The decay of one token, rates from 2^-20 to 2^-5: rounded to nearest, off
+    by u / 2 for values from 1/2 to 1; the sum p^2 / 2 + ... in front of it has
+    three roundings of less than 2^-11, u / 100 at most with the series's rest.
+    From 9 values on the scan's own operands have three bf16 pieces, off by u,
+    and the hardware's exponential is good to u."""
+    rates = np.exp2(np.linspace(-20, -5, 4096))
+    c = bare_state(4096, N, 1, rates, step)
+    note("one decay, N=%d step=%s" % (N, step))
+    want = np.exp(f64(c.A))
+    c.run(hip)
+    err = (c.pool()[0].reshape(4096, N) - want[:, None]) * 2.0 ** 24
+    lim = 0.51 if step or N <= 8 else 2.0
+    assert np.abs(err).max() <= lim
+    if step or N <= 8:
+        # 4096 errors of at most 0.51 each about zero: their mean is off by
+        # 0.04 once in exp(2 (0.04 4096)^2 / (4096 1.02^2)) > 10^5 such tests
+        assert abs(err.mean()) <= 0.04
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("N", [1, 5])
+def test_a_slow_state_keeps_its_value(hip, N, step):
+    """T tokens of a rate of about 2^-10.  Every token rounds the state once,
+    by u at most and to either side: T such errors sum up to more than 6 sqrt(T)
+    u once in exp(6^2 / 2) / 2 > 10^7 states; a decay that is 0.12 u too
+    small in every token would leave 0.12 T u, nearly twice as much.  The scan
+    joins up to 64 units of equal decays, each rounded once: 64 u for these,
+    64 u for the products, and the last unit's tokens: less than that."""
+    T, H = 8192, 64
+    rates = np.exp2(np.linspace(-10.5, -9.5, H))
+    c = bare_state(H, N, T, rates, step)
+    note("slow state, N=%d step=%s" % (N, step))
+    want = np.exp(T * f64(c.A))
+    if step:
+        d = c.descriptor()
+        torch.cuda.synchronize()
+        for _ in range(T):
+            bh.check(hip.bm_hip_ssm_step_dev(C.byref(d), None))
+        torch.cuda.synchronize()
+    else:
+        c.run(hip)
+    err = (c.pool()[0].reshape(H, N) / want[:, None] - 1.0) * 2.0 ** 24
+    assert np.abs(err).max() <= 6 * T ** 0.5
+
+
+@pytest.mark.parametrize("N", [1, 2, 3, 8])
+def test_an_infinite_state_stays_infinite(hip, N):
+    """An infinite state under finite inputs and decays, over units that end
+    within a tile of rows, and by single tokens."""
+    for lens, step in (([37, 16, 1], False), ([1] * 3, True)):
+        c = SsmCase("f32", 2, 20, 1, N, lens, slots=None, spare=0, seed=N, step=step)
+        c.A = gpu(np.array([-1e-6, -2.0]), torch.float32)
+        c.pool_buf[1, :] = float("inf")
+        note("infinite state, N=%d step=%s" % (N, step))
+        c.run(hip)
+        p = c.pool()
+        assert np.isposinf(p[1]).all() and np.isfinite(p[[0, 2]]).all()
