@@ -512,8 +512,10 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
 //
 // Causality holds for infinities and NaN too: a product takes 0 for M above
 // the diagonal, and 0 times such an x would reach earlier rows, so x enters
-// that product as 0 and the rows from it on become NaN.
+// that product as 0 and the rows from it on become NaN.  An fp32 x whose first
+// piece is infinite (kInfinite and more) is treated the same.
 constexpr int kQ = 32, kWaves = 4;
+constexpr float kInfinite = 0x1.ffp127f;  // rounds to an infinite bf16
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -937,15 +939,17 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = raw_f32<T>(nx[r]);
       int first = kQ;
-      float probe = 0.0f;  // NaN once any x is not finite
+      // Not finite once any x is not, or is fp32 past bf16's range: at 4 x no
+      // finite sum before it keeps such a one from overflowing.
+      float probe = 0.0f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) probe = __builtin_fmaf(x[r], 0.0f, probe);
-      const bool odd = __ballot(probe != probe) != 0;
+      for (int r = 0; r < 16; ++r) probe = __builtin_fmaf(x[r], IN == 3 ? 4.0f : 0.0f, probe);
+      const bool odd = __ballot(!(__builtin_fabsf(probe) < __builtin_inff())) != 0;
       if (odd) {
         asm volatile("");  // a branch, not selects
 #pragma unroll
         for (int r = 15; r >= 0; --r)
-          if (!(__builtin_fabsf(x[r]) < __builtin_inff())) {
+          if (!(__builtin_fabsf(x[r]) < kInfinite)) {
             first = acc_row(r, half);
             x[r] = 0.0f;
           }

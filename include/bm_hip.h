@@ -401,7 +401,10 @@ int bm_hip_conv_step_dev(const bm_hip_conv_t *op, void *stream);
 
 /* Per head h of group g = h / (n_heads / n_groups), with d = dt[t][h] +
  * dt_bias[h], taken through log(1 + exp(d)) if dt_softplus, and a =
- * exp(A[h] * d):
+ * exp(A[h] * d).  A channel whose x is infinite or NaN is one of the two
+ * from that row on; earlier rows, other channels and sequences are not
+ * reached.  With d_state > 8, fp32 values of 2^128 - 2^119 and more count
+ * as infinite.
  *   S[p][n] = a * S[p][n] + d * x[t][h][p] * B[t][g][n]
  *   y[t][h][p] = (sum_n C[t][g][n] * S[p][n] + D[h][p] * x[t][h][p])
  *                * z[t][h][p] / (1 + exp(-z[t][h][p])) */

@@ -184,3 +184,31 @@ def test_an_infinite_state_stays_infinite(hip, N):
         c.run(hip)
         p = c.pool()
         assert np.isposinf(p[1]).all() and np.isfinite(p[[0, 2]]).all()
+
+
+@pytest.mark.parametrize("N", [5, 24, 128])
+@pytest.mark.parametrize("value", [3.4e38, float(np.finfo(np.float32).min), 1e38])
+def test_the_largest_floats_do_not_reach_earlier_rows(hip, N, value):
+    """A finite x at the end of fp32's range, past what a bf16 holds: earlier
+    rows, other channels and other sequences are bit for bit what they were.
+    Where it is within that range (1e38) or the state has up to 8 values, its
+    own row is right, too."""
+    H, P, lens, row, ch = 2, 40, [37, 90, 20], 37 + 50, 47
+    def case():
+        return SsmCase("f32", H, P, 1, N, lens, seed=9, gate=False, skip=False, soft=False)
+    clean, c = case(), case()
+    clean.run(hip)
+    c.x[row, ch] = value
+    note("x = %g, N=%d" % (value, N))
+    with np.errstate(over="ignore"):
+        rows, tols = c.want()[:2]
+    c.run(hip)
+    y0, y1 = f64(clean.y), f64(c.y)
+    keep = [r for r in range(sum(lens)) if r < row or r >= 37 + 90]
+    assert np.array_equal(y0[keep], y1[keep])
+    rest = [k for k in range(H * P) if k != ch]
+    assert np.array_equal(y0[row:37 + 90, rest], y1[row:37 + 90, rest])
+    for b in (0, 2):
+        assert np.array_equal(clean.pool()[c.slots[b]], c.pool()[c.slots[b]])
+    if N <= 8 or abs(value) < 3.3e38:
+        close(y1[row, ch], rows[row].reshape(-1)[ch], tols[row].reshape(-1)[ch], "f32", "its row")
