@@ -151,7 +151,7 @@ struct Moves {
 };
 __host__ __device__ inline int moves_cap(int n_slots) { return n_slots / 2 + 1; }
 
-__global__ __launch_bounds__(1024) void k_slots_plan(const int32_t* __restrict__ slots,
+__global__ __launch_bounds__(1024) void k_slots_plan(const int32_t* slots,
                                                      int32_t* new_slots, int n, int n_slots,
                                                      int32_t* n_live, Moves* mv) {
   constexpr int kWords = kMaxCompact / 32;
