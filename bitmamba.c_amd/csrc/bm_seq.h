@@ -191,7 +191,8 @@ __device__ __forceinline__ float with_low(float s, float lo, float add) {
 __device__ __forceinline__ float silu_f32(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + exp_f32(-x));
 }
-// the same to 2^-20, for what is rounded to bf16
+// the same to 2^-20 for |x| up to 8 and to |x| 2^-23 above, for what is rounded
+// to bf16
 __device__ __forceinline__ float silu_short(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e));
 }

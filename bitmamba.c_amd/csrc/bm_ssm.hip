@@ -496,8 +496,8 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
 // two, bf16 as one, all exact; of the products of two such sums those above
 // 2^-24 of the whole are kept (piece indices that add up to less than 3), and
 // everything is accumulated in fp32.  For a bf16 y the computed operands S and
-// M have two pieces (off by 2^-18, against y's rounding of 2^-9); the state
-// itself always gets three.
+// M have two pieces (off by 2^-18) and the gate a short exponential (silu_short),
+// against y's rounding of 2^-9; the state itself always gets three pieces.
 //
 // Layouts (lane l, half h = l / 32; accumulator r of a 32x32 tile is row
 // 8 (r / 4) + 4 h + r % 4, column l % 32).  The k order of a product is free
@@ -956,7 +956,7 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
         first = min(first, __shfl_xor(first, 32));
         if (first < kQ) eall = __builtin_nanf("");
       }
-      const float hi = shHi[li], lo = kExact ? shLo[li] : 0.0f;
+      const float hi = shHi[li], lo = shLo[li];
       const int diag = (int)here((uint32_t)(li - 4 * half));
       float m[16];
 #pragma unroll
@@ -969,9 +969,7 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
                     l4[4] = {jl.x, jl.y, jl.z, jl.w}, d4[4] = {jd.x, jd.y, jd.z, jd.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          // for a bf16 y the first parts' difference is exact enough: sums of
-          // up to 2^13, off by 2^-12 each
-          const float e = __builtin_amdgcn_exp2f(kExact ? (hi - h4[i]) + (lo - l4[i]) : hi - h4[i]);
+          const float e = __builtin_amdgcn_exp2f((hi - h4[i]) + (lo - l4[i]));
           float v = cbv[i] * (e * d4[i]);
           asm volatile("" : "+v"(v));  // a select, not a branch around the exponential
           m[4 * q + i] = 8 * q + i <= diag ? v : 0.0f;

@@ -345,7 +345,10 @@ int bm_hip_ternary_gemm_i32_dev(const int8_t *xq,
 /* Common to the calls:                                                 */
 /* - Tensors of the descriptor's `type` are read and written at any     */
 /*   row stride (in elements, below 2^24) and any element alignment;    */
-/*   everything is computed in fp32 or more, y is rounded once.         */
+/*   everything is computed in fp32 or more, y is rounded once.  For a  */
+/*   bf16 y of prompts with d_state > 8 two operands of its sums carry  */
+/*   16 bits (2^-17 of each term) and the gate is good to 2^-20, from   */
+/*   |z| = 8 on to |z| 2^-23; its own rounding is up to 2^-8.           */
 /* - At most 2^20 sequences and 2^30 - 1 rows; 2^16 sequences with a    */
 /*   list of slots, whose search for repeated entries grows with their  */
 /*   square (it is small up to about a thousand).                       */

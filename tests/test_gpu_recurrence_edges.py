@@ -212,3 +212,32 @@ def test_the_largest_floats_do_not_reach_earlier_rows(hip, N, value):
         assert np.array_equal(clean.pool()[c.slots[b]], c.pool()[c.slots[b]])
     if N <= 8 or abs(value) < 3.3e38:
         close(y1[row, ch], rows[row].reshape(-1)[ch], tols[row].reshape(-1)[ch], "f32", "its row")
+
+
+def test_bf16_after_steps_that_forget_everything(hip):
+    """Twenty steps whose decays vanish (exponents of -5120 powers of two in
+    all), then twelve small ones: decays between the small ones are as good as
+    without the sum before them.  u = 2^-24.  Of each term the bf16 operands
+    have two pieces (2^-17 for both products), its sums and the exponential
+    4 N + 200 roundings at most; the result is rounded once, by half of its own
+    last place."""
+    H, P, N, T = 2, 32, 32, 96
+    c = SsmCase("bf16", H, P, 1, N, [T], seed=5, gate=False, skip=False, bias=False, soft=False)
+    c.A = gpu(np.array([-1.0, -2.5]), torch.float32)
+    r = np.random.default_rng(5)
+    dt = np.exp(r.uniform(-6, -2, (T, H)))
+    dt[np.arange(T) % 32 < 20] = 200.0
+    c.dt.copy_(torch.as_tensor(dt))
+    x, B, Cm = f64(c.x).reshape(T, H, P), f64(c.B), f64(c.Cm)
+    dt, A, S = f64(c.dt), f64(c.A), c.pool()[c.slots[0]]
+    M, want, mag = np.abs(S), np.empty((T, H, P)), np.empty((T, H, P))
+    for t in range(T):
+        a = np.exp(A * dt[t])[:, None, None]
+        add = dt[t][:, None, None] * x[t][:, :, None] * B[t]
+        S, M = a * S + add, a * M + np.abs(add)
+        want[t], mag[t] = (S * Cm[t]).sum(-1), (M * np.abs(Cm[t])).sum(-1)
+    note("bf16 after vanishing decays")
+    c.run(hip)
+    off = (2.0 ** -17 + (4 * N + 200) * 2.0 ** -24) * mag
+    half = np.exp2(np.floor(np.log2(np.abs(want) + off)) - 8)
+    assert (np.abs(f64(c.y).reshape(T, H, P) - want) <= off + half).all()
