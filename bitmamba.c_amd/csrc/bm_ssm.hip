@@ -176,7 +176,9 @@ static hipError_t launch_step_t(const SsmArgs& a, hipStream_t s) {
 //
 // Workspace: per unit `ends` (laid out as the kernels hold a state) and
 // `decays` (one per head).  A sequence's last unit has no end of its own: the
-// first pass leaves the sequence's own state in its place.
+// first pass leaves the sequence's own state in its place.  A decay past fp32
+// (A d > 0), which a state may still come through, being zero or small, is
+// kept as minus its exponent.
 // ---------------------------------------------------------------------------
 struct ScanPlan {
   int len;         // rows per unit
@@ -186,6 +188,14 @@ struct ScanPlan {
   float* ends;
   float* decays;
 };
+
+// s times such a decay; t: the third part of its exponent, in powers of two.
+// Three factors, none of them infinite, take every state but zero as far as the
+// whole one would.
+__device__ __forceinline__ float grown(float s, float t) {
+  const float f = __builtin_amdgcn_exp2f(t < 127.0f ? t : 127.0f);
+  return s * f * f * f;
+}
 
 struct ScanUnit {
   Unit u;
@@ -304,6 +314,22 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
         for (int n = 0; n < NS; ++n)
           v[i][n] = e[j * unit_floats + (int64_t)min(n, a.n - 1) * channels];
       }
+      float least = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) least = fminf(least, d[i]);
+      if (__ballot(least < 0.0f)) {
+        asm volatile("");
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (j0 + i >= w.u.k) break;
+#pragma unroll
+          for (int n = 0; n < NS; ++n)
+            S[n] = n < a.n ? (d[i] < 0.0f ? grown(S[n], d[i] * (kLog2e / -3.0f)) : S[n] * d[i]) +
+                                 v[i][n]
+                           : 0.0f;
+        }
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (j0 + i >= w.u.k) break;
@@ -392,7 +418,8 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
       if (n < a.n) e[(int64_t)n * channels] = S[n];
     if (c % a.hd == 0) {
       const Decay all = decay_of((float)total);
-      pl.decays[unit * a.heads + h] = all.hi + all.lo;
+      const float f = all.hi + all.lo;
+      pl.decays[unit * a.heads + h] = f == __builtin_inff() ? (float)-total : f;
     }
   } else if (w.slot >= 0 && w.u.k == w.last) {
     float* st = a.state + (int64_t)w.slot * a.ss + (int64_t)c * a.n;
@@ -459,6 +486,21 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
       load_f32<float, V>(v[i], e + j * unit_floats);
       d[i] = dec[(int64_t)j * heads];
     }
+    float least = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) least = fminf(least, d[i]);
+    if (__ballot(least < 0.0f)) {
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (j0 + i >= w.last) break;
+        store_f32<float, V>(e + (j0 + i) * unit_floats, S);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          S[k] = (d[i] < 0.0f ? grown(S[k], d[i] * (-1.0f / 3.0f)) : S[k] * d[i]) + v[i][k];
+      }
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (j0 + i >= w.last) break;
@@ -510,11 +552,18 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
 // is good to fp32 however large c is.  A row's exponent is held at -256
 // powers of two, where its decay is long zero, so that the sums stay exact.
 //
+// Growth (A d > 0): a decay over several rows can be infinite where the state or
+// x that it multiplies is zero or small, and multiplies what the products lose
+// of pieces below 2^-126.  A chunk ends before its positive exponents sum up to
+// kGrowth, for all the block's waves, since they share B and C.  Where that can
+// happen each chunk waits for what the other waves say, 1 to 2 % of its time.
+//
 // Causality holds for infinities and NaN too: a product takes 0 for M above
 // the diagonal, and 0 times such an x would reach earlier rows, so x enters
 // that product as 0 and the rows from it on become NaN.  An fp32 x whose first
 // piece is infinite (kInfinite and more) is treated the same.
 constexpr int kQ = 32, kWaves = 4;
+constexpr double kGrowth = 16.0;  // powers of two
 constexpr float kInfinite = 0x1.ffp127f;  // rounds to an infinite bf16
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -736,8 +785,7 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
   // and C have been through LDS
   uint32_t nx[16], ndt = 0;
   Raw4<T> nb[kItems][4];
-  auto fetch_bc = [&](int t, auto load4) {
-    const int rows = min(kQ, w.t1 - t);
+  auto fetch_bc = [&](int t, int rows, auto load4) {
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       const int first = wave * 64 + k * kThreads;  // kBlocks: whole waves
@@ -752,25 +800,24 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
       for (int q = 0; q < 4; ++q) nb[k][q] = load4(src, off + q * stride, n);
     }
   };
-  auto fetch_x = [&](int t) {
-    const auto bx = rows_of<T>(a.x, t, a.xs, min(kQ, w.t1 - t));
+  auto fetch_x = [&](int t, int rows) {
+    const auto bx = rows_of<T>(a.x, t, a.xs, rows);
     const uint32_t xo = here(xoff);
 #pragma unroll
     for (int r = 0; r < 16; ++r) nx[r] = load_raw<T>(bx, xo + acc_row(r, 0) * xs);
   };
-  auto fetch = [&](int t) {
-    const int rows = min(kQ, w.t1 - t);
+  auto fetch = [&](int t, int rows) {
     const auto bdt = rows_of<T>(a.dt, t, a.dts, rows);
     ndt = load_raw<T>(bdt, li * (uint32_t)(a.dts * sizeof(T)) + h * (uint32_t)sizeof(T));
     if (wide)
-      fetch_bc(t, [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
+      fetch_bc(t, rows, [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
         return load_raw4<T>(r, n < a.n ? off : kNoColumn);
       });
-    if (!FULL) fetch_x(t);
+    if (!FULL) fetch_x(t, rows);
   };
   // value by value, where four do not lie on one load's alignment: not ahead
-  auto fetch_narrow = [&](int t) {
-    fetch_bc(t, [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
+  auto fetch_narrow = [&](int t, int rows) {
+    fetch_bc(t, rows, [&](__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
       Raw4<T> o;
       uint32_t v[4];
 #pragma unroll
@@ -811,13 +858,14 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
   // them, in the wave's own part of LDS; out of dt fetched before.  Done ahead
   // of the chunk, in the shadow of the products before it.
   float eall = 1.0f;
+  double whole = 0.0;
   auto exponents = [&](int rows) {
     const float d = li < rows ? step_of(a, raw_f32<T>(ndt), bias) : 0.0f;
     double cum = (double)A * (double)d * 1.4426950408889634;
     cum = cum < -256.0 ? -256.0 : (cum > 256.0 ? 256.0 : cum);
+    const bool grows = __ballot(cum > 0.0) != 0;
     cum = half_scan(cum);
-    const double whole = lane_f64(cum, kQ - 1);
-    total += whole;
+    whole = lane_f64(cum, kQ - 1);
     eall = __builtin_amdgcn_exp2f((float)whole);
     if (half == 0) {
       const float hi = (float)cum;
@@ -827,16 +875,44 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
       shE[li] = __builtin_amdgcn_exp2f(hi);
       shW[li] = __builtin_amdgcn_exp2f((float)(whole - cum)) * d;
     }
+    return grows;
+  };
+  // in the columns of C B^T that pad its rows, for each wave: whether any
+  // exponent of its chunk is positive, the rows that can go together then, and
+  // whether any can be positive: A > 0, or steps of either sign
+  int *shGrows = (int*)shCb + kQ, *shRows = shGrows + 1, *shMay = shGrows + 2;
+  const int pad = (lane & (kWaves - 1)) * L::kRowCb;
+  auto ahead = [&](int rows) {
+    const bool grows = exponents(rows);
+    if (lane == 0) shGrows[wave * L::kRowCb] = grows;
   };
 
   if (w.t0 < w.t1) {
-    fetch(w.t0);
-    exponents(min(kQ, w.t1 - w.t0));
+    fetch(w.t0, min(kQ, w.t1 - w.t0));
+    ahead(min(kQ, w.t1 - w.t0));
   }
-  for (int t = w.t0; t < w.t1; t += kQ) {
-    const int rows = min(kQ, w.t1 - t);
+  if (lane == 0) shMay[wave * L::kRowCb] = !a.softplus || A > 0.0f;
+  __syncthreads();
+  const uint32_t may_grow = __ballot(shMay[pad]) != 0;
+  int rows = 0;
+  for (int t = w.t0; t < w.t1; t += rows) {
+    rows = min(kQ, w.t1 - t);
+    // the same in all waves; here(): one loop, not one for each of two values
+    if (__builtin_amdgcn_readfirstlane(here(may_grow)) && __ballot(shGrows[pad])) {
+      const float d = li < rows ? step_of(a, raw_f32<T>(ndt), bias) : 0.0f;
+      const double up = half_scan((double)fminf(fmaxf(A * d * kLog2e, 0.0f), 256.0f));
+      if (lane == 0) shRows[wave * L::kRowCb] = __popc((uint32_t)__ballot(up < kGrowth));
+      __syncthreads();
+      const int most = shRows[pad];
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) rows = min(rows, __builtin_amdgcn_readlane(most, k));
+      rows = max(rows, 1);
+      fetch(t, rows);
+      (void)exponents(rows);
+    }
+    total += whole;
     // B and C into LDS
-    if (!wide) fetch_narrow(t);
+    if (!wide) fetch_narrow(t, rows);
     constexpr int kHeld = L::kShared && FULL ? kItems : 1;
     Raw4<T> held[kHeld][4];  // B, where its transpose has to wait
 #pragma unroll
@@ -861,13 +937,14 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
       for (int r = 0; r < 16; ++r) x[r] = raw_f32<T>(nx[r]);
     uint32_t z[16];
     if (FULL) {
-      fetch_x(t);
+      fetch_x(t, rows);
       const auto bz = rows_of<T>(a.z, t, a.zs, a.z ? rows : 0);
       const uint32_t zo = here(zoff);
 #pragma unroll
       for (int r = 0; r < 16; ++r) z[r] = load_raw<T>(bz, zo + acc_row(r, 0) * zs);
     }
-    if (t + kQ < w.t1) fetch(t + kQ);
+    const int next = t + rows, after = min(kQ, w.t1 - next);
+    if (after > 0) fetch(next, after);
     __syncthreads();
 
     if constexpr (FULL) {
@@ -1029,7 +1106,7 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
           S[nt] = mfma32<kStatePieces>(pb, xw[s], S[nt]);
         }
       }
-      if (t + kQ < w.t1) exponents(min(kQ, w.t1 - t - kQ));
+      if (after > 0) ahead(after);
     }
     __syncthreads();  // the next chunk may overwrite LDS
   }
@@ -1038,8 +1115,9 @@ __global__ __launch_bounds__(64 * kWaves, NT < 8 ? 2 : 1) void k_scan_mm(SsmArgs
     if (!active) return;
     float* e = pl.ends + unit * unit_floats + tile_at;
     put_tile(e, S);
+    const float sum = (float)total;
     if (pt == 0 && lane == 0)
-      pl.decays[unit * a.heads + h] = __builtin_amdgcn_exp2f((float)total);
+      pl.decays[unit * a.heads + h] = sum >= 128.0f ? -sum : __builtin_amdgcn_exp2f(sum);
   } else if (w.slot >= 0 && w.u.k == w.last) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)

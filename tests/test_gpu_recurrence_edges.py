@@ -10,7 +10,7 @@ import torch
 
 import native
 from native import bh
-from recurrence import ConvCase, SsmCase, at, check_rows, close, f64, gpu
+from recurrence import TYPES, ConvCase, SsmCase, at, check_rows, close, f64, gpu, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -241,3 +241,92 @@ def test_bf16_after_steps_that_forget_everything(hip):
     off = (2.0 ** -17 + (4 * N + 200) * 2.0 ** -24) * mag
     half = np.exp2(np.floor(np.log2(np.abs(want) + off)) - 8)
     assert (np.abs(f64(c.y).reshape(T, H, P) - want) <= off + half).all()
+
+
+# ---------------------------------------------------------------------------
+# growth: A d > 0.  The bounds of tests/recurrence.py take the exponents in.
+# ---------------------------------------------------------------------------
+GROWTH = [("f32", 1), ("f32", 5), ("f32", 9), ("f32", 24), ("bf16", 24), ("f16", 40), ("f32", 128),
+          ("bf16", 128), ("f32", 200)]
+
+
+def growing(type_name, N, T, rate, start, heads=2):
+    """Head 0 grows by e^rate in each token, the last one decays."""
+    c = SsmCase(type_name, heads, 40, 1, N, [T, 5], gate=False, skip=False, bias=False, soft=False,
+                slots=None, spare=0, seed=N + T)
+    c.A[:] = rate
+    c.A[-1] = -0.5
+    c.dt.fill_(1.0)
+    c.pool_buf[0] = start
+    return c
+
+
+def check_growth(c, hip, what, rows_in_range=None, relative=0.0, lost=0.0):
+    """c.check, where a result that rounds past the type's largest value, half
+    a step above it, is infinite.  From row rows_in_range on the states of all
+    heads but the last pass fp32's range and are not looked at.  relative and
+    lost (of y): what the bounds of tests/recurrence.py do not have."""
+    last = slice(c.H - 1, c.H)
+    rows, tols, pool, stol = c.want()
+    c.run(hip)
+    got = f64(c.y).reshape(-1, c.H, c.P)
+    top = torch.finfo(TYPES[c.type][1]).max * (1 + half_step(c.type) / 2)
+    for t in rows:
+        heads = slice(None) if rows_in_range is None or t < rows_in_range else last
+        g, want = got[t][heads], rows[t][heads]
+        tol = tols[t][heads] + relative * np.abs(want) + lost
+        inf = np.isinf(g) & (np.abs(want) + tol >= top) & (g * want > 0)
+        assert inf[np.abs(want) - tol > top].all(), "%s row %d" % (what, t)
+        close(np.where(inf, 0.0, g), np.where(inf, 0.0, want), tol, c.type, "%s row %d" % (what, t))
+    for k in stol:
+        heads = slice(None) if rows_in_range is None or k == 0 else last
+        close(c.pool()[k][heads], pool[k][heads], (stol[k] + relative * np.abs(pool[k]))[heads],
+              "f32", "%s slot %d" % (what, k))
+
+
+@pytest.mark.parametrize("type_name,N", GROWTH)
+@pytest.mark.parametrize("T,rate", [(33, 3.0), (70, 3.0), (150, 1.0), (700, 0.5), (300, 30.0), (64, 80.0)])
+def test_nothing_grows_into_nothing(hip, type_name, N, T, rate):
+    """Growth past fp32 of a zero state under zero inputs: zero until the last
+    token, whose own part is finite, in one unit and over several."""
+    c = growing(type_name, N, T, rate, 0.0, heads=5)
+    c.x[:T - 1] = 0.0
+    note("zero state, %s N=%d, %d tokens of e^%g" % (type_name, N, T, rate))
+    check_growth(c, hip, "nothing grows", T)
+
+
+@pytest.mark.parametrize("type_name,N", GROWTH)
+@pytest.mark.parametrize("T,rate,exponent", [(40, 3.0, -123), (180, 0.8, -123), (41, 2.0, -110),
+                                             (36, 4.5, -145)])
+def test_a_small_state_grows_past_any_decay(hip, type_name, N, T, rate, exponent):
+    """A state of 2^exponent and no input: the decays over a unit, or over 32
+    tokens, are past fp32, the states are not.  Below 2^-126 the two roundings
+    of a token are 2^-150 each, whatever the state; those of token k grow with
+    it, to 2^(-149 - exponent) e^(-rate k) of it: the sum over k below.  From 9
+    values on each of a state's three bf16 pieces counts as zero below 2^-126,
+    times a chunk's growth of up to 2^16 and C."""
+    c = growing(type_name, N, T, rate, 2.0 ** exponent)
+    c.x.zero_()
+    if type_name != "f32":  # y itself would be rounded to nothing, or past fp16
+        c.Cm.zero_()
+    note("small state, %s N=%d, %d tokens of e^%g" % (type_name, N, T, rate))
+    lost = 3 * 2.0 ** (16 - 126) * np.abs(f64(c.Cm)).max() * N if N > 8 else 0.0
+    check_growth(c, hip, "small state", T, 2.0 ** (-149 - exponent) / (np.exp(rate) - 1), lost)
+    assert np.isfinite(c.pool()[0]).all() and c.pool()[0, 0].min() > 1.0
+
+
+@pytest.mark.parametrize("N", [1, 9, 128])
+def test_a_chunk_with_some_growing_tokens(hip, N):
+    """Steps of both signs: runs of growth that need a cut anywhere in a chunk,
+    in one head of several that share B and C."""
+    c = SsmCase("f32", 6, 40, 1, N, [300, 90, 33], gate=True, skip=True, bias=False, soft=False,
+                seed=N)
+    r = np.random.default_rng(N)
+    dt = np.abs(r.standard_normal((423, 6))) * 0.5
+    for at_ in (0, 7, 14, 21, 29, 37, 44, 60, 140, 147, 155, 290, 300, 307, 315, 380, 388, 395, 403):
+        dt[at_:at_ + 3, 2] = -r.uniform(16, 20, 3)  # to e^60 at most
+        dt[at_ + 3:at_ + 7, 2] = 30.0  # and forgotten
+    c.dt.copy_(torch.as_tensor(dt))
+    c.A[:] = -1.0
+    note("steps of both signs, N=%d" % N)
+    check_growth(c, hip, "both signs")
