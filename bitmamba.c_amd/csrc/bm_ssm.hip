@@ -523,15 +523,15 @@ __global__ __launch_bounds__(256) void k_scan_join(SeqView q, ScanPlan pl, int64
 // two blocks per CU beat one block of eight, whose waves all wait for the same
 // barriers (second pass at d_state 128, bf16: 319 against 335 us then).
 //
-// What bounds it: per 32 rows and channels at d_state 128, bf16, 966 vector
+// What bounds it: per 32 rows and channels at d_state 128, bf16, 1004 vector
 // instructions (splitting S, the decays, gates; 47 of them MFMAs).  With two
-// waves per SIMD (214 registers) the vector pipe is busy 55 % of the time, the
-// matrix pipe 19 %; leaving out all memory accesses takes 228 us to 177.  Tried without
+// waves per SIMD (220 registers) the vector pipe is busy 55 % of the time, the
+// matrix pipe 19 %; leaving out all memory accesses took 228 us to 177.  Tried without
 // gain: x and z a chunk ahead, a third wave per SIMD (spills), dot products in
 // place of subtractions in the split, uniform row offsets, one exponential per
 // row in place of one per pair.  64 heads of 64, d_state 128, one group, bf16,
-// 16384 rows: 105 + 18 + 227 us for the passes and the join, 417 MB (82 us);
-// 32 heads, d_state 64, fp32, 3001 rows: 22 + 10 + 38 us, 84 MB (16 us).
+// 16384 rows: 105 + 18 + 236 us for the passes and the join, 417 MB (82 us);
+// 32 heads, d_state 64, fp32, 3001 rows: 23 + 10 + 40 us, 84 MB (16 us).
 //
 // Precision.  MFMA operands are bf16.  An fp32 value is carried as the sum of
 // three bf16 pieces (8 bits each, the remainder of the piece before), fp16 as
