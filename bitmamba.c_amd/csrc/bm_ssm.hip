@@ -403,8 +403,8 @@ __global__ __launch_bounds__(64) void k_scan_small(SsmArgs a, ScanPlan pl, int h
     }
     // The tile's decays were the nearest floats.  What that left of them: for
     // the state from before the tile all of it, for what its rows added up to
-    // 16 halves of 2^-24 too much (a second product per row instead takes 57.5
-    // against 56.0 us at 4 values, fp16, 6000 rows of 32 heads of 64).
+    // 16 halves of 2^-24 too much (a second product per row instead took 57.5
+    // against 56.0 us at 4 values, fp16, 6000 rows of 32 heads of 64; 52.3 now).
 #pragma unroll
     for (int n = 0; n < NS; ++n) S[n] = with_low(S[n], low, S[n]);
     if (!FULL) total += (double)exponents;

@@ -436,7 +436,7 @@ typedef struct {
  * memory on 256 bytes with any contents (NULL where that is 0; it depends
  * on the sizes of op alone, not on the pointers).  A workspace of an op
  * serves every call whose n_seqs and n_tokens are both no larger, with the
- * same heads, groups and d_state. */
+ * same n_heads, head_dim and d_state. */
 size_t bm_hip_ssm_workspace_bytes(const bm_hip_ssm_t *op);
 int bm_hip_ssm_dev(const bm_hip_ssm_t *op, void *workspace, void *stream);
 /* One token of each sequence. */
