@@ -330,3 +330,20 @@ def test_a_chunk_with_some_growing_tokens(hip, N):
     c.A[:] = -1.0
     note("steps of both signs, N=%d" % N)
     check_growth(c, hip, "both signs")
+
+
+@pytest.mark.parametrize("type_name,N", [("f32", 1), ("f32", 24), ("bf16", 128), ("f32", 256)])
+@pytest.mark.parametrize("head", [0, 3, 6])
+def test_one_growing_head_under_softplus(hip, type_name, N, head):
+    """Steps that softplus makes positive, one head of seven with A > 0: it
+    alone grows, from nothing, past fp32 several times over."""
+    T = 290
+    c = SsmCase(type_name, 7, 40, 1, N, [T], bias=True, gate=True, skip=True, seed=N + head,
+                slots=None, spare=0)
+    c.A[head] = 3.0
+    c.dt[:, head] = 2.0
+    c.dt_bias[head] = 0.0
+    c.pool_buf[0].view(7, 40, N)[head] = 0.0
+    c.x[:T - 2].view(T - 2, -1)[:, 40 * head:40 * head + 40] = 0.0
+    note("head %d grows, %s N=%d" % (head, type_name, N))
+    check_growth(c, hip, "softplus")
