@@ -71,6 +71,28 @@ class Ssm(C.Structure):
                 ("y_stride", _i64)]
 
 
+class Delta(C.Structure):
+    """bm_hip_delta_t (include/bm_hip.h)."""
+    _fields_ = [("type", _i), ("n_heads", _i), ("head_dim", _i), ("n_groups", _i), ("d_state", _i),
+                ("dt_softplus", _i), ("beta_sigmoid", _i), ("qk_norm", _i), ("frozen", _i),
+                ("norm_eps", _f), ("scale", _f), ("n_seqs", _i), ("n_tokens", _i),
+                ("seq_start", _vp), ("slots", _vp), ("fresh", _vp), ("q", _vp), ("k", _vp),
+                ("v", _vp), ("dt", _vp), ("beta", _vp), ("z", _vp), ("q_stride", _i64),
+                ("k_stride", _i64), ("v_stride", _i64), ("dt_stride", _i64),
+                ("beta_stride", _i64), ("z_stride", _i64), ("A", _vp), ("dt_bias", _vp),
+                ("state", _vp), ("state_stride", _i64), ("n_slots", _i), ("y", _vp),
+                ("y_stride", _i64)]
+
+
+class Verify(C.Structure):
+    """bm_hip_verify_t (include/bm_hip.h)."""
+    _fields_ = [("type", _i), ("vocab", _i), ("n_seqs", _i), ("n_rows", _i), ("row_start", _vp),
+                ("target", _vp), ("target_stride", _i64), ("target_weights", _i), ("draft", _vp),
+                ("draft_stride", _i64), ("draft_weights", _i), ("temp", _f), ("tokens", _vp),
+                ("u", _vp), ("n_accepted", _vp), ("next_token", _vp), ("ratio", _vp),
+                ("split_start", _vp)]
+
+
 class Slots(C.Structure):
     """bm_hip_slots_t (include/bm_hip.h)."""
     _fields_ = [("base", _vp), ("n_slots", _i), ("n_layers", _i), ("slot_bytes", _i64),
@@ -126,6 +148,11 @@ SIGNATURES = {
     "bm_hip_ssm_workspace_bytes": (_sz, [C.POINTER(Ssm)]),
     "bm_hip_ssm_dev": (_i, [C.POINTER(Ssm), _vp, _vp]),
     "bm_hip_ssm_step_dev": (_i, [C.POINTER(Ssm), _vp]),
+    "bm_hip_delta_workspace_bytes": (_sz, [C.POINTER(Delta)]),
+    "bm_hip_delta_dev": (_i, [C.POINTER(Delta), _vp, _vp]),
+    "bm_hip_delta_step_dev": (_i, [C.POINTER(Delta), _vp]),
+    "bm_hip_verify_workspace_bytes": (_sz, [C.POINTER(Verify)]),
+    "bm_hip_verify_dev": (_i, [C.POINTER(Verify), _vp, _vp]),
     "bm_hip_slots_copy_dev": (_i, [C.POINTER(Slots), _i, _vp, _vp, _i, _vp]),
     "bm_hip_slots_compact_workspace_bytes": (_sz, [_i]),
     "bm_hip_slots_compact_dev": (_i, [C.POINTER(Slots), _i, _vp, _vp, _i, _vp, _vp, _vp]),

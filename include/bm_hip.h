@@ -442,6 +442,58 @@ int bm_hip_ssm_dev(const bm_hip_ssm_t *op, void *workspace, void *stream);
 /* One token of each sequence. */
 int bm_hip_ssm_step_dev(const bm_hip_ssm_t *op, void *stream);
 
+/* The gated delta rule (no counterpart in the reference), for blocks whose
+ * state is a table from keys to values: per head h of group g = h / (n_heads
+ * / n_groups), with d = dt[t][h] + dt_bias[h], taken through log(1 + exp(d))
+ * if dt_softplus, a = exp(min(A[h] * d, 0)), b = beta[t][h], taken through
+ * 1 / (1 + exp(-b)) if beta_sigmoid, and q, k the rows of the group, each
+ * divided by sqrt(sum of its squares + norm_eps) if qk_norm,
+ *   S[p][n] = a * S[p][n]
+ *   w[p] = b * (v[t][h][p] - sum_n S[p][n] * k[t][g][n])
+ *   S[p][n] = S[p][n] + w[p] * k[t][g][n]
+ *   y[t][h][p] = scale * sum_n S[p][n] * q[t][g][n]
+ *                * z[t][h][p] / (1 + exp(-z[t][h][p]))
+ * Rows, sequences, slots and streams as above; frozen != 0 reads the slots
+ * and leaves them as they are: drafted tokens are scored, and the accepted
+ * ones given again (bm_hip_verify_dev's split_start).
+ *
+ * A key with b * (sum of k's squares) above 2 makes the rule grow without
+ * end; qk_norm with b in 0..2 cannot.  Where such a growth passes fp32, the
+ * head's later rows of the sequence are infinite, NaN or undefined.  A head's
+ * q, k, dt or beta that is infinite or NaN, or whose squares' sum is, makes
+ * the head NaN from that row on (q: in that row), a v[p] or state row p that
+ * row of the state; earlier rows, other rows of the state, other heads and
+ * sequences are not reached.  fp32 values of 2^128 - 2^119 and more count as
+ * infinite.  */
+typedef struct {
+    int type;                      /* of q, k, v, dt, beta, z, y */
+    int n_heads, head_dim;         /* v, z, y rows: [n_heads][head_dim] */
+    int n_groups, d_state;         /* q, k rows: [n_groups][d_state]; n_groups divides n_heads, d_state <= 256 */
+    int dt_softplus, beta_sigmoid, qk_norm, frozen;
+    float norm_eps, scale;         /* norm_eps at least 0, read with qk_norm */
+    int n_seqs, n_tokens;
+    const int32_t *seq_start;      /* device [n_seqs + 1], or NULL */
+    const int32_t *slots;          /* device [n_seqs], or NULL */
+    const uint8_t *fresh;          /* device [n_seqs], or NULL */
+    const void *q, *k, *v, *dt, *beta, *z; /* dt: NULL without A; beta: NULL for 1; z: NULL for no gate */
+    int64_t q_stride, k_stride, v_stride, dt_stride, beta_stride, z_stride;
+    const float *A;                /* [n_heads], or NULL for a = 1 */
+    const float *dt_bias;          /* [n_heads], or NULL */
+    float *state;                  /* slot i at state + i * state_stride: [n_heads][head_dim][d_state] */
+    int64_t state_stride;
+    int n_slots;
+    void *y;
+    int64_t y_stride;
+} bm_hip_delta_t;
+
+/* Prompts.  The workspace as bm_hip_ssm_dev's: any contents, on 256 bytes,
+ * one of an op serves every call of no more sequences and rows with the same
+ * type, n_heads and d_state. */
+size_t bm_hip_delta_workspace_bytes(const bm_hip_delta_t *op);
+int bm_hip_delta_dev(const bm_hip_delta_t *op, void *workspace, void *stream);
+/* One token of each sequence; y may be written over v itself. */
+int bm_hip_delta_step_dev(const bm_hip_delta_t *op, void *stream);
+
 /* A pool of slots: slot i of layer l is slot_bytes bytes at base +
  * l * layer_stride + i * slot_stride (strides in bytes). */
 typedef struct {
@@ -471,6 +523,68 @@ size_t bm_hip_slots_compact_workspace_bytes(int n_slots);
 int bm_hip_slots_compact_dev(const bm_hip_slots_t *pools, int n_pools,
                              const int32_t *slots, int32_t *new_slots, int n,
                              int32_t *n_live, void *workspace, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* Verification of drafted tokens (no counterpart in the reference;     */
+/* asynchronous on `stream`, allocates nothing, may be captured).       */
+/* Sequence b has rows row_start[b] .. row_start[b + 1] - 1 (device,    */
+/* n_seqs + 1 ascending entries, clamped to 0..n_rows; NULL for one     */
+/* sequence of n_rows rows): one per drafted token and a last one.      */
+/* Row i's target distribution p_i is that of the token that tokens[i]  */
+/* drafts, the last row's that of the token behind all drafts.  Drafts  */
+/* are taken in order while u[i] * q_i(tokens[i]) < p_i(tokens[i]).     */
+/* The token after those taken is drawn from max(p_i - q_i, 0) of the   */
+/* first row refused (p_i where that is zero everywhere), or from the   */
+/* last row's p, with the last row's u: the first token at which the    */
+/* running sum exceeds u times the whole.  So with u uniform in 0..1    */
+/* (1 excluded) and drafts drawn from q, tokens are distributed as if   */
+/* drawn from p one by one.                                             */
+/*                                                                      */
+/* - A row is logits, p = softmax(row / temp), or with target_weights   */
+/*   (draft_weights) numbers p is proportional to, whose negative,      */
+/*   infinite and NaN ones count as 0.  With temp below 0.05 (as the    */
+/*   sampler's greedy branch) a row of logits is 1 at its largest, the  */
+/*   first of equal ones.  -inf and NaN logits have p = 0, +inf ones    */
+/*   share everything equally.                                          */
+/* - draft NULL: the drafts were not drawn, q is 1 at tokens[i].        */
+/* - A draft outside the vocabulary is refused (p = 0 and q = 0).       */
+/*   A target row without any p > 0 refuses, and has next_token -1 if   */
+/*   it is the one drawn from.                                          */
+/* - Sums and exponentials are in 64 bits; nothing depends on an order. */
+/* - A sequence without rows gets n_accepted 0 and next_token -1.       */
+/* - 0, -2 for arguments that do not fit (nothing is launched), -1 for  */
+/*   a HIP error; the reason is in bm_hip_last_error().                 */
+/* ------------------------------------------------------------------ */
+typedef struct {
+    int type;                   /* of target and draft */
+    int vocab;                  /* 1..256000 */
+    int n_seqs, n_rows;         /* up to 2^20, below 2^30 */
+    const int32_t *row_start;   /* device [n_seqs + 1], or NULL */
+    const void *target;         /* rows of vocab values */
+    int64_t target_stride;      /* in elements, below 2^24 */
+    int target_weights;
+    const void *draft;          /* rows of vocab values (a sequence's last is not read), or NULL */
+    int64_t draft_stride;
+    int draft_weights;
+    float temp;                 /* finite, read for rows of logits */
+    const int32_t *tokens;      /* device [n_rows] (a sequence's last is not read) */
+    const float *u;             /* device [n_rows] */
+    int32_t *n_accepted;        /* device [n_seqs]: drafts taken */
+    int32_t *next_token;        /* device [n_seqs] */
+    float *ratio;               /* device [n_rows], or NULL: min(1, p / q) of each draft; last rows keep what they hold */
+    int32_t *split_start;       /* device [2 * n_seqs + 1], or NULL: see below */
+} bm_hip_verify_t;
+
+/* split_start holds the rows of 2 n_seqs sequences: 2b is sequence b's rows
+ * whose tokens stand (its first and one per draft taken), 2b + 1 its others.
+ * Given as seq_start, with slots -1 for the odd ones, to bm_hip_conv_dev,
+ * bm_hip_ssm_dev or bm_hip_delta_dev it advances each state by the tokens
+ * that stand and no more, without a round trip to the host.
+ * workspace: bm_hip_verify_workspace_bytes(op) bytes of device memory on 256
+ * bytes with any contents; one of an op serves every call of no more
+ * sequences, rows and vocabulary. */
+size_t bm_hip_verify_workspace_bytes(const bm_hip_verify_t *op);
+int bm_hip_verify_dev(const bm_hip_verify_t *op, void *workspace, void *stream);
 
 /* ------------------------------------------------------------------ */
 /* Device-resident model: the reference's model API (src/bitmamba.h:    */
