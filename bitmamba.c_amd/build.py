@@ -27,6 +27,13 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
+# of single files
+FILE_FLAGS = {
+    # results of matrix instructions in vector registers: with more than 256 in
+    # use the compiler puts them into accumulation registers otherwise, and
+    # copies them for every other instruction
+    "bm_delta.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+}
 C_FLAGS = ["-std=gnu11", "-O2", "-fPIC", "-fopenmp", "-ffp-contract=off",
            "-Wall", "-Wextra"]
 INCLUDES = ["-I" + os.path.join(ROOT, "include"),
@@ -54,7 +61,8 @@ def build(verbose=False):
         if f.endswith(".hip"):
             src = os.path.join(HERE, "csrc", f)
             obj = os.path.join(obj_dir, f[:-4] + ".o")
-            jobs.append([hipcc] + HIP_FLAGS + INCLUDES + ["-c", src, "-o", obj])
+            jobs.append([hipcc] + HIP_FLAGS + FILE_FLAGS.get(f, []) + INCLUDES +
+                        ["-c", src, "-o", obj])
     for f in sorted(os.listdir(os.path.join(HERE, "host"))):
         if f.endswith(".c"):
             src = os.path.join(HERE, "host", f)

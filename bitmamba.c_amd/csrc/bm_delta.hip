@@ -8,7 +8,6 @@
 #include <math.h>
 
 #include "bm_dev.h"
-#include "bm_mma.h"
 #include "bm_seq.h"
 
 namespace bm {
@@ -39,10 +38,10 @@ __device__ __forceinline__ float beta_of(const DeltaArgs& a, float b) {
   if (!a.beta) return 1.0f;
   return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_f32(-b)) : b;
 }
-// 1 / sqrt(squares + eps); NaN where the squares' sum is not finite
+// what a row of q or k is multiplied by; NaN where its squares' sum is not finite
 __device__ __forceinline__ float unit_of(const DeltaArgs& a, float squares) {
-  if (!a.norm) return 1.0f;
-  return squares < __builtin_inff() ? __builtin_amdgcn_rsqf(squares + a.eps) : __builtin_nanf("");
+  const float unit = a.norm ? __builtin_amdgcn_rsqf(squares + a.eps) : 1.0f;
+  return squares < __builtin_inff() ? unit : __builtin_nanf("");
 }
 
 // sum over teams of T neighbouring lanes, in every lane of the team
@@ -99,7 +98,7 @@ __device__ __forceinline__ float value_of(const RawRow<T, V>& r, int i) {
 //   S' q = a (S q) + w (k . q).
 // ---------------------------------------------------------------------------
 template <typename T, int TEAM, int V, int E, int U, bool STREAM, bool STEP>
-__global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a) {
+__global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a, int most) {
   constexpr int kRows = 64 / TEAM;
   const int b = blockIdx.x, h = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -110,6 +109,7 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a) {
   if (!STEP) {
     t0 = a.q.seq_start ? seq_row(a.q, b) : 0;
     t1 = a.q.seq_start ? seq_row(a.q, b + 1) : a.q.n_tokens;
+    if (t1 - t0 > most) return;
   }
   const int slot = find_slot(a.q, b, slots);
   if (slot == kNoSlot) return;
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a) {
 }
 
 template <typename T, int TEAM, int V, int E, bool STEP>
-static hipError_t launch_rows(const DeltaArgs& a, hipStream_t s) {
+static hipError_t launch_rows(const DeltaArgs& a, int most, hipStream_t s) {
   constexpr int U = E >= 4 ? 2 : (E == 2 ? 4 : (TEAM >= 16 ? (STEP ? 8 : 4) : 2));
   constexpr int kRows = 64 / TEAM * U;  // rows of the state per wave
   const int waves = (a.hd + kRows - 1) / kRows;
@@ -231,23 +231,1037 @@ static hipError_t launch_rows(const DeltaArgs& a, hipStream_t s) {
   // as the scan's single tokens: states of 64 MiB or more go past the caches
   constexpr bool kLarge = STEP && V == 4 && TEAM >= 4;
   if (kLarge && (int64_t)a.q.n_seqs * a.heads * a.hd * a.n >= (1 << 24))
-    return launch(k_delta_rows<T, TEAM, V, E, U, kLarge, STEP>, grid, dim3(64 * nw), 0, s, a);
-  return launch(k_delta_rows<T, TEAM, V, E, U, false, STEP>, grid, dim3(64 * nw), 0, s, a);
+    return launch(k_delta_rows<T, TEAM, V, E, U, kLarge, STEP>, grid, dim3(64 * nw), 0, s, a, most);
+  return launch(k_delta_rows<T, TEAM, V, E, U, false, STEP>, grid, dim3(64 * nw), 0, s, a, most);
 }
 
 template <typename T, bool STEP>
-static hipError_t launch_rows_t(const DeltaArgs& a, hipStream_t s) {
+static hipError_t launch_rows_t(const DeltaArgs& a, int most, hipStream_t s) {
   if (a.n % 4 == 0) {  // a state row's loads of four floats need no more than a float's alignment
-    if (a.n <= 16) return launch_rows<T, 4, 4, 1, STEP>(a, s);
-    if (a.n <= 32) return launch_rows<T, 8, 4, 1, STEP>(a, s);
-    if (a.n <= 64) return launch_rows<T, 16, 4, 1, STEP>(a, s);
-    if (a.n <= 128) return launch_rows<T, 16, 4, 2, STEP>(a, s);
-    return launch_rows<T, 16, 4, 4, STEP>(a, s);
+    if (a.n <= 16) return launch_rows<T, 4, 4, 1, STEP>(a, most, s);
+    if (a.n <= 32) return launch_rows<T, 8, 4, 1, STEP>(a, most, s);
+    if (a.n <= 64) return launch_rows<T, 16, 4, 1, STEP>(a, most, s);
+    if (a.n <= 128) return launch_rows<T, 16, 4, 2, STEP>(a, most, s);
+    return launch_rows<T, 16, 4, 4, STEP>(a, most, s);
   }
-  if (a.n <= 4) return launch_rows<T, 4, 1, 1, STEP>(a, s);
-  if (a.n <= 16) return launch_rows<T, 16, 1, 1, STEP>(a, s);
-  if (a.n <= 64) return launch_rows<T, 16, 1, 4, STEP>(a, s);
-  return launch_rows<T, 64, 1, 4, STEP>(a, s);
+  if (a.n <= 4) return launch_rows<T, 4, 1, 1, STEP>(a, most, s);
+  if (a.n <= 16) return launch_rows<T, 16, 1, 1, STEP>(a, most, s);
+  if (a.n <= 64) return launch_rows<T, 16, 1, 4, STEP>(a, most, s);
+  return launch_rows<T, 64, 1, 4, STEP>(a, most, s);
+}
+
+// ---------------------------------------------------------------------------
+// Prompts: chunks of kC rows on the matrix cores.  With c_i the sum of the
+// exponents of a chunk's rows up to i and S the state before it, what the rows
+// write, w, solves
+//   w_i + sum_{j<i} L_ij w_j = b_i (v_i - e^{c_i} S k_i),
+//   L_ij = b_i e^{c_i - c_j} (k_i . k_j),
+// so with T = (I + L)^-1 (unit lower triangular) and A_ij = e^{c_i - c_j}
+// (q_i . k_j) for j <= i, as products of kC rows
+//   w = T (b (v - e^c K S)),  y = e^c Q S + A w,  S' = e^{c_C} S + (e^{c_C - c} K)^T w.
+// T and A need no state: the first launch makes them for all chunks and heads
+// at once, the second walks each sequence's chunks.
+//
+// Precision.  MFMA operands are fp16.  A value is one half, or the sum of two
+// (22 bits) where it is computed or fp32; what leaves fp16's range of exponents
+// is scaled by powers of two: the rows of K, Q, T and A once, the columns of
+// the state and of w (one value of v each) as they grow and shrink.  The state
+// itself stays in fp32 accumulators.  bf16 in three pieces is as exact and
+// needs no scaling, but twice the products and 2.7 times the conversions.
+//
+// An infinity or NaN must not reach earlier rows of its chunk through a zero
+// of T or A: a head's first row of that kind (k, a or b) ends what its chunk
+// computes, and a column's (v, or what is computed from it) enters the
+// products as zero; the rows from it on and the state become NaN.
+// ---------------------------------------------------------------------------
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr int kC = 64;       // rows of a chunk
+constexpr int kShort = 32;   // sequences of up to these rows go row by row
+template <typename T>
+constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;  // of a value of K or Q
+constexpr int kTri = 6 * 2 * 1024;  // bytes of T or A: blocks of 16 rows and 32 columns on and below the diagonal
+// per place and head after T and A, 64 floats each: b; e^c of k; e^{c_C - c} of k; e^c of q; the
+// scales of A and T; then the decay (two parts), the first bad row, the largest of the third
+enum { kBeta, kGrowK, kLeft, kGrowQ, kFacA, kFacT, kMisc };
+constexpr int kScalars = 7 * 256;
+
+struct DeltaPlan {
+  bool chunks;     // a sequence may have more than kShort rows
+  bool by_rows;    // where a sequence's chunks lie: from row / 32, or from row / kC + b
+  bool wide;       // eight values of a row of Q or K on one load's alignment
+  int64_t units;   // chunks in the worst case
+  int64_t places;
+  uint8_t *heads, *keys;  // per place and head: T, A, scalars; per place and group: K, Q, K by columns
+  int64_t head_bytes, key_bytes;
+  size_t bytes;
+};
+
+// Operands.  A lane of a 16x16x32 product holds eight values of row (or column)
+// lane % 16, at 8 (lane / 16) and on, and of a result rows 4 (lane / 16) .. + 3
+// of column lane % 16.  Row r of tile t stands for row (of the chunk, or
+// column of K) spread_row(t, r): the results of tiles 2s and 2s + 1 are then
+// eight neighbours, 32 s + 8 (lane / 16) and on, and serve as operands as they are.
+__host__ __device__ constexpr int spread_row(int t, int r) {
+  return 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3);
+}
+// where the block of T or A of row tile w and columns 32 s .. lies
+__device__ __forceinline__ int tri_block(int w, int s) { return (w < 2 ? w : 2 * w - 2 + s) * 2048; }
+
+// c += (sum of a) (sum of b) without the product of two second halves
+template <int NA, int NB>
+__device__ __forceinline__ v4f mfma_h(const v8h (&a)[NA], const v8h (&b)[NB], v4f c) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (i + j < 2) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// two values as halves of a word: the nearest ones, and the nearest to what is left
+template <int N>
+__device__ __forceinline__ void halves2(uint32_t (&p)[N], float x, float y) {
+  v2f v = {x, y};
+  p[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
+  if constexpr (N == 2) {
+    // x - half in one instruction; p[0] waits for x and y, so these do too
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(x) : "v"(p[0]), "v"(x));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=v"(y)
+        : "v"(p[0]), "v"(y));
+    v = v2f{x, y};
+    p[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
+  }
+}
+template <int N>
+__device__ __forceinline__ void halves8(v8h (&p)[N], const float (&v)[8]) {
+  u32x4 w[N];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    uint32_t o[N];
+    halves2<N>(o, v[2 * e], v[2 * e + 1]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i][e] = o[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = __builtin_bit_cast(v8h, w[i]);
+}
+template <int N>
+__device__ __forceinline__ void halves8(v8h (&p)[N], v4f a, v4f b) {
+  const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  halves8<N>(p, v);
+}
+
+// the larger magnitude, NaN if either is
+__device__ __forceinline__ float max_abs(float m, float a) {
+  return __builtin_elementwise_maximum(m, __builtin_fabsf(a));
+}
+// over the four lanes with one lane % 16, in each of them
+template <typename F>
+__device__ __forceinline__ float over_quads(float v, F f) {
+  uint32_t b = __float_as_uint(v);
+  const auto x = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  b = __float_as_uint(f(__uint_as_float(x[0]), __uint_as_float(x[1])));
+  const auto y = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  return f(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float quads_max(float v) {
+  return over_quads(v, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+}
+__device__ __forceinline__ float quads_add(float v) {
+  return over_quads(v, [](float a, float b) { return a + b; });
+}
+
+// the power of two that takes a row's largest magnitude into 1 .. 2, and its inverse
+struct Scale {
+  float up, down;
+};
+__device__ __forceinline__ Scale scale_of(float largest) {
+  const int e = min(max((int)(__float_as_uint(largest) >> 23 & 255), 1), 253);
+  return Scale{__uint_as_float((uint32_t)(254 - e) << 23), __uint_as_float((uint32_t)e << 23)};
+}
+
+// a value that all lanes share, in a scalar register: what a buffer's address or
+// size is made of (quotients and clamps are worked out in vector registers, and
+// a resource in those costs a loop around each access)
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// keeps what is cheaply worked out anew from being held in registers over a loop
+__device__ __forceinline__ uint32_t anew(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// the block's LDS accesses are done; global ones stay in flight
+__device__ __forceinline__ void lds_sync() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ double scan_f64(double v) {  // running sums over the wave
+  auto add = [&](auto dpp) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)dpp((int)(uint32_t)b), hi = (uint32_t)dpp((int)(uint32_t)(b >> 32));
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);  // +0 without a source
+  };
+  add([](int x) { return dpp_or0<0x111>(x); });
+  add([](int x) { return dpp_or0<0x112>(x); });
+  add([](int x) { return dpp_or0<0x114>(x); });
+  add([](int x) { return dpp_or0<0x118>(x); });
+  add([](int x) { return dpp_or0<0x142, 0xa>(x); });
+  add([](int x) { return dpp_or0<0x143, 0xc>(x); });
+  return v;
+}
+
+constexpr int kRowL = kC + 4;  // floats of a row of L or T in LDS
+
+// T = (I + L)^-1, both [kC][kRowL] in LDS, in fp32.  Blocks of 16 by
+// substitution, a wave each; then blocks of 32 and the whole by
+// [[B, 0], [M, D]]^-1 = [[B', 0], [-D' M B', D']], which keeps to the sizes that
+// T itself has (sums of powers of L would not).
+__device__ __forceinline__ void invert(const float* L, float* T, int wave, int lane) {
+  const int c = lane & 15, q = lane >> 4;
+  {
+    const float* l = L + 16 * wave * kRowL + 16 * wave;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == c ? -1.0f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < i; j += 4) {
+        const float4 v = *(const float4*)(l + i * kRowL + j);
+        s = __builtin_fmaf(v.x, x[j], s);
+        if (j + 1 < i) s = __builtin_fmaf(v.y, x[j + 1], s);
+        if (j + 2 < i) s = __builtin_fmaf(v.z, x[j + 2], s);
+        if (j + 3 < i) s = __builtin_fmaf(v.w, x[j + 3], s);
+      }
+      x[i] = -s;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((i & 3) == q) T[(16 * wave + i) * kRowL + 16 * wave + c] = x[i];
+  }
+  lds_sync();
+  // d += block (bi, bk) of M times p, whose lane holds rows 4 q + i of 16
+  auto times = [&](const float* M, int bi, int bk, const float (&p)[4], v4f d) {
+    const float4 m = *(const float4*)(M + (16 * bi + c) * kRowL + 16 * bk + 4 * q);
+    const float mv[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x4f32(mv[i], p[i], d, 0, 0, 0);
+    return d;
+  };
+  auto block_of = [&](int bi, int bj, float (&p)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = T[(16 * bi + 4 * q + i) * kRowL + 16 * bj + c];
+  };
+  auto put = [&](int bi, int bj, v4f d) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) T[(16 * bi + 4 * q + i) * kRowL + 16 * bj + c] = -d[i];
+  };
+  const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (wave < 2) {
+    const int bi = 2 * wave + 1, bj = 2 * wave;
+    float p[4];
+    block_of(bj, bj, p);
+    const v4f m = times(L, bi, bj, p, zero);
+    const float mv[4] = {m[0], m[1], m[2], m[3]};
+    put(bi, bj, times(T, bi, bi, mv, zero));
+  }
+  lds_sync();
+  {
+    const int ra = wave >> 1, cb = wave & 1;
+    v4f d = zero;
+    for (int k = 0; k <= ra; ++k) {  // row k of L's block times column cb of T's first
+      v4f m = zero;
+      for (int e = cb; e < 2; ++e) {
+        float p[4];
+        block_of(e, cb, p);
+        m = times(L, 2 + k, e, p, m);
+      }
+      const float mv[4] = {m[0], m[1], m[2], m[3]};
+      d = times(T, 2 + ra, 2 + k, mv, d);
+    }
+    put(2 + ra, cb, d);
+  }
+  lds_sync();
+}
+
+// eight values of a row as the loads leave them
+template <typename T, bool WIDE>
+struct Eight {
+  uint32_t w[WIDE ? 2 * sizeof(T) : 8];
+};
+template <typename T, bool WIDE>
+__device__ __forceinline__ Eight<T, WIDE> load_eight(__amdgpu_buffer_rsrc_t r, uint32_t off, int n,
+                                                     int d_state) {
+  Eight<T, WIDE> o;
+  if constexpr (WIDE) {
+    const uint32_t at = n < d_state ? off : kNoColumn;
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, at + 16 * k, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o.w[4 * k + i] = v[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      o.w[i] = load_raw<T>(r, n + i < d_state ? off + i * (uint32_t)sizeof(T) : kNoColumn);
+  }
+  return o;
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ float eight_f32(const Eight<T, WIDE>& e, int i) {
+  if constexpr (!WIDE) return raw_f32<T>(e.w[i]);
+  else if constexpr (sizeof(T) == 4) return __uint_as_float(e.w[i]);
+  else return (float)__builtin_bit_cast(T, (uint16_t)(e.w[i >> 1] >> (16 * (i & 1))));
+}
+
+// ---------------------------------------------------------------------------
+// One chunk of one head: T, A and the rows' scalars; for a group's first head
+// also K and Q as operands.  Wave w has the rows of tile w (spread_row).
+// ---------------------------------------------------------------------------
+template <typename T, int NK, bool WIDE>
+__global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) {
+  constexpr int KP = kHalves<T>, kTile = NK * KP * 1024;  // bytes of 16 rows
+  constexpr int kShared = 4 * kTile > kC * kRowL * 4 ? 4 * kTile : kC * kRowL * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t shK[kShared];  // K; then T
+  __shared__ __attribute__((aligned(16))) float shL[kC * kRowL];
+  __shared__ __attribute__((aligned(16))) float shHi[kC], shLo[kC], shRk[kC];
+  __shared__ float shKk[kC], shKd[kC], shQf[kC];
+  float* shT = (float*)shK;
+  Unit u = find_unit(a.q, (int)wide_block(), kC);
+  u = Unit{uniform(u.b), uniform(u.k), uniform(u.s), uniform(u.e)};
+  if (u.b < 0 || u.e - u.s <= kShort) return;
+  const int t0 = u.s + u.k * kC;
+  if (t0 >= u.e) return;
+  const int rows = min(kC, u.e - t0);
+  const int64_t place = (pl.by_rows ? u.s / 32 : (int64_t)(u.s / kC) + u.b) + u.k;
+  const int h = blockIdx.y, per = a.heads / a.groups, g = uniform(h / per);
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+  const int wave = uniform(tid >> 6);
+  uint8_t* out = pl.heads + (place * a.heads + h) * pl.head_bytes;
+  uint8_t* keys = pl.keys + (place * a.groups + g) * pl.key_bytes;
+  const bool first_head = h == g * per;
+  const int tiles = wave < 2 ? 2 : 4;  // of rows up to the wave's
+  const int mine = spread_row(wave, r);
+
+  // the wave's rows of K and Q, all loads before the first use
+  Eight<T, WIDE> rk8[NK], rq8[NK];
+  {
+    const int half = 32 * (wave >> 1), have = uniform(max(0, min(32, rows - half)));
+    const int64_t gcol = (int64_t)g * a.n;
+    const auto bK = rows_of<T>((const T*)a.K + gcol, t0 + half, a.Ks, have);
+    const auto bQ = rows_of<T>((const T*)a.Q + gcol, t0 + half, a.Qs, have);
+    const uint32_t kr = (uint32_t)(mine - half) * (uint32_t)(a.Ks * sizeof(T)),
+                   qr = (uint32_t)(mine - half) * (uint32_t)(a.Qs * sizeof(T));
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      const int n = 32 * s + 8 * q;
+      rk8[s] = load_eight<T, WIDE>(bK, kr + (uint32_t)(n * sizeof(T)), n, a.n);
+    }
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      const int n = 32 * s + 8 * q;
+      rq8[s] = load_eight<T, WIDE>(bQ, qr + (uint32_t)(n * sizeof(T)), n, a.n);
+    }
+  }
+  // row = lane, the same in every wave
+  const int64_t row = t0 + min(lane, rows - 1);
+  const float dt = a.A ? (float)((const T*)a.dt)[row * a.dts + h] : 0.0f;
+  const float bt = a.beta ? (float)((const T*)a.beta)[row * a.bs + h] : 0.0f;
+  const float expo = exponent_of(a, a.A ? a.A[h] : 0.0f, dt, a.dt_bias ? a.dt_bias[h] : 0.0f);
+  const float beta = beta_of(a, bt);
+
+  // K and Q as operands, rows scaled
+  v8h qf[NK][KP];
+  {
+    float m = 0.0f, kk = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NK; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = eight_f32<T, WIDE>(rk8[s], i);
+        m = max_abs(m, v);
+        kk = __builtin_fmaf(v, v, kk);
+      }
+    const Scale sc = scale_of(quads_max(m));
+    kk = quads_add(kk);
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = eight_f32<T, WIDE>(rk8[s], i) * sc.up;
+      v8h p[KP];
+      halves8<KP>(p, v);
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        *(v8h*)(shK + wave * kTile + (s * KP + i) * 1024 + lane * 16) = p[i];
+        if (first_head) *(v8h*)(keys + wave * kTile + (s * KP + i) * 1024 + lane * 16) = p[i];
+      }
+    }
+    float mq = 0.0f, qq = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NK; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = eight_f32<T, WIDE>(rq8[s], i);
+        mq = max_abs(mq, v);
+        qq = __builtin_fmaf(v, v, qq);
+      }
+    const Scale sq = scale_of(quads_max(mq));
+    qq = quads_add(qq);
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = eight_f32<T, WIDE>(rq8[s], i) * sq.up;
+      halves8<KP>(qf[s], v);
+      if (first_head)
+#pragma unroll
+        for (int i = 0; i < KP; ++i)
+          *(v8h*)(keys + (4 + wave) * kTile + (s * KP + i) * 1024 + lane * 16) = qf[s][i];
+    }
+    if (q == 0) {
+      shKk[mine] = kk;
+      shKd[mine] = sc.down;
+      shQf[mine] = a.scale * unit_of(a, qq) * sq.down;
+    }
+  }
+  lds_sync();
+
+  // the rows' scalars, in every wave alike
+  const float squares = shKk[lane], rq = lane < rows ? shQf[lane] : 0.0f;
+  const bool in = lane < rows;
+  const bool bad = in && !(expo <= 0.0f && __builtin_fabsf(beta) < __builtin_inff() &&
+                           squares < __builtin_inff());
+  const uint64_t bads = __ballot(bad);
+  const int first = bads ? __ffsll((unsigned long long)bads) - 1 : kC;
+  const bool live = in && lane < first;
+  double cum = live ? (double)expo * 1.4426950408889634 : 0.0;
+  cum = scan_f64(cum < -256.0 ? -256.0 : cum);
+  const double whole = __shfl(cum, 63);
+  const float rk = live ? unit_of(a, squares) * shKd[lane] : 0.0f;
+  const float b = live ? beta : 0.0f;
+  const float hi = (float)cum, grow = __builtin_amdgcn_exp2f(hi);
+  shHi[lane] = hi;
+  shLo[lane] = (float)(cum - (double)hi);
+  shRk[lane] = rk;
+  float* scalars = (float*)(out + 2 * kTri);
+  if (wave == 0) {
+    const float left = __builtin_amdgcn_exp2f((float)(whole - cum)) * rk;
+    scalars[kBeta * 64 + lane] = b;
+    scalars[kGrowK * 64 + lane] = grow * rk;
+    scalars[kLeft * 64 + lane] = left;
+    scalars[kGrowQ * 64 + lane] = grow * rq;
+    const float most = wave_max_f32(left);
+    if (lane == 0) {
+      const Decay d = decay_of((float)(whole * 0.6931471805599453));
+      scalars[kMisc * 64] = d.hi;
+      scalars[kMisc * 64 + 1] = d.lo;
+      ((int*)scalars)[kMisc * 64 + 2] = first;
+      scalars[kMisc * 64 + 3] = most;
+    }
+  }
+  const float bi = __shfl(b * rk, mine), qi = __shfl(rq, mine);
+
+  // (k_j . k_i) and (k_j . q_i): i a row of the wave's, by lane; j up to it
+  v4f kk[4], kq[4];
+  const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    kk[t] = kq[t] = zero;
+    if (t < tiles) {
+#pragma unroll
+      for (int s = 0; s < NK; ++s) {
+        v8h pj[KP], pi[KP];
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+          pj[i] = *(const v8h*)(shK + t * kTile + (s * KP + i) * 1024 + lane * 16);
+          pi[i] = *(const v8h*)(shK + wave * kTile + (s * KP + i) * 1024 + lane * 16);
+        }
+        kk[t] = mfma_h(pj, pi, kk[t]);
+        kq[t] = mfma_h(pj, qf[s], kq[t]);
+      }
+    }
+  }
+  if (first_head) {
+    // K by columns: 16 columns of a tile and 32 rows each, as products with ones
+#pragma unroll
+    for (int x = 0; x < NK; ++x) {
+      const int t = 2 * x + (wave & 1), sp = wave >> 1;  // columns of step x
+      v8h one;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        one[e] = spread_row(t, r) == 32 * x + 8 * q + e ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+      for (int i = 0; i < KP; ++i) {
+        const uint8_t* at = shK + 2 * sp * kTile + (x * KP + i) * 1024 + lane * 16;
+        const v4f c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const v8h*)at, one, zero, 0, 0, 0);
+        const v4f c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const v8h*)(at + kTile), one, zero, 0, 0, 0);
+        v8h o[1];
+        halves8<1>(o, c0, c1);
+        *(v8h*)(keys + 8 * kTile + ((t * 2 + sp) * KP + i) * 1024 + lane * 16) = o[0];
+      }
+    }
+  }
+  // L into LDS, A out
+  const float ihi = shHi[mine], ilo = shLo[mine];
+  float m8[2][8], ma = 0.0f;
+#pragma unroll
+  for (int sp = 0; sp < 2; ++sp) {
+    if (2 * sp < tiles) {
+      float l[8];
+      const int j0 = 32 * sp + 8 * q;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float4 jh = *(const float4*)(shHi + j0 + 4 * k), jl = *(const float4*)(shLo + j0 + 4 * k),
+                     jr = *(const float4*)(shRk + j0 + 4 * k);
+        const float h4[4] = {jh.x, jh.y, jh.z, jh.w}, l4[4] = {jl.x, jl.y, jl.z, jl.w},
+                    r4[4] = {jr.x, jr.y, jr.z, jr.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + 4 * k + e;
+          const float d = __builtin_amdgcn_exp2f((ihi - h4[e]) + (ilo - l4[e])) * r4[e];
+          const float lv = bi * (d * kk[2 * sp + k][e]), mv = qi * (d * kq[2 * sp + k][e]);
+          l[4 * k + e] = j < mine && mine < first ? lv : 0.0f;
+          m8[sp][4 * k + e] = j <= mine && j < first ? mv : 0.0f;
+          ma = max_abs(ma, m8[sp][4 * k + e]);
+        }
+      }
+      *(float4*)(shL + mine * kRowL + j0) = make_float4(l[0], l[1], l[2], l[3]);
+      *(float4*)(shL + mine * kRowL + j0 + 4) = make_float4(l[4], l[5], l[6], l[7]);
+    }
+  }
+  auto put_tri = [&](uint8_t* at, float (&v)[2][8], float largest, int k) {
+    const Scale sc = scale_of(quads_max(largest));
+#pragma unroll
+    for (int sp = 0; sp < 2; ++sp) {
+      if (2 * sp < tiles) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[sp][e] *= sc.up;
+        v8h p[2];
+        halves8<2>(p, v[sp]);
+        uint8_t* o = at + tri_block(wave, sp) + lane * 16;
+        *(v8h*)o = p[0];
+        *(v8h*)(o + 1024) = p[1];
+      }
+    }
+    if (q == 0) scalars[k * 64 + mine] = sc.down;
+  };
+  put_tri(out + kTri, m8, ma, kFacA);
+  lds_sync();
+  invert(shL, shT, wave, lane);
+  float v8[2][8], mt = 0.0f;
+#pragma unroll
+  for (int sp = 0; sp < 2; ++sp) {
+    if (2 * sp < tiles) {
+      const int j0 = 32 * sp + 8 * q;
+      const float4 x = *(const float4*)(shT + mine * kRowL + j0),
+                   y = *(const float4*)(shT + mine * kRowL + j0 + 4);
+      const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v8[sp][e] = j0 + e < mine ? w[e] : 0.0f;  // without the ones
+        mt = max_abs(mt, v8[sp][e]);
+      }
+    }
+  }
+  put_tri(out, v8, mt, kFacT);
+}
+
+// ---------------------------------------------------------------------------
+// A sequence's chunks in turn, for 16 rows of a head's state (16 columns of v),
+// by two waves.  The first carries the state, all of whose columns it holds in
+// accumulators, from chunk to chunk; the second, a chunk behind, makes y from
+// the state and the w that the first leaves in LDS.  Nothing is exchanged
+// between lanes: results serve as operands (spread_row).
+//
+// The state S and w are held times a power of two per column, `unit`, which
+// keeps the largest of S, w and b (v - e^c K S) between kLow and kTop, where two
+// halves are good to 2^-22 of it.  It changes only when one leaves that range.
+// ---------------------------------------------------------------------------
+constexpr float kTop = 32768.0f, kLow = 1.0f;
+
+__device__ __forceinline__ int exponent_bits(float v) { return (int)(__float_as_uint(v) >> 23 & 255); }
+// The power of two, of up to 2^-126 and 2^100, that takes a magnitude with the
+// exponent bits e to about 2^8, as far as `unit` times it stays in that range.
+__device__ __forceinline__ float to_range(int e, float unit) {
+  const int ue = exponent_bits(unit);
+  const int d = min(max(8 + 127 - e, max(1 - ue, -126)), min(227 - ue, 100));
+  return __uint_as_float((uint32_t)(127 + d) << 23);
+}
+
+template <int NK>
+struct ScanLds {
+  static constexpr int kS = NK * 2 * 1024, kW = 2 * 2 * 1024;
+  static constexpr int kBuffer = kS + kW + 3 * 64;  // S, w; per column: units of both, first bad row
+};
+
+template <typename T, int NK>
+__global__ __launch_bounds__(128, 1) void k_delta_scan(
+    DeltaArgs a, DeltaPlan pl, int64_t items, int slices, bool by_seq) {
+  using L = ScanLds<NK>;
+  constexpr int KP = kHalves<T>, NT = 2 * NK;
+  __shared__ __attribute__((aligned(16))) uint8_t sh[2][L::kBuffer];
+  const int64_t block = wide_block();
+  const int64_t part = block / a.heads;
+  const int h = uniform((int)(block - part * a.heads));
+  const int64_t item = part / slices;
+  const int slice = uniform((int)(part - item * slices));
+  if (item >= items) return;
+  int b, s, e;
+  const int slots = first_slots(a.q);
+  if (by_seq) {
+    b = (int)item;
+    s = a.q.seq_start ? seq_row(a.q, b) : 0;
+    e = a.q.seq_start ? seq_row(a.q, b + 1) : a.q.n_tokens;
+  } else {  // the sequence whose first row on a multiple of 32 this is
+    if (32 * item >= a.q.n_tokens) return;
+    b = find_row(a.q, (int)(32 * item), &e);
+    if (b < 0) return;
+    s = a.q.seq_start ? seq_row(a.q, b) : 0;
+    if ((s + 31) / 32 != item) return;
+  }
+  b = uniform(b);
+  s = uniform(s);
+  e = uniform(e);
+  if (e - s <= kShort) return;
+  const int slot = uniform(find_slot(a.q, b, slots));
+  if (slot == kNoSlot) return;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int g = uniform(h / (a.heads / a.groups));
+  const int64_t place0 = pl.by_rows ? s / 32 : (int64_t)(s / kC) + b;
+  const int chunks = (e - s + kC - 1) / kC;
+  const int p = slice * 16 + r;
+  const uint32_t col = p < a.hd ? (uint32_t)(((int64_t)h * a.hd + p) * sizeof(T)) : kNoColumn;
+  // what the first launch left of a chunk
+  const uint8_t* keys0 = pl.keys + (place0 * a.groups + g) * pl.key_bytes;
+  const uint8_t* heads0 = pl.heads + (place0 * a.heads + h) * pl.head_bytes;
+  const int64_t key_step = a.groups * pl.key_bytes, head_step = a.heads * pl.head_bytes;
+  auto keys_of = [&](int c) { return rows_at(keys0 + c * key_step, (uint32_t)pl.key_bytes); };
+  auto head_of = [&](int c) { return rows_at(heads0 + c * head_step, (uint32_t)pl.head_bytes); };
+  auto operand = [&](__amdgpu_buffer_rsrc_t at, int off) {  // a kilobyte, 16 bytes per lane
+    return __builtin_bit_cast(v8h, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16, off, 0));
+  };
+  auto scalars = [&](__amdgpu_buffer_rsrc_t at, int k, v4f (&v)[4]) {  // of the lane's rows of each tile
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      v[w] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(
+                                         at, q * 32, 2 * kTri + k * 256 + spread_row(w, 0) * 4, 0));
+  };
+  auto triangle = [&](__amdgpu_buffer_rsrc_t at, int off, v8h (&f)[6][2]) {
+#pragma unroll
+    for (int k = 0; k < 6; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[k][i] = operand(at, off + k * 2048 + i * 1024);
+  };
+  // block (w, x) of T or A times rows 32 x .. of v, for all four row tiles
+  auto times_triangle = [&](const v8h (&f)[6][2], const v8h (&v)[2][2], v4f (&o)[4]) {
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    o[0] = mfma_h(f[0], v[0], zero);
+    o[1] = mfma_h(f[1], v[0], zero);
+    o[2] = mfma_h(f[2], v[0], zero);
+    o[3] = mfma_h(f[4], v[0], zero);
+    o[2] = mfma_h(f[3], v[1], o[2]);
+    o[3] = mfma_h(f[5], v[1], o[3]);
+  };
+  // 16 values of v or z in the lane's column
+  auto values = [&](const void* at, int64_t stride, int c, uint32_t (&v)[4][4]) {
+    const uint32_t step = (uint32_t)(stride * sizeof(T)), at0 = anew(col + 8 * q * step);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row = s + c * kC + 32 * half;
+      const auto from = rows_of<T>(at, row, stride, at ? uniform(max(0, min(32, e - row))) : 0);
+#pragma unroll
+      for (int w = 2 * half; w < 2 * half + 2; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[w][i] = load_raw<T>(from, at0 + (spread_row(w & 1, 0) + i) * step);
+    }
+  };
+  const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+
+  if (threadIdx.x < 64) {
+    // ---- the state ----
+    const bool keep = slot >= 0 && !(a.q.fresh && a.q.fresh[b]);
+    const auto bst = rows_at(a.state + (slot >= 0 ? (int64_t)slot * a.ss : 0) +
+                                 ((int64_t)h * a.hd + slice * 16) * a.n,
+                             slot >= 0 ? (uint32_t)(min(16, a.hd - slice * 16) * a.n * 4) : 0);
+    auto state_off = [&](uint32_t n0, int t, int i) {
+      const int n = (int)n0 + spread_row(t, i);
+      return n < a.n ? (uint32_t)((r * a.n + n) * 4) : kNoColumn;
+    };
+    v4f S[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        S[t][i] = keep ? load_row<float, 1>(bst, state_off(8 * q, t, i)).v[0] : 0.0f;
+    // Operands are loaded a step of the chunk or two before their products:
+    // K in the shadow of the chunk before, T of K S, K by columns of T R.
+    v8h kf[NK][4][KP], kt[NT][2][KP], tf[6][2];
+    uint32_t vr[4][4];
+    v4f beta[4], grow[4], left[4], fac[4];
+    auto fetch_k = [&](int c) {
+      const auto k = keys_of(c);
+#pragma unroll
+      for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < KP; ++i) kf[x][w][i] = operand(k, ((w * NK + x) * KP + i) * 1024);
+    };
+    float unit = 1.0f;
+    auto rescale = [&](float f) {
+      unit *= f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) S[t] *= f;
+    };
+    auto fetch_kt = [&](int c) {
+        const auto k = keys_of(c);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < KP; ++i)
+              kt[t][x][i] = operand(k, (8 * NK * KP + (t * 2 + x) * KP + i) * 1024);
+    };
+    fetch_k(0);
+    triangle(head_of(0), 0, tf);
+    scalars(head_of(0), kFacT, fac);
+    fetch_kt(0);
+    values(a.v, a.vs, 0, vr);
+    scalars(head_of(0), kBeta, beta);
+    scalars(head_of(0), kGrowK, grow);
+    for (int c = 0; c < chunks; ++c) {
+      const int next = c + 1 < chunks ? c + 1 : c;
+      const auto head = head_of(c);
+      const float* misc = (const float*)(heads0 + c * head_step + 2 * kTri) + kMisc * 64;
+      const float dec_hi = misc[0], dec_lo = misc[1], most = fmaxf(misc[3], 1.0f);
+      const int first = ((const int*)misc)[2];
+      uint8_t* buf = sh[c & 1];
+      float ms = 0.0f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ms = max_abs(ms, S[t][i]);
+      ms = quads_max(ms);
+      if (__ballot(!(ms <= kTop))) {
+        const float f = ms > kTop && ms < __builtin_inff() ? to_range(exponent_bits(ms), unit) : 1.0f;
+        rescale(f);
+        ms *= f;
+      }
+      // K S, and S for the other wave
+      v4f X[4];
+      auto product = [&](auto keys) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) X[w] = zero;
+#pragma unroll
+        for (int x = 0; x < NK; ++x) {
+          v8h sf[2];
+          halves8<2>(sf, S[2 * x], S[2 * x + 1]);
+          *(v8h*)(buf + x * 2048 + lane * 16) = sf[0];
+          *(v8h*)(buf + x * 2048 + 1024 + lane * 16) = sf[1];
+          keys(x, [&](int w, const v8h (&k)[KP]) { X[w] = mfma_h(k, sf, X[w]); });
+        }
+        if (q == 0) ((float*)(buf + L::kS + L::kW))[r] = __builtin_amdgcn_rcpf(unit);
+      };
+      product([&](int x, auto f) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) f(w, kf[x][w]);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_k(next);
+      // R = b (v - e^c K S)
+      v4f R[4];
+      auto residue = [&]() {
+        float m = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            R[w][i] = beta[w][i] * __builtin_fmaf(-grow[w][i], X[w][i], raw_f32<T>(vr[w][i]) * unit);
+            m = max_abs(m, R[w][i]);
+          }
+        return quads_max(m);
+      };
+      // infinities and NaN leave the products; `at` is the first row of one
+      int at = kC;
+      auto tame = [&](v4f (&v)[4]) {
+        float m = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!(__builtin_fabsf(v[w][i]) < __builtin_inff())) {
+              at = min(at, spread_row(w, 4 * q + i));
+              v[w][i] = 0.0f;
+            }
+            m = max_abs(m, v[w][i]);
+          }
+        return quads_max(m);
+      };
+      const float mr = residue(), mm = __builtin_elementwise_maximum(mr, ms);
+      if (__ballot(!(mr <= kTop) || (mm < kLow && mm > 0.0f && unit < 0x1p100f))) {
+        // The unit by the largest finite value, in bits of an exponent; what was
+        // computed in the old one may have passed fp32 or been too small for
+        // halves, S among it, and is worked out anew.
+        int bits = exponent_bits(mm);
+        if (!(mr < __builtin_inff())) {
+          float mv = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = __builtin_fabsf(raw_f32<T>(vr[w][i]));
+              mv = v < __builtin_inff() ? fmaxf(mv, v) : mv;
+            }
+          mv = quads_max(mv);
+          bits = max(exponent_bits(mv) + exponent_bits(unit) - 127,
+                     ms < __builtin_inff() ? exponent_bits(ms) : 0);
+          if (mv == 0.0f && !(ms > 0.0f)) bits = 8 + 127;
+        }
+        const bool off = !(mr <= kTop) || (mm < kLow && mm > 0.0f);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // one power of two may not reach
+          const float f = off ? to_range(bits, unit) : 1.0f;
+          rescale(f);
+          bits += exponent_bits(f) - 127;
+        }
+        const auto k = keys_of(c);
+        product([&](int x, auto fn) {
+          for (int w = 0; w < 4; ++w) {
+            v8h kw[KP];
+#pragma unroll
+            for (int i = 0; i < KP; ++i) kw[i] = operand(k, ((w * NK + x) * KP + i) * 1024);
+            switch (w) {  // registers have no index
+              case 0: fn(0, kw); break;
+              case 1: fn(1, kw); break;
+              case 2: fn(2, kw); break;
+              default: fn(3, kw); break;
+            }
+          }
+        });
+        (void)residue();
+        const float m = tame(R), f = m > kTop ? to_range(exponent_bits(m), unit) : 1.0f;
+        rescale(f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) R[w] *= f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      scalars(head, kLeft, left);
+      values(a.v, a.vs, next, vr);
+      scalars(head_of(next), kBeta, beta);
+      scalars(head_of(next), kGrowK, grow);
+      // w = T R, T without its ones
+      v4f W[4];
+      auto solve = [&]() {
+        v8h rf[2][2];
+        halves8<2>(rf[0], R[0], R[1]);
+        halves8<2>(rf[1], R[2], R[3]);
+        times_triangle(tf, rf, W);
+        float m = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            W[w][i] = __builtin_fmaf(fac[w][i], W[w][i], R[w][i]);
+            m = max_abs(m, W[w][i]);
+          }
+        return quads_max(m);
+      };
+      float mw = solve();
+      if (__ballot(!(mw * most <= kTop))) {
+        if (__ballot(!(mw < __builtin_inff()))) mw = tame(W);
+        const float f = mw * most > kTop
+                            ? to_range(exponent_bits(mw) + exponent_bits(most) - 127, unit)
+                            : 1.0f;
+        rescale(f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) W[w] *= f;
+      }
+      int from = first;  // the column's rows from here on are NaN
+      if (__ballot(at < kC)) {
+        at = min(at, __shfl_xor(at, 16));
+        from = min(from, min(at, __shfl_xor(at, 32)));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      triangle(head_of(next), 0, tf);
+      scalars(head_of(next), kFacT, fac);
+      // w for the other wave, and times e^{c_C - c} for the state
+      v8h lf[2][2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        v8h wf[2];
+        halves8<2>(wf, W[2 * x], W[2 * x + 1]);
+        *(v8h*)(buf + L::kS + x * 2048 + lane * 16) = wf[0];
+        *(v8h*)(buf + L::kS + x * 2048 + 1024 + lane * 16) = wf[1];
+        halves8<2>(lf[x], W[2 * x] * left[2 * x], W[2 * x + 1] * left[2 * x + 1]);
+      }
+      if (q == 0) {
+        ((float*)(buf + L::kS + L::kW))[16 + r] = __builtin_amdgcn_rcpf(unit);
+        ((int*)(buf + L::kS + L::kW))[32 + r] = from;
+      }
+      const float keep_hi = from < kC ? __builtin_nanf("") : dec_hi;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[t][i] = __builtin_fmaf(S[t][i], keep_hi, S[t][i] * dec_lo);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) S[t] = mfma_h(kt[t][x], lf[x], S[t]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_kt(next);
+      lds_sync();
+    }
+    if (a.frozen) return;
+    const float down = __builtin_amdgcn_rcpf(unit);
+    const uint32_t n0 = anew(8 * q);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float o[1] = {S[t][i] * down};
+        store_row<float, 1>(bst, state_off(n0, t, i), o);
+      }
+  } else {
+    // ---- y ----
+    const uint32_t ys = (uint32_t)(a.ys * sizeof(T));
+    v8h qf[NK][4][KP], af[6][2];
+    uint32_t zr[4][4];
+    v4f grow[4], fac[4];
+    auto fetch_q = [&](int c) {
+      const auto k = keys_of(c);
+#pragma unroll
+      for (int x = 0; x < NK; ++x)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < KP; ++i) qf[x][w][i] = operand(k, (((4 + w) * NK + x) * KP + i) * 1024);
+    };
+    fetch_q(0);
+    for (int c = 0; c < chunks; ++c) {
+      const int next = c + 1 < chunks ? c + 1 : c;
+      const uint8_t* buf = sh[c & 1];
+      const auto head = head_of(c);
+      triangle(head, kTri, af);
+      values(a.z, a.zs, c, zr);
+      scalars(head, kGrowQ, grow);
+      scalars(head, kFacA, fac);
+      lds_sync();
+      v4f X[4] = {zero, zero, zero, zero}, Y[4];
+#pragma unroll
+      for (int x = 0; x < NK; ++x) {
+        const v8h sf[2] = {*(const v8h*)(buf + x * 2048 + lane * 16),
+                           *(const v8h*)(buf + x * 2048 + 1024 + lane * 16)};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) X[w] = mfma_h(qf[x][w], sf, X[w]);
+      }
+      fetch_q(next);
+      v8h wf[2][2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          wf[x][i] = *(const v8h*)(buf + L::kS + x * 2048 + i * 1024 + lane * 16);
+      times_triangle(af, wf, Y);
+      const float* cols = (const float*)(buf + L::kS + L::kW);
+      const float us = cols[r], uw = cols[16 + r];
+      const int from = ((const int*)cols)[32 + r];
+      float y[4][4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          y[w][i] = __builtin_fmaf(us * grow[w][i], X[w][i], uw * fac[w][i] * Y[w][i]);
+      if (a.z) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[w][i] *= sizeof(T) == 4 ? silu_f32(raw_f32<T>(zr[w][i])) : silu_short(raw_f32<T>(zr[w][i]));
+      }
+      if (__ballot(from < kC)) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[w][i] = spread_row(w, 4 * q + i) < from ? y[w][i] : __builtin_nanf("");
+      }
+      const uint32_t at0 = anew(col + 8 * q * ys);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = s + c * kC + 32 * half;
+        const auto by = rows_of<T>(a.y, row, a.ys, uniform(max(0, min(32, e - row))));
+#pragma unroll
+        for (int w = 2 * half; w < 2 * half + 2; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float o[1] = {y[w][i]};
+            store_row<T, 1>(by, at0 + (spread_row(w & 1, 0) + i) * ys, o);
+          }
+      }
+    }
+  }
+}
+
+static int delta_nk(int n) { return n <= 64 ? 2 : (n <= 128 ? 4 : 8); }
+
+template <typename T, int NK>
+static hipError_t launch_chunks(const DeltaArgs& a, const DeltaPlan& pl, hipStream_t s) {
+  const dim3 grid = wide_grid(pl.units, a.heads);
+  const hipError_t e = pl.wide ? launch(k_delta_chunk<T, NK, true>, grid, dim3(256), 0, s, a, pl)
+                               : launch(k_delta_chunk<T, NK, false>, grid, dim3(256), 0, s, a, pl);
+  if (e != hipSuccess) return e;
+  // of the sequences, or the rows on multiples of 32, whichever are fewer
+  const int64_t marks = a.q.n_tokens / 32 + 1;
+  const bool by_seq = a.q.n_seqs <= marks;
+  const int64_t items = by_seq ? a.q.n_seqs : marks;
+  const int slices = (a.hd + 15) / 16;
+  return launch(k_delta_scan<T, NK>, wide_grid(items * slices * a.heads, 1), dim3(128), 0, s, a, pl,
+                items, slices, by_seq);
+}
+
+template <typename T>
+static hipError_t launch_delta(const DeltaArgs& a, const DeltaPlan& pl, bool step, hipStream_t s) {
+  if (step) return launch_rows_t<T, true>(a, 1, s);
+  if (a.q.seq_start || !pl.chunks) {
+    const hipError_t e = launch_rows_t<T, false>(a, kShort, s);
+    if (e != hipSuccess || !pl.chunks) return e;
+  }
+  switch (delta_nk(a.n)) {
+    case 2: return launch_chunks<T, 2>(a, pl, s);
+    case 4: return launch_chunks<T, 4>(a, pl, s);
+    default: return launch_chunks<T, 8>(a, pl, s);
+  }
+}
+
+// The places of sequences of more than kShort rows: from row / kC + b on there
+// are enough for any, from row / 32 on for those (n / 32 rounded down is at
+// least n / kC rounded up then).  Both counts only grow with rows and sequences.
+static DeltaPlan delta_plan(const bm_hip_delta_t* op, void* workspace) {
+  DeltaPlan pl{};
+  pl.chunks = op->n_tokens > kShort;
+  if (!pl.chunks) return pl;
+  const size_t elem = type_bytes(op->type);
+  pl.wide = op->d_state % 8 == 0 && op->q_stride * elem % 4 == 0 && op->k_stride * elem % 4 == 0 &&
+            ((uintptr_t)op->q | (uintptr_t)op->k) % 4 == 0;
+  pl.units = unit_count(op->n_seqs, op->n_tokens, kC);
+  const int64_t by_rows = op->n_tokens / 32 + 1;
+  pl.by_rows = by_rows < pl.units;
+  pl.places = pl.by_rows ? by_rows : pl.units;
+  pl.head_bytes = 2 * kTri + kScalars;
+  pl.key_bytes = (int64_t)12 * delta_nk(op->d_state) * (elem == 4 ? 2 : 1) * 1024;
+  const size_t heads = (size_t)(pl.places * op->n_heads * pl.head_bytes);
+  pl.heads = (uint8_t*)workspace;
+  pl.keys = (uint8_t*)((uintptr_t)workspace + heads);
+  pl.bytes = heads + (size_t)(pl.places * op->n_groups * pl.key_bytes);
+  return pl;
 }
 
 static bool delta_fits(const char* name, const bm_hip_delta_t* op) {
@@ -270,7 +1284,7 @@ static bool delta_fits(const char* name, const bm_hip_delta_t* op) {
 
 extern "C" size_t bm_hip_delta_workspace_bytes(const bm_hip_delta_t* op) {
   if (!bm::delta_fits("delta_workspace", op) || op->n_tokens < 0 || op->n_seqs < 0) return 0;
-  return 0;
+  return bm::delta_plan(op, nullptr).bytes;
 }
 
 static int delta_call(const bm_hip_delta_t* op, void* workspace, void* stream, bool step) {
@@ -310,7 +1324,11 @@ static int delta_call(const bm_hip_delta_t* op, void* workspace, void* stream, b
     bm_set_error("%s: A and dt_bias need addresses on 4 bytes", name);
     return -2;
   }
-  (void)workspace;
+  const bm::DeltaPlan pl = bm::delta_plan(op, workspace);
+  if (!step && pl.bytes && (!workspace || (uintptr_t)workspace % 256)) {
+    bm_set_error("%s: a workspace of %zu bytes on 256 bytes is required", name, pl.bytes);
+    return -2;
+  }
   if (op->n_seqs == 0) return 0;
   if (!bm_hip_init()) return -1;
   bm::OnDevice dev;
@@ -350,16 +1368,9 @@ static int delta_call(const bm_hip_delta_t* op, void* workspace, void* stream, b
   hipStream_t s = bm::stream_of(stream);
   hipError_t e;
   switch (op->type) {
-    case BM_HIP_F32:
-      e = step ? bm::launch_rows_t<float, true>(a, s) : bm::launch_rows_t<float, false>(a, s);
-      break;
-    case BM_HIP_BF16:
-      e = step ? bm::launch_rows_t<__bf16, true>(a, s) : bm::launch_rows_t<__bf16, false>(a, s);
-      break;
-    default:
-      e = step ? bm::launch_rows_t<_Float16, true>(a, s)
-               : bm::launch_rows_t<_Float16, false>(a, s);
-      break;
+    case BM_HIP_F32: e = bm::launch_delta<float>(a, pl, step, s); break;
+    case BM_HIP_BF16: e = bm::launch_delta<__bf16>(a, pl, step, s); break;
+    default: e = bm::launch_delta<_Float16>(a, pl, step, s); break;
   }
   BM_HIP_CHECK_RET(e, -1);
   return 0;

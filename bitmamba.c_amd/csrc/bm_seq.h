@@ -276,6 +276,28 @@ __device__ __forceinline__ Unit find_unit(const SeqView& q, int u, int len) {
   }
 }
 
+// The sequence that a row belongs to, -1: none; all lanes with the same row.
+// Its rows are s .. e - 1.
+__device__ __forceinline__ int find_row(const SeqView& q, int row, int* e) {
+  *e = q.n_tokens;
+  if (!q.seq_start) return 0;
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = q.n_seqs;  // entries lo .. hi; the last is no sequence's first
+  for (;;) {
+    const int step = (hi - lo + 62) / 63;
+    const int i = min(lo + lane * step, hi);
+    const int r = seq_row(q, i);
+    const int c = __popcll(__ballot(i < hi && r <= row));
+    if (c == 0) return -1;
+    if (step == 1) {
+      *e = __builtin_amdgcn_readlane(r, c);
+      return row < *e ? lo + c - 1 : -1;
+    }
+    lo += (c - 1) * step;
+    hi = min(hi, lo + step);
+  }
+}
+
 constexpr int kNoSlot = -1, kNoPool = -2;
 // The slots of the first 64 sequences, one per lane: a load that waits for
 // nothing, issued before the sequence is known.

@@ -459,12 +459,13 @@ int bm_hip_ssm_step_dev(const bm_hip_ssm_t *op, void *stream);
  *
  * A key with b * (sum of k's squares) above 2 makes the rule grow without
  * end; qk_norm with b in 0..2 cannot.  Where such a growth passes fp32, the
- * head's later rows of the sequence are infinite, NaN or undefined.  A head's
- * q, k, dt or beta that is infinite or NaN, or whose squares' sum is, makes
- * the head NaN from that row on (q: in that row), a v[p] or state row p that
- * row of the state; earlier rows, other rows of the state, other heads and
- * sequences are not reached.  fp32 values of 2^128 - 2^119 and more count as
- * infinite.  */
+ * head's later rows of the sequence are infinite, NaN or undefined.
+ *
+ * Where a head's a or b is NaN or b infinite, or the sum of k's squares is
+ * either (in fp32), the head is NaN from that row on, y and state; where that
+ * of q is, its y in that row.  An infinite or NaN v[p] or S[p][n] makes y[p]
+ * and S[p] infinite or NaN from its row on.  Earlier rows, other p, other heads
+ * and other sequences are not reached. */
 typedef struct {
     int type;                      /* of q, k, v, dt, beta, z, y */
     int n_heads, head_dim;         /* v, z, y rows: [n_heads][head_dim] */
@@ -488,7 +489,7 @@ typedef struct {
 
 /* Prompts.  The workspace as bm_hip_ssm_dev's: any contents, on 256 bytes,
  * one of an op serves every call of no more sequences and rows with the same
- * type, n_heads and d_state. */
+ * type, n_heads, n_groups and d_state. */
 size_t bm_hip_delta_workspace_bytes(const bm_hip_delta_t *op);
 int bm_hip_delta_dev(const bm_hip_delta_t *op, void *workspace, void *stream);
 /* One token of each sequence; y may be written over v itself. */
