@@ -19,8 +19,11 @@
 
 namespace bm {
 
-constexpr int kVerifyThreads = 256, kPerThread = 16;
-constexpr int kSegment = kVerifyThreads * kPerThread;  // values of a row per block
+constexpr int kSegment = 4096;  // values of a row per block
+// threads and values of each: many of one row's values in flight where all rows
+// are read, short chains where a sequence waits for one
+constexpr int kRowsThreads = 256, kRowsValues = kSegment / kRowsThreads;
+constexpr int kDrawThreads = 1024, kDrawValues = kSegment / kDrawThreads;
 constexpr int kMaxVocab = 256000;
 static_assert((kMaxVocab + kSegment - 1) / kSegment <= 64, "a segment per lane");
 
@@ -35,7 +38,8 @@ struct RowSum {
 };
 // What the draw of a sequence goes by
 struct Draw {
-  int row, last;       // row -1: none
+  int row;             // -1: none
+  float u;
   int p_kind, q_kind;  // q_kind -1: p alone
   float pm, qm;        // maxima
   int q_at;            // of a q that is 1 at one token
@@ -59,70 +63,96 @@ struct VerifyArgs {
   Draw* draws;   // [sequences]
 };
 
-// 2^t for t at most 0 (NaN: 0): the series of e^{f ln 2}, |f| <= 1/2, up to
-// f^11, which leaves (ln 2 / 2)^12 / 12! < 2^-47
+// 2^t for t at most 0 (NaN: 0): a polynomial on the fraction that is off by
+// 2^-46 at most (fitted to 2^f on -1/2 .. 1/2 by exchange of its extrema)
 __device__ __forceinline__ double exp2_f64(double t) {
-  constexpr double c1 = 0.693147180559945309417, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3,
-                   c4 = c3 * c1 / 4, c5 = c4 * c1 / 5, c6 = c5 * c1 / 6, c7 = c6 * c1 / 7,
-                   c8 = c7 * c1 / 8, c9 = c8 * c1 / 9, c10 = c9 * c1 / 10, c11 = c10 * c1 / 11;
-  t = __builtin_fmax(t, -1100.0);
+  constexpr double c[10] = {0x1.0000000000039p+0,  0x1.62e42fefa3752p-1,  0x1.ebfbdff81570dp-3,
+                            0x1.c6b08d70d2003p-5,  0x1.3b2ab72a1098dp-7,  0x1.5d87fd9011eeep-10,
+                            0x1.43088fca9a183p-13, 0x1.ffce24611c0dap-17, 0x1.63edf1058a76ep-20,
+                            0x1.b3f421492867dp-24};
+  // the larger one, -1100 for NaN: one instruction, where fmax() takes two
+  asm("v_max_f64 %0, %1, %2" : "=v"(t) : "v"(t), "s"(-1100.0));
   const double n = __builtin_rint(t), f = t - n;
-  double r = c11;
-  r = __builtin_fma(r, f, c10);
-  r = __builtin_fma(r, f, c9);
-  r = __builtin_fma(r, f, c8);
-  r = __builtin_fma(r, f, c7);
-  r = __builtin_fma(r, f, c6);
-  r = __builtin_fma(r, f, c5);
-  r = __builtin_fma(r, f, c4);
-  r = __builtin_fma(r, f, c3);
-  r = __builtin_fma(r, f, c2);
-  r = __builtin_fma(r, f, c1);
-  r = __builtin_fma(r, f, 1.0);
+  double r = c[9];
+  // with the coefficient in scalar registers; the compiler copies each into the
+  // result's registers first, two moves per step
+#pragma unroll
+  for (int i = 8; i >= 0; --i)
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(r), "v"(f), "s"(c[i]));
   return __builtin_ldexp(r, (int)n);
 }
-// a value's share of a row whose largest is m, before the sum divides it
-__device__ __forceinline__ double share_of(int kind, float v, float m, double k) {
+// What a row's shares are taken from: its largest value, or 0 where that is no
+// finite one
+struct Top {
+  double m;
+  bool odd;  // the largest is infinite: +inf has everything, or there is nothing
+  float at;
+};
+__device__ __forceinline__ Top top_of(float m) {
+  const bool odd = !(__builtin_fabsf(m) < __builtin_inff());
+  return Top{odd ? 0.0 : (double)m, odd, m};
+}
+// a value's share of a row, up to the row's sum
+__device__ __forceinline__ double share_of(int kind, float v, const Top& m, double k) {
   if (kind == kWeights) return v > 0.0f && v < __builtin_inff() ? (double)v : 0.0;
-  const double d = v == m ? 0.0 : (double)v - (double)m;  // infinite ones too
-  return m == -__builtin_inff() ? 0.0 : exp2_f64(d * k);
+  if (m.odd) return m.at > 0.0f && v == m.at ? 1.0 : 0.0;
+  return exp2_f64(((double)v - m.m) * k);
 }
 
-// Values i .. i + 15 of a row on any alignment of T; `none` past its end.  Words
-// of four bytes are read, so a row of two-byte values that starts or ends within
-// a word is read with its neighbour in that word.
-struct alignas(4) Words4 {
-  uint32_t w[4];
-};
-template <typename T>
-__device__ __forceinline__ void load16(float (&o)[kPerThread], const T* row, int i, int vocab,
-                                       float none) {
-  static_assert(kPerThread == 16, "");
-  if (i + 16 > vocab) {
+// the shares of N values; one branch for all of them
+template <int N>
+__device__ __forceinline__ void shares(double (&o)[N], int kind, const float (&v)[N], float largest,
+                                       double k) {
+  const Top top = top_of(largest);
+  if (kind == kWeights) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] = i + j < vocab ? (float)row[i + j] : none;
+    for (int j = 0; j < N; ++j) o[j] = share_of(kWeights, v[j], top, k);
+  } else if (top.odd) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = top.at > 0.0f && v[j] == top.at ? 1.0 : 0.0;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = exp2_f64(((double)v[j] - top.m) * k);
+  }
+}
+
+// Values i .. i + N - 1 of a row on any alignment of T; `none` past its end.
+// Words of four bytes are read, so a row of two-byte values that starts or ends
+// within a word is read with its neighbour in that word.
+template <int W>
+struct alignas(4) Words {
+  uint32_t w[W];
+};
+template <typename T, int N>
+__device__ __forceinline__ void load_row_at(float (&o)[N], const T* row, int i, int vocab, float none) {
+  static_assert(N % 4 == 0, "");
+  if (i + N > vocab) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = i + j < vocab ? (float)row[i + j] : none;
     return;
   }
   if constexpr (sizeof(T) == 4) {
-    Words4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *(const Words4*)(row + i + 4 * j);
+    for (int j = 0; j < N; j += 4) {
+      const Words<4> v = *(const Words<4>*)(row + i + j);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[j] = __uint_as_float(v[j >> 2].w[j & 3]);
+      for (int k = 0; k < 4; ++k) o[j + k] = __uint_as_float(v.w[k]);
+    }
   } else {
     const uintptr_t at = (uintptr_t)(row + i);
     const int odd = (int)(at >> 1 & 1);  // the same for the whole row, i being even
     const uint32_t* w = (const uint32_t*)(at - 2 * odd);
-    const Words4 a = *(const Words4*)w, b = *(const Words4*)(w + 4);
-    uint32_t v[9];
+    constexpr int kWords = N / 2, kEach = kWords < 4 ? kWords : 4;
+    uint32_t v[kWords + 1];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = a.w[j];
-      v[4 + j] = b.w[j];
+    for (int j = 0; j < kWords; j += kEach) {
+      const Words<kEach> x = *(const Words<kEach>*)(w + j);
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) v[j + k] = x.w[k];
     }
-    v[8] = odd ? w[8] : 0;
+    v[kWords] = odd ? w[kWords] : 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kWords; ++j) {
       const uint32_t x = odd ? __builtin_amdgcn_alignbit(v[j + 1], v[j], 16) : v[j];
       o[2 * j] = (float)__builtin_bit_cast(T, (uint16_t)x);
       o[2 * j + 1] = (float)__builtin_bit_cast(T, (uint16_t)(x >> 16));
@@ -130,17 +160,41 @@ __device__ __forceinline__ void load16(float (&o)[kPerThread], const T* row, int
   }
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+// running sums over the wave on DPP
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  auto add = [&](auto dpp) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)dpp((int)(uint32_t)b), hi = (uint32_t)dpp((int)(uint32_t)(b >> 32));
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);  // +0 without a source
+  };
+  add([](int x) { return dpp_or0<0x111>(x); });
+  add([](int x) { return dpp_or0<0x112>(x); });
+  add([](int x) { return dpp_or0<0x114>(x); });
+  add([](int x) { return dpp_or0<0x118>(x); });
+  add([](int x) { return dpp_or0<0x142, 0xa>(x); });
+  add([](int x) { return dpp_or0<0x143, 0xc>(x); });
   return v;
 }
+__device__ __forceinline__ double read_lane(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane),
+                 hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_f64(double v) { return read_lane(wave_scan_f64(v), 63); }
 __device__ __forceinline__ int wave_min_i32(int v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v = min(v, __shfl_xor(v, m));
-  return v;
+  v = min(v, dpp_mov<0xB1>(v));
+  v = min(v, dpp_mov<0x4E>(v));
+  v = min(v, dpp_mov<0x141>(v));
+  v = min(v, dpp_mov<0x140>(v));
+  return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
+// what a sum to the largest value v counts in one to m
+__device__ __forceinline__ double from_top(float v, float m, double k) {
+  return v == m ? 1.0 : exp2_f64(((double)v - (double)m) * k);
+}
 // the maximum of four waves' and the sum to it
 template <int N>
 __device__ __forceinline__ RowSum join_sums(int kind, const RowSum (&v)[N], double k) {
@@ -154,8 +208,7 @@ __device__ __forceinline__ RowSum join_sums(int kind, const RowSum (&v)[N], doub
   o.s = 0.0;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    o.s += kind == kWeights ? v[i].s
-                            : v[i].s * (v[i].m == o.m ? 1.0 : exp2_f64(((double)v[i].m - o.m) * k));
+    o.s += kind == kWeights ? v[i].s : v[i].s * from_top(v[i].m, o.m, k);
   return o;
 }
 
@@ -163,33 +216,36 @@ __device__ __forceinline__ RowSum join_sums(int kind, const RowSum (&v)[N], doub
 // One segment of one row of the target (z 0) or the draft (z 1).
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kVerifyThreads) void k_verify_rows(VerifyArgs a) {
-  __shared__ RowSum part[kVerifyThreads / 64];
+__global__ __launch_bounds__(kRowsThreads) void k_verify_rows(VerifyArgs a) {
+  __shared__ RowSum part[kRowsThreads / 64];
   const bool draft = blockIdx.y != 0;
   const int64_t block = wide_block();
   const int64_t row = block / a.segments;
   if (row >= a.q.n_tokens) return;
-  int end;
-  if (find_row(a.q, (int)row, &end) < 0 || (draft && row == end - 1)) return;
   const int seg = (int)(block - row * a.segments);
   const int kind = draft ? a.q_kind : a.p_kind;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int i0 = seg * kSegment + tid * kPerThread;
-  float v[kPerThread];
-  load16<T>(v, (const T*)(draft ? a.d : a.p) + row * (draft ? a.ds : a.ps), i0, a.vocab,
-            kind == kWeights ? 0.0f : -__builtin_inff());
+  const int i0 = seg * kSegment + tid * kRowsValues;
+  const float none = kind == kWeights ? 0.0f : -__builtin_inff();
+  float v[kRowsValues];
+  if (!draft) load_row_at<T>(v, (const T*)a.p + row * a.ps, i0, a.vocab, none);  // in the search's shadow
+  int end;
+  if (find_row(a.q, (int)row, &end) < 0 || (draft && row == end - 1)) return;
+  if (draft) load_row_at<T>(v, (const T*)a.d + row * a.ds, i0, a.vocab, none);
   RowSum o{0.0, -__builtin_inff(), INT32_MAX};
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) o.m = fmaxf(o.m, v[j]);
+  for (int j = 0; j < kRowsValues; ++j) o.m = fmaxf(o.m, v[j]);
   o.m = wave_max_f32(o.m);
   if (kind == kLargest) {
 #pragma unroll
-    for (int j = kPerThread - 1; j >= 0; --j)
+    for (int j = kRowsValues - 1; j >= 0; --j)
       if (v[j] == o.m) o.at = i0 + j;
     o.at = wave_min_i32(o.at);
   } else {
+    double w[kRowsValues];
+    shares(w, kind, v, o.m, a.k);
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) o.s += share_of(kind, v[j], o.m, a.k);
+    for (int j = 0; j < kRowsValues; ++j) o.s += w[j];
     o.s = wave_sum_f64(o.s);
   }
   if (lane == 0) part[wave] = o;
@@ -199,53 +255,59 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_rows(VerifyArgs a) {
         join_sums(kind == kLargest ? (int)kWeights : kind, part, a.k);
 }
 
-// a whole row, in all lanes
-__device__ __forceinline__ RowSum row_sum(const VerifyArgs& a, int kind, int64_t row, bool draft) {
+// a row's segments, one per lane, and the whole row, in all lanes
+__device__ __forceinline__ RowSum load_sum(const VerifyArgs& a, int64_t row, bool draft) {
   const int lane = threadIdx.x & 63;
   RowSum o{0.0, -__builtin_inff(), INT32_MAX};
   if (lane < a.segments) o = a.sums[(row + (draft ? a.q.n_tokens : 0)) * a.segments + lane];
+  return o;
+}
+__device__ __forceinline__ RowSum whole_sum(const VerifyArgs& a, int kind, RowSum o) {
   const float m = wave_max_f32(o.m);
   if (kind == kLargest) {
     o.at = wave_min_i32(o.m == m && m > -__builtin_inff() ? o.at : INT32_MAX);
     if (o.at == INT32_MAX) o.at = -1;
     o.s = o.at < 0 ? 0.0 : 1.0;
   } else {
-    if (kind == kLogits) o.s *= o.m == m ? 1.0 : exp2_f64(((double)o.m - m) * a.k);
-    o.s = wave_sum_f64(lane < a.segments ? o.s : 0.0);
+    if (kind == kLogits) o.s *= from_top(o.m, m, a.k);
+    o.s = wave_sum_f64(o.s);
   }
   o.m = m;
   return o;
 }
-// the probability of a token, given the row's sum
-template <typename T>
-__device__ __forceinline__ double prob_of(const VerifyArgs& a, int kind, const T* row, RowSum r,
+// the probability of a token of the vocabulary, given its value and the row's sum
+__device__ __forceinline__ double prob_of(const VerifyArgs& a, int kind, float v, const RowSum& r,
                                           int token) {
-  if (token < 0 || token >= a.vocab) return 0.0;
   if (kind == kToken) return 1.0;
   if (kind == kLargest) return token == r.at ? 1.0 : 0.0;
-  return r.s > 0.0 ? share_of(kind, (float)row[token], r.m, a.k) / r.s : 0.0;
+  return r.s > 0.0 ? share_of(kind, v, top_of(r.m), a.k) / r.s : 0.0;
 }
 
 // a token's weight in the draw
-template <typename T>
-__device__ __forceinline__ void weights16(double (&w)[kPerThread], const VerifyArgs& a,
+template <typename T, int N>
+__device__ __forceinline__ void draw_weights(double (&w)[N], const VerifyArgs& a,
                                           const Draw& d, int i0) {
-  float v[kPerThread];
-  load16<T>(v, (const T*)a.p + (int64_t)d.row * a.ps, i0, a.vocab,
+  float v[N];
+  load_row_at<T>(v, (const T*)a.p + (int64_t)d.row * a.ps, i0, a.vocab,
             d.p_kind == kWeights ? 0.0f : -__builtin_inff());
+  shares(w, d.p_kind, v, d.pm, a.k);
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) w[j] = share_of(d.p_kind, v[j], d.pm, a.k) * d.p_inv;
+  for (int j = 0; j < N; ++j) w[j] *= d.p_inv;
   if (d.q_kind < 0) return;
   if (d.q_kind == kToken) {
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) w[j] = i0 + j == d.q_at ? 0.0 : w[j];
+    for (int j = 0; j < N; ++j) w[j] = i0 + j == d.q_at ? 0.0 : w[j];
     return;
   }
-  load16<T>(v, (const T*)a.d + (int64_t)d.row * a.ds, i0, a.vocab,
+  load_row_at<T>(v, (const T*)a.d + (int64_t)d.row * a.ds, i0, a.vocab,
             d.q_kind == kWeights ? 0.0f : -__builtin_inff());
+  double q[N];
+  shares(q, d.q_kind, v, d.qm, a.k);
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j)
-    w[j] = __builtin_fmax(w[j] - share_of(d.q_kind, v[j], d.qm, a.k) * d.q_inv, 0.0);
+  for (int j = 0; j < N; ++j) {
+    const double left = w[j] - q[j] * d.q_inv;
+    w[j] = left > 0.0 ? left : 0.0;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -254,9 +316,9 @@ __device__ __forceinline__ void weights16(double (&w)[kPerThread], const VerifyA
 // (a launch of its own would cost more than the few rows of a draft); the
 // first writes what was decided, and goes through all rows for their ratios.
 // ---------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(kVerifyThreads) void k_verify_stop(VerifyArgs a, int blocks) {
-  constexpr int kWavesV = kVerifyThreads / 64;
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_verify_stop(VerifyArgs a, int blocks) {
+  constexpr int kWavesV = THREADS / 64, kValues = kSegment / THREADS;
   __shared__ Draw shared;
   __shared__ int first;
   __shared__ double part[kWavesV];
@@ -280,6 +342,7 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_stop(VerifyArgs a, in
     }
     return;
   }
+  const float u_last = a.u[e - 1];
   if (tid == 0) first = INT32_MAX;
   __syncthreads();
   for (int r0 = s; r0 < e; r0 += kWavesV) {
@@ -288,21 +351,24 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_stop(VerifyArgs a, in
     RowSum p{0.0, 0.0f, -1}, q{1.0, 0.0f, -1};
     int token = -1;
     if (have) {
-      p = row_sum(a, a.p_kind, row, false);
+      const bool drawn = !last && a.q_kind != kToken && a.p_kind != kLargest;
+      // all loads of a row before anything is made of them
+      if (!last) token = a.tokens[row];
+      const float u = last ? 0.0f : a.u[row];
+      p = load_sum(a, row, false);
+      if (drawn) q = load_sum(a, row, true);
+      const bool inside = token >= 0 && token < a.vocab;
+      const float pv = inside ? (float)((const T*)a.p)[row * a.ps + token] : 0.0f;
+      const float qv = inside && drawn ? (float)((const T*)a.d)[row * a.ds + token] : 0.0f;
+      p = whole_sum(a, a.p_kind, p);
       bool stands = false;
+      if (drawn) q = whole_sum(a, a.q_kind, q);
       if (!last) {
-        token = a.tokens[row];
-        const double pd = prob_of<T>(a, a.p_kind, (const T*)a.p + row * a.ps, p, token);
-        if (a.p_kind == kLargest) {
-          stands = pd > 0.0;
-          if (writer && a.ratio && lane == 0) a.ratio[row] = (float)pd;
-        } else {
-          if (a.q_kind != kToken) q = row_sum(a, a.q_kind, row, true);
-          const double qd = prob_of<T>(a, a.q_kind, (const T*)a.d + row * a.ds, q, token);
-          stands = (double)a.u[row] * qd < pd;
-          if (writer && a.ratio && lane == 0)
-            a.ratio[row] = pd > 0.0 ? (float)(pd < qd ? pd / qd : 1.0) : 0.0f;
-        }
+        const double pd = inside ? prob_of(a, a.p_kind, pv, p, token) : 0.0;
+        const double qd = inside ? prob_of(a, a.q_kind, qv, q, token) : 0.0;
+        stands = a.p_kind == kLargest ? pd > 0.0 : (double)u * qd < pd;
+        if (writer && a.ratio && lane == 0)
+          a.ratio[row] = pd > 0.0 ? (a.p_kind == kLargest || pd >= qd ? 1.0f : (float)(pd / qd)) : 0.0f;
       }
       if (!stands && lane == 0) atomicMin(&first, row);
     }
@@ -311,7 +377,7 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_stop(VerifyArgs a, in
     if (have && row == stop && lane == 0) {
       Draw d;
       d.row = p.s > 0.0 ? row : -1;
-      d.last = e - 1;
+      d.u = u_last;
       d.p_kind = a.p_kind;
       d.pm = p.m;
       d.p_inv = p.s > 0.0 ? 1.0 / p.s : 0.0;
@@ -335,10 +401,10 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_stop(VerifyArgs a, in
   const Draw d = shared;
   double sum = 0.0;
   if (d.row >= 0) {
-    double w[kPerThread];
-    weights16<T>(w, a, d, seg * kSegment + tid * kPerThread);
+    double w[kValues];
+    draw_weights<T>(w, a, d, seg * kSegment + tid * kValues);
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) sum += w[j];
+    for (int j = 0; j < kValues; ++j) sum += w[j];
   }
   sum = wave_sum_f64(sum);
   if (lane == 0) part[wave] = sum;
@@ -351,26 +417,15 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_stop(VerifyArgs a, in
   }
 }
 
-// running sums over the wave
-__device__ __forceinline__ double wave_scan_f64(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const double o = __shfl_up(v, m);
-    if (lane >= m) v += o;
-  }
-  return v;
-}
-
 // ---------------------------------------------------------------------------
 // The draw of one sequence: the segment in which the running sum passes u
 // times the whole, then the token in it.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kVerifyThreads) void k_verify_draw(VerifyArgs a) {
-  constexpr int kWavesV = kVerifyThreads / 64;
+__global__ __launch_bounds__(kDrawThreads) void k_verify_draw(VerifyArgs a) {
+  constexpr int kWavesV = kDrawThreads / 64;
   __shared__ double part[kWavesV];
-  __shared__ int at, most;
+  __shared__ int at[kWavesV], most[kWavesV];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Draw d = a.draws[b];
   if (d.row < 0) {
@@ -383,25 +438,21 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_draw(VerifyArgs a) {
     if (lane < a.segments) {
       const RowSum o = a.sums[(int64_t)d.row * a.segments + lane];
       mine = o.s * d.p_inv;
-      if (d.p_kind == kLogits) mine *= o.m == d.pm ? 1.0 : exp2_f64(((double)o.m - d.pm) * a.k);
+      if (d.p_kind == kLogits) mine *= from_top(o.m, d.pm, a.k);
     }
   }
   const double run = wave_scan_f64(mine);
-  const double want = (double)a.u[d.last] * __shfl(run, 63);
+  const double want = (double)d.u * read_lane(run, 63);
   const uint64_t in = __ballot(mine > 0.0 && run > want);
   const uint64_t any = __ballot(mine > 0.0);
   const int seg = in ? __ffsll((unsigned long long)in) - 1
                      : (any ? 63 - __clzll((long long)any) : 0);
-  const double before = seg > 0 ? __shfl(run, seg - 1) : 0.0;
-  if (tid == 0) {
-    at = INT32_MAX;
-    most = -1;
-  }
-  double w[kPerThread], sum = 0.0;
-  const int i0 = seg * kSegment + tid * kPerThread;
-  weights16<T>(w, a, d, i0);
+  const double before = seg > 0 ? read_lane(run, seg - 1) : 0.0;
+  double w[kDrawValues], sum = 0.0;
+  const int i0 = seg * kSegment + tid * kDrawValues;
+  draw_weights<T>(w, a, d, i0);
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) sum += w[j];
+  for (int j = 0; j < kDrawValues; ++j) sum += w[j];
   const double upto = wave_scan_f64(sum);
   if (lane == 63) part[wave] = upto;
   __syncthreads();
@@ -410,17 +461,27 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_draw(VerifyArgs a) {
   c += upto - sum;
   int got = INT32_MAX, last = -1;
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) {
+  for (int j = 0; j < kDrawValues; ++j) {
     c += w[j];
     if (w[j] > 0.0) {
       last = i0 + j;
       if (got == INT32_MAX && c > want) got = i0 + j;
     }
   }
-  if (got != INT32_MAX) atomicMin(&at, got);
-  if (last >= 0) atomicMax(&most, last);
+  got = wave_min_i32(got);
+  last = -wave_min_i32(-last);
+  if (lane == 0) {
+    at[wave] = got;
+    most[wave] = last;
+  }
   __syncthreads();
-  if (tid == 0) a.next[b] = at != INT32_MAX ? at : most;
+  if (tid == 0) {
+    for (int i = 1; i < kWavesV; ++i) {
+      got = min(got, at[i]);
+      last = max(last, most[i]);
+    }
+    a.next[b] = got != INT32_MAX ? got : last;
+  }
 }
 
 template <typename T>
@@ -429,14 +490,19 @@ static hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
   if (a.q.n_tokens > 0) {
     const hipError_t e = launch(k_verify_rows<T>, wide_grid((int64_t)a.q.n_tokens * a.segments,
                                                             rows_of_draft ? 2 : 1),
-                                dim3(kVerifyThreads), 0, s, a);
+                                dim3(kRowsThreads), 0, s, a);
     if (e != hipSuccess) return e;
   }
   const int blocks = greedy ? 1 : a.segments;
-  const hipError_t e = launch(k_verify_stop<T>, wide_grid((int64_t)a.q.n_seqs * blocks, 1),
-                              dim3(kVerifyThreads), 0, s, a, blocks);
+  // Blocks that all run at once end sooner with more waves (one sequence of five
+  // rows of 50257: 6.9 us with 1024 threads, 8.4 with 256); of more blocks each
+  // wave repeats the decision (64 sequences: 22 and 12 us).
+  const int64_t all = (int64_t)a.q.n_seqs * blocks;
+  const dim3 grid = wide_grid(all, 1);
+  const hipError_t e = all <= 256 ? launch(k_verify_stop<T, 1024>, grid, dim3(1024), 0, s, a, blocks)
+                                  : launch(k_verify_stop<T, 256>, grid, dim3(256), 0, s, a, blocks);
   if (e != hipSuccess || greedy) return e;
-  return launch(k_verify_draw<T>, dim3(a.q.n_seqs), dim3(kVerifyThreads), 0, s, a);
+  return launch(k_verify_draw<T>, dim3(a.q.n_seqs), dim3(kDrawThreads), 0, s, a);
 }
 
 struct VerifySpace {
