@@ -284,10 +284,10 @@ constexpr int kShort = 32;   // sequences of up to these rows go row by row
 template <typename T>
 constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;  // of a value of K or Q
 constexpr int kTri = 6 * 2 * 1024;  // bytes of T or A: blocks of 16 rows and 32 columns on and below the diagonal
-// per place and head after T and A, 64 floats each: b; e^c of k; e^{c_C - c} of k; e^c of q; the
-// scales of A and T; then the decay (two parts), the first bad row, the largest of the third
-enum { kBeta, kGrowK, kLeft, kGrowQ, kFacA, kFacT, kMisc };
-constexpr int kScalars = 7 * 256;
+// per place and head after T and A, 64 floats each: e^c of k; e^{c_C - c} of k; e^c of q; the
+// scales of A and T; then the decay (two parts), the first bad row, the largest of the second
+enum { kGrowK, kLeft, kGrowQ, kFacA, kFacT, kMisc };
+constexpr int kScalars = 6 * 256;
 
 struct DeltaPlan {
   bool chunks;     // a sequence may have more than kShort rows
@@ -531,6 +531,7 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
   __shared__ __attribute__((aligned(16))) uint8_t shK[kShared];  // K; then T
   __shared__ __attribute__((aligned(16))) float shL[kC * kRowL];
   __shared__ __attribute__((aligned(16))) float shHi[kC], shLo[kC], shRk[kC];
+  __shared__ __attribute__((aligned(16))) float shB[kC];
   __shared__ float shKk[kC], shKd[kC], shQf[kC];
   float* shT = (float*)shK;
   Unit u = find_unit(a.q, (int)wide_block(), kC);
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
   float* scalars = (float*)(out + 2 * kTri);
   if (wave == 0) {
     const float left = __builtin_amdgcn_exp2f((float)(whole - cum)) * rk;
-    scalars[kBeta * 64 + lane] = b;
+    shB[lane] = b;
     scalars[kGrowK * 64 + lane] = grow * rk;
     scalars[kLeft * 64 + lane] = left;
     scalars[kGrowQ * 64 + lane] = grow * rq;
@@ -760,13 +761,16 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
   for (int sp = 0; sp < 2; ++sp) {
     if (2 * sp < tiles) {
       const int j0 = 32 * sp + 8 * q;
-      const float4 x = *(const float4*)(shT + mine * kRowL + j0),
-                   y = *(const float4*)(shT + mine * kRowL + j0 + 4);
-      const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v8[sp][e] = j0 + e < mine ? w[e] : 0.0f;  // without the ones
-        mt = max_abs(mt, v8[sp][e]);
+      for (int k = 0; k < 2; ++k) {
+        const float4 x = *(const float4*)(shT + mine * kRowL + j0 + 4 * k),
+                     y = *(const float4*)(shB + j0 + 4 * k);
+        const float t4[4] = {x.x, x.y, x.z, x.w}, b4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v8[sp][4 * k + e] = j0 + 4 * k + e <= mine ? t4[e] * b4[e] : 0.0f;
+          mt = max_abs(mt, v8[sp][4 * k + e]);
+        }
       }
     }
   }
@@ -780,19 +784,36 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 // the state and the w that the first leaves in LDS.  Nothing is exchanged
 // between lanes: results serve as operands (spread_row).
 //
-// The state S and w are held times a power of two per column, `unit`, which
-// keeps the largest of S, w and b (v - e^c K S) between kLow and kTop, where two
-// halves are good to 2^-22 of it.  It changes only when one leaves that range.
+// The state S and w are held times a power of two per column, `unit`, so that the
+// largest of S and w is at least kLow and S and w pass neither kTopS nor kTop:
+// there two halves are good to 2^-22 of it.  w is looked at in every chunk; of S
+// a bound is carried on, and its values looked at when that passes kTopS.  What
+// leaves the range, or fp32, goes another way, which works the chunk out anew.
 // ---------------------------------------------------------------------------
-constexpr float kTop = 32768.0f, kLow = 1.0f;
+constexpr float kTop = 32768.0f, kTopS = 4096.0f, kLow = 0.125f;
+constexpr int kAim = 127 + 1;  // exponent bits of what a new unit makes the largest
 
 __device__ __forceinline__ int exponent_bits(float v) { return (int)(__float_as_uint(v) >> 23 & 255); }
 // The power of two, of up to 2^-126 and 2^100, that takes a magnitude with the
-// exponent bits e to about 2^8, as far as `unit` times it stays in that range.
+// exponent bits e to kAim's, as far as `unit` times it stays in that range.
 __device__ __forceinline__ float to_range(int e, float unit) {
   const int ue = exponent_bits(unit);
-  const int d = min(max(8 + 127 - e, max(1 - ue, -126)), min(227 - ue, 100));
+  const int d = min(max(kAim - e, max(1 - ue, -126)), min(227 - ue, 100));
   return __uint_as_float((uint32_t)(127 + d) << 23);
+}
+__device__ __forceinline__ v4f mfma_one(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// c[.] += a[.] (sum of b), one product of halves after another, so that
+// neighbours do not wait for each other
+template <int M, int NA>
+__device__ __forceinline__ void mfma_many(v4f (&c)[M], const v8h (&a)[M][NA], const v8h (&b)[2]) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < 2 - i; ++j)
+#pragma unroll
+      for (int m = 0; m < M; ++m) c[m] = mfma_one(a[m][i], b[j], c[m]);
 }
 
 template <int NK>
@@ -862,12 +883,19 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
   // block (w, x) of T or A times rows 32 x .. of v, for all four row tiles
   auto times_triangle = [&](const v8h (&f)[6][2], const v8h (&v)[2][2], v4f (&o)[4]) {
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    o[0] = mfma_h(f[0], v[0], zero);
-    o[1] = mfma_h(f[1], v[0], zero);
-    o[2] = mfma_h(f[2], v[0], zero);
-    o[3] = mfma_h(f[4], v[0], zero);
-    o[2] = mfma_h(f[3], v[1], o[2]);
-    o[3] = mfma_h(f[5], v[1], o[3]);
+    // one product of halves after another, so that neighbours do not wait
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o[w] = mfma_one(f[w < 2 ? w : 2 * w - 2][0], v[0][0], zero);
+#pragma unroll
+    for (int w = 2; w < 4; ++w) o[w] = mfma_one(f[2 * w - 1][0], v[1][0], o[w]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o[w] = mfma_one(f[w < 2 ? w : 2 * w - 2][0], v[0][1], o[w]);
+#pragma unroll
+    for (int w = 2; w < 4; ++w) o[w] = mfma_one(f[2 * w - 1][0], v[1][1], o[w]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o[w] = mfma_one(f[w < 2 ? w : 2 * w - 2][1], v[0][0], o[w]);
+#pragma unroll
+    for (int w = 2; w < 4; ++w) o[w] = mfma_one(f[2 * w - 1][1], v[1][0], o[w]);
   };
   // 16 values of v or z in the lane's column
   auto values = [&](const void* at, int64_t stride, int c, uint32_t (&v)[4][4]) {
@@ -901,13 +929,11 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         S[t][i] = keep ? load_row<float, 1>(bst, state_off(8 * q, t, i)).v[0] : 0.0f;
-    // Operands are loaded a step of the chunk or two before their products:
-    // K in the shadow of the chunk before, T of K S, K by columns of T R.
-    v8h kf[NK][4][KP], kt[NT][2][KP], tf[6][2];
+    // operands of the next chunk are loaded when those of this one are done with
+    v8h kf[NK][4][KP], kt[2][NT][KP], tf[6][2];
     uint32_t vr[4][4];
-    v4f beta[4], grow[4], left[4], fac[4];
-    auto fetch_k = [&](int c) {
-      const auto k = keys_of(c);
+    v4f grow[4], left[4], fac[4];
+    auto fetch_k = [&](__amdgpu_buffer_rsrc_t k) {
 #pragma unroll
       for (int x = 0; x < NK; ++x)
 #pragma unroll
@@ -915,46 +941,53 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
 #pragma unroll
           for (int i = 0; i < KP; ++i) kf[x][w][i] = operand(k, ((w * NK + x) * KP + i) * 1024);
     };
-    float unit = 1.0f;
-    auto rescale = [&](float f) {
-      unit *= f;
+    auto fetch_kt = [&](__amdgpu_buffer_rsrc_t k) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) S[t] *= f;
-    };
-    auto fetch_kt = [&](int c) {
-        const auto k = keys_of(c);
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int i = 0; i < KP; ++i)
-              kt[t][x][i] = operand(k, (8 * NK * KP + (t * 2 + x) * KP + i) * 1024);
+          for (int i = 0; i < KP; ++i)
+            kt[x][t][i] = operand(k, (8 * NK * KP + (t * 2 + x) * KP + i) * 1024);
     };
-    fetch_k(0);
-    triangle(head_of(0), 0, tf);
-    scalars(head_of(0), kFacT, fac);
-    fetch_kt(0);
-    values(a.v, a.vs, 0, vr);
-    scalars(head_of(0), kBeta, beta);
-    scalars(head_of(0), kGrowK, grow);
+    float unit = 1.0f, bound = 0.0f, lost = 0.0f;
+    auto rescale = [&](float f) {
+      unit *= f;
+      bound *= f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) S[t] *= f;
+    };
+    auto largest = [&]() {  // of the state's column
+      float m = 0.0f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max_abs(m, S[t][i]);
+      return quads_max(m);
+    };
+    {
+      const auto k = keys_of(0);
+      const auto o = head_of(0);
+      fetch_k(k);
+      values(a.v, a.vs, 0, vr);
+      scalars(o, kGrowK, grow);
+      triangle(o, 0, tf);
+      scalars(o, kFacT, fac);
+      fetch_kt(k);
+      scalars(o, kLeft, left);
+    }
+    bound = __builtin_inff();
     for (int c = 0; c < chunks; ++c) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      const auto head = head_of(c);
+      const auto head1 = head_of(next), keys1 = keys_of(next);
       const float* misc = (const float*)(heads0 + c * head_step + 2 * kTri) + kMisc * 64;
       const float dec_hi = misc[0], dec_lo = misc[1], most = fmaxf(misc[3], 1.0f);
       const int first = ((const int*)misc)[2];
       uint8_t* buf = sh[c & 1];
-      float ms = 0.0f;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ms = max_abs(ms, S[t][i]);
-      ms = quads_max(ms);
-      if (__ballot(!(ms <= kTop))) {
-        const float f = ms > kTop && ms < __builtin_inff() ? to_range(exponent_bits(ms), unit) : 1.0f;
+      if (__ballot(!(bound <= kTopS))) {
+        bound = largest();
+        const float f = bound > kTopS && bound < __builtin_inff() ? to_range(exponent_bits(bound), unit) : 1.0f;
         rescale(f);
-        ms *= f;
       }
       // K S, and S for the other wave
       v4f X[4];
@@ -967,52 +1000,61 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
           halves8<2>(sf, S[2 * x], S[2 * x + 1]);
           *(v8h*)(buf + x * 2048 + lane * 16) = sf[0];
           *(v8h*)(buf + x * 2048 + 1024 + lane * 16) = sf[1];
-          keys(x, [&](int w, const v8h (&k)[KP]) { X[w] = mfma_h(k, sf, X[w]); });
+          keys(x, sf);
         }
         if (q == 0) ((float*)(buf + L::kS + L::kW))[r] = __builtin_amdgcn_rcpf(unit);
       };
-      product([&](int x, auto f) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) f(w, kf[x][w]);
-      });
+      product([&](int x, const v8h (&sf)[2]) { mfma_many(X, kf[x], sf); });
       __builtin_amdgcn_sched_barrier(0);
-      fetch_k(next);
-      // R = b (v - e^c K S)
-      v4f R[4];
+      fetch_k(keys1);
+      // R = v - e^c K S, w = T b R
+      v4f R[4], W[4];
       auto residue = [&]() {
-        float m = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            R[w][i] = beta[w][i] * __builtin_fmaf(-grow[w][i], X[w][i], raw_f32<T>(vr[w][i]) * unit);
-            m = max_abs(m, R[w][i]);
-          }
-        return quads_max(m);
+          for (int i = 0; i < 4; ++i)
+            R[w][i] = __builtin_fmaf(-grow[w][i], X[w][i], raw_f32<T>(vr[w][i]) * unit);
       };
-      // infinities and NaN leave the products; `at` is the first row of one
-      int at = kC;
-      auto tame = [&](v4f (&v)[4]) {
+      auto solve = [&]() {
+        v8h rf[2][2];
+        halves8<2>(rf[0], R[0], R[1]);
+        halves8<2>(rf[1], R[2], R[3]);
+        times_triangle(tf, rf, W);
         float m = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 4; ++w) {
+          W[w] *= fac[w];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!(__builtin_fabsf(v[w][i]) < __builtin_inff())) {
-              at = min(at, spread_row(w, 4 * q + i));
-              v[w][i] = 0.0f;
-            }
-            m = max_abs(m, v[w][i]);
-          }
+          for (int i = 0; i < 4; ++i) m = max_abs(m, W[w][i]);
+        }
         return quads_max(m);
       };
-      const float mr = residue(), mm = __builtin_elementwise_maximum(mr, ms);
-      if (__ballot(!(mr <= kTop) || (mm < kLow && mm > 0.0f && unit < 0x1p100f))) {
-        // The unit by the largest finite value, in bits of an exponent; what was
-        // computed in the old one may have passed fp32 or been too small for
-        // halves, S among it, and is worked out anew.
-        int bits = exponent_bits(mm);
-        if (!(mr < __builtin_inff())) {
+      residue();
+      float mw = solve();
+      int from = first;  // the column's rows from here on are NaN
+      if (__ballot(!(mw * most <= kTop) || (mw < kLow && mw > 0.0f && unit < 0x1p100f))) {
+        const float ms = largest();
+        const bool over = !(mw * most <= kTop), under = mw < kLow && ms < kLow && unit < 0x1p100f;
+        if (__ballot(over || under)) {
+          // infinities and NaN leave the products; `at` is the first row of one
+          int at = kC;
+          auto tame = [&](v4f (&v)[4]) {
+            float m = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (!(__builtin_fabsf(v[w][i]) < __builtin_inff())) {
+                  at = min(at, spread_row(w, 4 * q + i));
+                  v[w][i] = 0.0f;
+                }
+                m = max_abs(m, v[w][i]);
+              }
+            return quads_max(m);
+          };
+          // A unit by the largest finite of v and the state, in bits of an
+          // exponent; then all of it anew.
           float mv = 0.0f;
 #pragma unroll
           for (int w = 0; w < 4; ++w)
@@ -1022,101 +1064,72 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
               mv = v < __builtin_inff() ? fmaxf(mv, v) : mv;
             }
           mv = quads_max(mv);
-          bits = max(exponent_bits(mv) + exponent_bits(unit) - 127,
-                     ms < __builtin_inff() ? exponent_bits(ms) : 0);
-          if (mv == 0.0f && !(ms > 0.0f)) bits = 8 + 127;
-        }
-        const bool off = !(mr <= kTop) || (mm < kLow && mm > 0.0f);
+          int bits = max(mv > 0.0f ? exponent_bits(mv) + exponent_bits(unit) - 127 : 0,
+                         ms > 0.0f && ms < __builtin_inff() ? exponent_bits(ms) : 0);
+          const bool off = (over || under) && bits > 0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {  // one power of two may not reach
-          const float f = off ? to_range(bits, unit) : 1.0f;
-          rescale(f);
-          bits += exponent_bits(f) - 127;
-        }
-        const auto k = keys_of(c);
-        product([&](int x, auto fn) {
-          for (int w = 0; w < 4; ++w) {
-            v8h kw[KP];
+          for (int k = 0; k < 2; ++k) {  // one power of two may not reach
+            const float f = off ? to_range(bits, unit) : 1.0f;
+            rescale(f);
+            bits += exponent_bits(f) - 127;
+          }
+          bound = ms;
+          const auto k = keys_of(c);
+          product([&](int x, const v8h (&sf)[2]) {
 #pragma unroll
-            for (int i = 0; i < KP; ++i) kw[i] = operand(k, ((w * NK + x) * KP + i) * 1024);
-            switch (w) {  // registers have no index
-              case 0: fn(0, kw); break;
-              case 1: fn(1, kw); break;
-              case 2: fn(2, kw); break;
-              default: fn(3, kw); break;
+            for (int w = 0; w < 4; ++w) {
+              v8h kw[KP];
+#pragma unroll
+              for (int i = 0; i < KP; ++i) kw[i] = operand(k, ((w * NK + x) * KP + i) * 1024);
+              X[w] = mfma_h(kw, sf, X[w]);
             }
-          }
-        });
-        (void)residue();
-        const float m = tame(R), f = m > kTop ? to_range(exponent_bits(m), unit) : 1.0f;
-        rescale(f);
+          });
+          residue();
+          float m = tame(R), f = m > kTop ? to_range(exponent_bits(m), unit) : 1.0f;
+          rescale(f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) R[w] *= f;
+          for (int w = 0; w < 4; ++w) R[w] *= f;
+          (void)solve();
+          mw = tame(W);
+          f = mw * most > kTop ? to_range(exponent_bits(mw) + exponent_bits(most) - 127, unit) : 1.0f;
+          rescale(f);
+          mw *= f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) W[w] *= f;
+          bound = largest();
+          at = min(at, __shfl_xor(at, 16));
+          from = min(from, min(at, __shfl_xor(at, 32)));
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
-      scalars(head, kLeft, left);
       values(a.v, a.vs, next, vr);
-      scalars(head_of(next), kBeta, beta);
-      scalars(head_of(next), kGrowK, grow);
-      // w = T R, T without its ones
-      v4f W[4];
-      auto solve = [&]() {
-        v8h rf[2][2];
-        halves8<2>(rf[0], R[0], R[1]);
-        halves8<2>(rf[1], R[2], R[3]);
-        times_triangle(tf, rf, W);
-        float m = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            W[w][i] = __builtin_fmaf(fac[w][i], W[w][i], R[w][i]);
-            m = max_abs(m, W[w][i]);
-          }
-        return quads_max(m);
-      };
-      float mw = solve();
-      if (__ballot(!(mw * most <= kTop))) {
-        if (__ballot(!(mw < __builtin_inff()))) mw = tame(W);
-        const float f = mw * most > kTop
-                            ? to_range(exponent_bits(mw) + exponent_bits(most) - 127, unit)
-                            : 1.0f;
-        rescale(f);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) W[w] *= f;
-      }
-      int from = first;  // the column's rows from here on are NaN
-      if (__ballot(at < kC)) {
-        at = min(at, __shfl_xor(at, 16));
-        from = min(from, min(at, __shfl_xor(at, 32)));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      triangle(head_of(next), 0, tf);
-      scalars(head_of(next), kFacT, fac);
+      scalars(head1, kGrowK, grow);
+      triangle(head1, 0, tf);
+      scalars(head1, kFacT, fac);
       // w for the other wave, and times e^{c_C - c} for the state
       v8h lf[2][2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        v8h wf[2];
-        halves8<2>(wf, W[2 * x], W[2 * x + 1]);
-        *(v8h*)(buf + L::kS + x * 2048 + lane * 16) = wf[0];
-        *(v8h*)(buf + L::kS + x * 2048 + 1024 + lane * 16) = wf[1];
+      for (int w = 0; w < 4; ++w) *(v4f*)(buf + L::kS + w * 1024 + lane * 16) = W[w];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
         halves8<2>(lf[x], W[2 * x] * left[2 * x], W[2 * x + 1] * left[2 * x + 1]);
-      }
       if (q == 0) {
         ((float*)(buf + L::kS + L::kW))[16 + r] = __builtin_amdgcn_rcpf(unit);
         ((int*)(buf + L::kS + L::kW))[32 + r] = from;
       }
-      const float keep_hi = from < kC ? __builtin_nanf("") : dec_hi;
+      // The decay as one float: what its rounding loses goes into the next one,
+      // so that the product over all chunks is good to 2^-24.
+      const float low = __builtin_fmaf(dec_hi, lost, dec_lo), decay = dec_hi + low;
+      lost = decay > 0.0f ? ((dec_hi - decay) + low) * __builtin_amdgcn_rcpf(decay) : 0.0f;
+      bound = __builtin_fmaf(bound, decay, 128.0f * mw * most);  // |K| < 2, 64 rows
+      const float by = from < kC ? __builtin_nanf("") : decay;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int t = 0; t < NT; ++t) S[t] *= by;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S[t][i] = __builtin_fmaf(S[t][i], keep_hi, S[t][i] * dec_lo);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) S[t] = mfma_h(kt[t][x], lf[x], S[t]);
-      }
+      for (int x = 0; x < 2; ++x) mfma_many(S, kt[x], lf[x]);
       __builtin_amdgcn_sched_barrier(0);
-      fetch_kt(next);
+      fetch_kt(keys1);
+      scalars(head1, kLeft, left);
       lds_sync();
     }
     if (a.frozen) return;
@@ -1159,16 +1172,14 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       for (int x = 0; x < NK; ++x) {
         const v8h sf[2] = {*(const v8h*)(buf + x * 2048 + lane * 16),
                            *(const v8h*)(buf + x * 2048 + 1024 + lane * 16)};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) X[w] = mfma_h(qf[x][w], sf, X[w]);
+        mfma_many(X, qf[x], sf);
       }
       fetch_q(next);
       v8h wf[2][2];
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          wf[x][i] = *(const v8h*)(buf + L::kS + x * 2048 + i * 1024 + lane * 16);
+        halves8<2>(wf[x], *(const v4f*)(buf + L::kS + 2 * x * 1024 + lane * 16),
+                   *(const v4f*)(buf + L::kS + (2 * x + 1) * 1024 + lane * 16));
       times_triangle(af, wf, Y);
       const float* cols = (const float*)(buf + L::kS + L::kW);
       const float us = cols[r], uw = cols[16 + r];
