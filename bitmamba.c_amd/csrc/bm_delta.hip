@@ -44,13 +44,18 @@ __device__ __forceinline__ float unit_of(const DeltaArgs& a, float squares) {
   return squares < __builtin_inff() ? unit : __builtin_nanf("");
 }
 
+// a permutation of all lanes of a row, in the form that an addition takes in
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 // sum over teams of T neighbouring lanes, in every lane of the team
 template <int T>
 __device__ __forceinline__ float team_add(float v) {
-  if (T > 1) v += __int_as_float(dpp_mov<0xB1>(__float_as_int(v)));
-  if (T > 2) v += __int_as_float(dpp_mov<0x4E>(__float_as_int(v)));
-  if (T > 4) v += __int_as_float(dpp_mov<0x141>(__float_as_int(v)));
-  if (T > 8) v += __int_as_float(dpp_mov<0x140>(__float_as_int(v)));
+  if (T > 1) v += dpp_f32<0xB1>(v);
+  if (T > 2) v += dpp_f32<0x4E>(v);
+  if (T > 4) v += dpp_f32<0x141>(v);
+  if (T > 8) v += dpp_f32<0x140>(v);
 #pragma unroll
   for (int m = 16; m < T; m <<= 1) v += __shfl_xor(v, m);
   return v;
@@ -91,38 +96,30 @@ __device__ __forceinline__ float value_of(const RawRow<T, V>& r, int i) {
 }
 
 // ---------------------------------------------------------------------------
-// Row after row.  A team of TEAM lanes holds one row of the state, V
+// One row per sequence.  A team of TEAM lanes holds one row of the state, V
 // neighbouring values per lane and step of E; a wave takes 64 / TEAM rows at
 // once and U such groups.  S k and S q are both taken from the state before
-// the row, so that a row of the sequence reads it once:
+// the row, so that it is read once:
 //   S' q = a (S q) + w (k . q).
 // ---------------------------------------------------------------------------
-template <typename T, int TEAM, int V, int E, int U, bool STREAM, bool STEP>
-__global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a, int most) {
+template <typename T, int TEAM, int V, int E, int U, bool STREAM>
+__global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
   constexpr int kRows = 64 / TEAM;
   const int b = blockIdx.x, h = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int p0 = (blockIdx.z * (blockDim.x >> 6) + wave) * (kRows * U) + lane / TEAM;
   const int nl = (lane % TEAM) * V;
-  const int slots = first_slots(a.q);
-  int t0 = b, t1 = b + 1;
-  if (!STEP) {
-    t0 = a.q.seq_start ? seq_row(a.q, b) : 0;
-    t1 = a.q.seq_start ? seq_row(a.q, b + 1) : a.q.n_tokens;
-    if (t1 - t0 > most) return;
-  }
-  const int slot = find_slot(a.q, b, slots);
+  const int slot = find_slot(a.q, b, first_slots(a.q));
   if (slot == kNoSlot) return;
-  const bool keep = slot >= 0 && !(!STEP && a.q.fresh && a.q.fresh[b]);
-  if (!STEP && t1 <= t0 && (keep || slot < 0)) return;  // no rows, and nothing to start from zeros
+  const bool keep = slot >= 0;
   const int g = h / (a.heads / a.groups);
   const float A = a.A ? a.A[h] : 0.0f, bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
   // the head's part of the slot and of rows; what lies past them reads as
   // zeros and is not written
-  const auto st = rows_at(a.state + (slot >= 0 ? (int64_t)slot * a.ss : 0) + (int64_t)h * a.hd * a.n,
-                          slot >= 0 ? (uint32_t)(a.hd * a.n * 4) : 0);
+  const auto st = rows_at(a.state + (keep ? (int64_t)slot * a.ss : 0) + (int64_t)h * a.hd * a.n,
+                          keep ? (uint32_t)(a.hd * a.n * 4) : 0);
   const uint32_t head = (uint32_t)(a.hd * sizeof(T)), gn = (uint32_t)(a.n * sizeof(T));
-  const int64_t col = (int64_t)h * a.hd, gcol = (int64_t)g * a.n;
+  const int64_t t = b, col = (int64_t)h * a.hd, gcol = (int64_t)g * a.n;
 
   float s[U][E][V];
 #pragma unroll
@@ -134,81 +131,70 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a, int most) {
       load_floats<V, STREAM>(s[u][e], st,
                              keep && n < a.n ? (uint32_t)((p * a.n + n) * 4) : kNoColumn);
     }
-
   RawRow<T, V> kr[E], qr[E];
-  uint32_t vr[U], zr[U], dtr = 0, br = 0;
-  auto fetch = [&](int64_t t) {
-    const auto bk = rows_at((const T*)a.K + t * a.Ks + gcol, gn);
-    const auto bq = rows_at((const T*)a.Q + t * a.Qs + gcol, gn);
-    const auto bv = rows_at((const T*)a.v + t * a.vs + col, head);
-    const auto bz = rows_at((const T*)a.z + t * a.zs + col, a.z ? head : 0);
-    const uint32_t one = sizeof(T);
-    dtr = load_raw<T>(rows_at((const T*)a.dt + t * a.dts + h, a.A ? one : 0), 0);
-    br = load_raw<T>(rows_at((const T*)a.beta + t * a.bs + h, a.beta ? one : 0), 0);
+  uint32_t vr[U], zr[U];
+  const auto bk = rows_at((const T*)a.K + t * a.Ks + gcol, gn);
+  const auto bq = rows_at((const T*)a.Q + t * a.Qs + gcol, gn);
+  const auto bv = rows_at((const T*)a.v + t * a.vs + col, head);
+  const auto bz = rows_at((const T*)a.z + t * a.zs + col, a.z ? head : 0);
+  const auto by = rows_at((const T*)a.y + t * a.ys + col, head);
+  const uint32_t one = sizeof(T);
+  const uint32_t dtr = load_raw<T>(rows_at((const T*)a.dt + t * a.dts + h, a.A ? one : 0), 0);
+  const uint32_t br = load_raw<T>(rows_at((const T*)a.beta + t * a.bs + h, a.beta ? one : 0), 0);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int n = nl + e * TEAM * V;
-      kr[e] = load_values<T, V>(bk, (uint32_t)(n * sizeof(T)), n, a.n, a.wide);
-      qr[e] = load_values<T, V>(bq, (uint32_t)(n * sizeof(T)), n, a.n, a.wide);
-    }
+  for (int e = 0; e < E; ++e) {
+    const int n = nl + e * TEAM * V;
+    kr[e] = load_values<T, V>(bk, (uint32_t)(n * sizeof(T)), n, a.n, a.wide);
+    qr[e] = load_values<T, V>(bq, (uint32_t)(n * sizeof(T)), n, a.n, a.wide);
+  }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      vr[u] = load_raw<T>(bv, (uint32_t)((p0 + u * kRows) * sizeof(T)));
-      zr[u] = load_raw<T>(bz, (uint32_t)((p0 + u * kRows) * sizeof(T)));
+  for (int u = 0; u < U; ++u) {
+    vr[u] = load_raw<T>(bv, (uint32_t)((p0 + u * kRows) * sizeof(T)));
+    zr[u] = load_raw<T>(bz, (uint32_t)((p0 + u * kRows) * sizeof(T)));
+  }
+
+  float k[E][V], q[E][V], kk = 0.0f, qq = 0.0f, qk = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      k[e][i] = value_of<T, V>(kr[e], i);
+      q[e][i] = value_of<T, V>(qr[e], i);
+      kk = __builtin_fmaf(k[e][i], k[e][i], kk);
+      qq = __builtin_fmaf(q[e][i], q[e][i], qq);
+      qk = __builtin_fmaf(q[e][i], k[e][i], qk);
     }
-  };
-  if (t0 < t1) fetch(t0);
-  for (int64_t t = t0; t < t1; ++t) {
-    float k[E][V], q[E][V], v[U], z[U], kk = 0.0f, qq = 0.0f, qk = 0.0f;
+  const float beta = beta_of(a, raw_f32<T>(br));
+  const Decay decay = decay_of(exponent_of(a, A, raw_f32<T>(dtr), bias));
+  const float uk = unit_of(a, team_add<TEAM>(kk));
+  const float uq = a.scale * unit_of(a, team_add<TEAM>(qq));
+  qk = team_add<TEAM>(qk) * uk * uq;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float sk = 0.0f, sq = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        k[e][i] = value_of<T, V>(kr[e], i);
-        q[e][i] = value_of<T, V>(qr[e], i);
-        kk = __builtin_fmaf(k[e][i], k[e][i], kk);
-        qq = __builtin_fmaf(q[e][i], q[e][i], qq);
-        qk = __builtin_fmaf(q[e][i], k[e][i], qk);
+        sk = __builtin_fmaf(s[u][e][i], k[e][i], sk);
+        sq = __builtin_fmaf(s[u][e][i], q[e][i], sq);
       }
+    sk = team_add<TEAM>(sk) * uk;
+    sq = team_add<TEAM>(sq) * uq;
+    const float w = beta * (raw_f32<T>(vr[u]) - __builtin_fmaf(sk, decay.lo, sk * decay.hi));
+    const float wk = w * uk;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u] = raw_f32<T>(vr[u]);
-      z[u] = raw_f32<T>(zr[u]);
-    }
-    const float beta = beta_of(a, raw_f32<T>(br));
-    const Decay decay = decay_of(exponent_of(a, A, raw_f32<T>(dtr), bias));
-    if (!STEP && t + 1 < t1) fetch(t + 1);
-    const float uk = unit_of(a, team_add<TEAM>(kk));
-    const float uq = a.scale * unit_of(a, team_add<TEAM>(qq));
-    qk = team_add<TEAM>(qk) * uk * uq;
-    const auto by = rows_at((const T*)a.y + t * a.ys + col, head);
+    for (int e = 0; e < E; ++e)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float sk = 0.0f, sq = 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          sk = __builtin_fmaf(s[u][e][i], k[e][i], sk);
-          sq = __builtin_fmaf(s[u][e][i], q[e][i], sq);
-        }
-      sk = team_add<TEAM>(sk) * uk;
-      sq = team_add<TEAM>(sq) * uq;
-      const float w = beta * (v[u] - __builtin_fmaf(sk, decay.lo, sk * decay.hi));
-      const float wk = w * uk;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          s[u][e][i] = __builtin_fmaf(s[u][e][i], decay.hi,
-                                      __builtin_fmaf(s[u][e][i], decay.lo, wk * k[e][i]));
-      float y = __builtin_fmaf(sq, decay.lo, sq * decay.hi);
-      y = __builtin_fmaf(w, qk, y);
-      if (a.z) y *= silu_f32(z[u]);
-      const float out[1] = {y};
-      store_row<T, 1>(by, lane % TEAM == 0 ? (uint32_t)((p0 + u * kRows) * sizeof(T)) : kNoColumn,
-                      out);
-    }
+      for (int i = 0; i < V; ++i)
+        s[u][e][i] = __builtin_fmaf(s[u][e][i], decay.hi,
+                                    __builtin_fmaf(s[u][e][i], decay.lo, wk * k[e][i]));
+    float y = __builtin_fmaf(sq, decay.lo, sq * decay.hi);
+    y = __builtin_fmaf(w, qk, y);
+    if (a.z) y *= silu_f32(raw_f32<T>(zr[u]));
+    const float out[1] = {y};
+    store_row<T, 1>(by, lane % TEAM == 0 ? (uint32_t)((p0 + u * kRows) * sizeof(T)) : kNoColumn,
+                    out);
   }
   if (a.frozen) return;
 #pragma unroll
@@ -221,33 +207,285 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a, int most) {
     }
 }
 
-template <typename T, int TEAM, int V, int E, bool STEP>
-static hipError_t launch_rows(const DeltaArgs& a, int most, hipStream_t s) {
-  constexpr int U = E >= 4 ? 2 : (E == 2 ? 4 : (TEAM >= 16 ? (STEP ? 8 : 4) : 2));
+template <typename T, int TEAM, int V, int E>
+static hipError_t launch_step(const DeltaArgs& a, hipStream_t s) {
+  constexpr int U = E >= 4 ? 2 : (E == 2 ? 4 : (TEAM >= 16 ? 8 : 2));
   constexpr int kRows = 64 / TEAM * U;  // rows of the state per wave
   const int waves = (a.hd + kRows - 1) / kRows;
   const int nw = waves < 4 ? waves : 4;
   const dim3 grid(a.q.n_seqs, a.heads, (waves + nw - 1) / nw);
   // as the scan's single tokens: states of 64 MiB or more go past the caches
-  constexpr bool kLarge = STEP && V == 4 && TEAM >= 4;
+  constexpr bool kLarge = V == 4;
   if (kLarge && (int64_t)a.q.n_seqs * a.heads * a.hd * a.n >= (1 << 24))
-    return launch(k_delta_rows<T, TEAM, V, E, U, kLarge, STEP>, grid, dim3(64 * nw), 0, s, a, most);
-  return launch(k_delta_rows<T, TEAM, V, E, U, false, STEP>, grid, dim3(64 * nw), 0, s, a, most);
+    return launch(k_delta_step<T, TEAM, V, E, U, kLarge>, grid, dim3(64 * nw), 0, s, a);
+  return launch(k_delta_step<T, TEAM, V, E, U, false>, grid, dim3(64 * nw), 0, s, a);
 }
 
-template <typename T, bool STEP>
-static hipError_t launch_rows_t(const DeltaArgs& a, int most, hipStream_t s) {
+template <typename T>
+static hipError_t launch_step_t(const DeltaArgs& a, hipStream_t s) {
   if (a.n % 4 == 0) {  // a state row's loads of four floats need no more than a float's alignment
-    if (a.n <= 16) return launch_rows<T, 4, 4, 1, STEP>(a, most, s);
-    if (a.n <= 32) return launch_rows<T, 8, 4, 1, STEP>(a, most, s);
-    if (a.n <= 64) return launch_rows<T, 16, 4, 1, STEP>(a, most, s);
-    if (a.n <= 128) return launch_rows<T, 16, 4, 2, STEP>(a, most, s);
-    return launch_rows<T, 16, 4, 4, STEP>(a, most, s);
+    if (a.n <= 16) return launch_step<T, 4, 4, 1>(a, s);
+    if (a.n <= 32) return launch_step<T, 8, 4, 1>(a, s);
+    if (a.n <= 64) return launch_step<T, 16, 4, 1>(a, s);
+    if (a.n <= 128) return launch_step<T, 16, 4, 2>(a, s);
+    return launch_step<T, 16, 4, 4>(a, s);
   }
-  if (a.n <= 4) return launch_rows<T, 4, 1, 1, STEP>(a, most, s);
-  if (a.n <= 16) return launch_rows<T, 16, 1, 1, STEP>(a, most, s);
-  if (a.n <= 64) return launch_rows<T, 16, 1, 4, STEP>(a, most, s);
-  return launch_rows<T, 64, 1, 4, STEP>(a, most, s);
+  if (a.n <= 4) return launch_step<T, 4, 1, 1>(a, s);
+  if (a.n <= 16) return launch_step<T, 16, 1, 1>(a, s);
+  if (a.n <= 64) return launch_step<T, 16, 1, 4>(a, s);
+  return launch_step<T, 64, 1, 4>(a, s);
+}
+
+// ---------------------------------------------------------------------------
+// A few rows per sequence: kFew at a time.  What the state of before them gives
+// each row's key and query, X = [K Q]^T S, is one product on the matrix cores, in
+// fp32 as the state is; with G = [K Q]^T [K Q] the rest needs no more than kFew
+// numbers per row of the state.  With P_j the product of the decays up to row j
+// and wu_i = (what row i wrote) / |k_i|, decayed up to j, row j writes and reads
+//   w_j = b_j (v_j - (P_j X_j + sum_{i<j} G_ij wu_i) / |k_j|),
+//   y_j = (P_j X'_j + sum_{i<=j} G'_ij wu_i) scale / |q_j|,
+// and the state after them is P S + sum_i wu_i k_i^T, a product again.
+//
+// A wave takes 64 rows of the state, four tiles of 16.  A lane of a 16x16x4
+// product holds row (or column) lane % 16 of an operand at the step's value
+// lane / 16, and rows 4 (lane / 16) .. + 3 of column lane % 16 of the result; four
+// steps are four neighbours of a row, so that the state, n = 16 x + 4 (lane / 16)
+// and on of row lane % 16, is operand and accumulator as it is loaded.
+// ---------------------------------------------------------------------------
+typedef float v4f __attribute__((ext_vector_type(4)));
+constexpr int kShort = 32;  // sequences of up to these rows go this way
+constexpr int kFew = 8;
+
+// keeps what is cheaply worked out anew from being held in registers over a loop
+__device__ __forceinline__ uint32_t anew(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// x[i] of lane group j becomes x[j] of lane group i, groups of 16 lanes
+__device__ __forceinline__ void transpose_groups(float (&x)[4]) {
+  auto swap = [](auto how, float& a, float& b) {
+    const auto r = how(__float_as_uint(a), __float_as_uint(b));
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+  };
+  auto halves = [](uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  };
+  auto rows = [](uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  };
+  swap(halves, x[0], x[2]);
+  swap(halves, x[1], x[3]);
+  swap(rows, x[0], x[1]);
+  swap(rows, x[2], x[3]);
+}
+
+template <typename T, int NX, int M, bool WIDE>
+__global__ __launch_bounds__(64, NX > 8 ? 1 : 2) void k_delta_few(DeltaArgs a) {
+  const int b = blockIdx.x, h = blockIdx.y;
+  const int lane = threadIdx.x, c = lane & 15, q = lane >> 4;
+  const int first = blockIdx.z * (16 * M);
+  const int t0 = a.q.seq_start ? seq_row(a.q, b) : 0;
+  const int t1 = a.q.seq_start ? seq_row(a.q, b + 1) : a.q.n_tokens;
+  if (t1 - t0 > kShort) return;
+  const int slot = find_slot(a.q, b, first_slots(a.q));
+  if (slot == kNoSlot) return;
+  const bool keep = slot >= 0 && !(a.q.fresh && a.q.fresh[b]);
+  if (t1 <= t0 && (keep || a.frozen || slot < 0)) return;
+  const int g = h / (a.heads / a.groups);
+  // the head's part of the slot; what lies past it reads as zeros and is not written
+  float* const state = a.state + (slot >= 0 ? (int64_t)slot * a.ss : 0) + (int64_t)h * a.hd * a.n;
+  const uint32_t state_bytes = (uint32_t)(a.hd * a.n * 4), head = (uint32_t)(a.hd * sizeof(T));
+  const int p = first + lane;  // the lane's row of the state
+  const uint32_t mine = lane < 16 * M ? (uint32_t)(p * sizeof(T)) : kNoColumn;
+  const int64_t col = (int64_t)h * a.hd, gcol = (int64_t)g * a.n;
+  auto place = [&](int m, int n) {
+    return n < a.n ? (uint32_t)(((first + 16 * m + c) * a.n + n) * 4) : kNoColumn;
+  };
+
+  const auto to = rows_at(state, slot >= 0 ? state_bytes : 0);
+  if (t1 <= t0) {  // no rows, and a state that begins with zeros
+    const float zero[1] = {0.0f};
+    for (int m = 0; m < M; ++m)
+      for (int n = q; n < a.n; n += 4) store_floats<1>(to, place(m, n), zero);
+    return;
+  }
+  v4f S[M][NX];
+  const auto from = rows_at(state, keep ? state_bytes : 0);
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      const int n = 16 * x + 4 * q;
+      if constexpr (WIDE) {
+        S[m][x] = __builtin_bit_cast(
+            v4f, __builtin_amdgcn_raw_buffer_load_b128(from, place(m, n), 0, 0));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[1];
+          load_floats<1>(f, from, place(m, n + i));
+          S[m][x][i] = f[0];
+        }
+      }
+    }
+  // each lane works out one row's decay and b
+  static_assert(kShort <= 64, "one for each lane");
+  const int64_t own = t0 + min(lane, t1 - t0 - 1);
+  const float dt = a.A ? (float)((const T*)a.dt)[own * a.dts + h] : 0.0f;
+  const Decay decays =
+      decay_of(exponent_of(a, a.A ? a.A[h] : 0.0f, dt, a.dt_bias ? a.dt_bias[h] : 0.0f));
+  const float betas = beta_of(a, a.beta ? (float)((const T*)a.beta)[own * a.bs + h] : 0.0f);
+
+  int64_t t = t0;
+  do {
+    const int rows = min(kFew, (int)(t1 - t));
+    // Rows past the last one are that one again: nothing of theirs is used.
+    const int64_t r = t + min(c & 7, rows - 1);
+    const T* src = c < 8 ? (const T*)a.K + r * a.Ks + gcol : (const T*)a.Q + r * a.Qs + gcol;
+    const int nq = (int)anew(4 * q);
+    v4f f[NX];
+    if constexpr (WIDE) {
+      Raw4<T> raw[NX];
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        const int n = 16 * x + nq;
+        raw[x] = *(const Raw4<T>*)__builtin_assume_aligned(src + (n < a.n ? n : 0), 4 * sizeof(T));
+      }
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[x][i] = 16 * x + nq < a.n ? raw4_f32<T>(raw[x], i) : 0.0f;
+    } else {
+      T raw[NX][4];
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[x][i] = src[min(16 * x + nq + i, a.n - 1)];
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[x][i] = 16 * x + nq + i < a.n ? (float)raw[x][i] : 0.0f;
+    }
+    T v[kFew], z[kFew];
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
+      const int64_t tj = t + min(j, rows - 1);
+      v[j] = ((const T*)a.v + tj * a.vs + col)[min(p, a.hd - 1)];
+      if (a.z) z[j] = ((const T*)a.z + tj * a.zs + col)[min(p, a.hd - 1)];
+    }
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    v4f G = zero, X[4] = {zero, zero, zero, zero};
+#pragma unroll
+    for (int x = 0; x < NX; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        G = __builtin_amdgcn_mfma_f32_16x16x4f32(f[x][i], f[x][i], G, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+          X[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[x][i], S[m][x][i], X[m], 0, 0, 0);
+      }
+    const bool on = !a.frozen || t + kFew < t1;  // the state is needed again
+    T kt[2][NX];
+    if (on) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const T* k = (const T*)a.K + (t + min(4 * s + q, rows - 1)) * a.Ks + gcol;
+#pragma unroll
+        for (int x = 0; x < NX; ++x) kt[s][x] = k[min(16 * x + (int)anew(c), a.n - 1)];
+      }
+    }
+    // 1 / |k| and scale / |q| of row 4 q + i, in lane 16 q + 4 q + i
+    const float square = (c & 2) ? ((c & 1) ? G[3] : G[2]) : ((c & 1) ? G[1] : G[0]);
+    const float units = unit_of(a, square) * (c < 8 ? 1.0f : a.scale);
+    auto unit = [&](int i) { return lane_f32(units, 16 * (i >> 2) + i); };
+    auto dot = [&](int i, int j) { return lane_f32(G[i & 3], 16 * (i >> 2) + j); };
+    float seen[16];  // X of the lane's row of the state
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x[4] = {X[0][i], X[1][i], X[2][i], X[3][i]};
+      transpose_groups(x);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) seen[4 * m + i] = x[m];
+    }
+    Decay all = {1.0f, 0.0f};
+    float wu[kFew];
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
+      wu[j] = 0.0f;
+      if (j >= rows) continue;
+      const int row = (int)(t - t0) + j;
+      const Decay decay = {lane_f32(decays.hi, row), lane_f32(decays.lo, row)};
+      const float hi = all.hi * decay.hi;
+      const float lo = __builtin_fmaf(all.hi, decay.hi, -hi) +
+                       __builtin_fmaf(all.hi, decay.lo, all.lo * decay.hi);
+      all.hi = hi + lo;
+      all.lo = (hi - all.hi) + lo;
+      float sk = __builtin_fmaf(seen[j], all.lo, seen[j] * all.hi);
+      float sq = __builtin_fmaf(seen[8 + j], all.lo, seen[8 + j] * all.hi);
+#pragma unroll
+      for (int i = 0; i < j; ++i) {
+        wu[i] *= decay.hi;
+        sk = __builtin_fmaf(dot(j, i), wu[i], sk);
+        sq = __builtin_fmaf(dot(8 + j, i), wu[i], sq);
+      }
+      const float uk = unit(j);
+      wu[j] = lane_f32(betas, row) * __builtin_fmaf(-uk, sk, (float)v[j]) * uk;
+      float y = __builtin_fmaf(dot(8 + j, j), wu[j], sq) * unit(8 + j);
+      if (a.z) y *= silu_f32((float)z[j]);
+      const float out[1] = {y};
+      store_row<T, 1>(rows_at((const T*)a.y + (t + j) * a.ys + col, head), mine, out);
+    }
+    if (!on) return;
+    float w[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[s][i] = wu[4 * s + i];
+      transpose_groups(w[s]);
+    }
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+        S[m][x] = __builtin_elementwise_fma(S[m][x], v4f{all.hi, all.hi, all.hi, all.hi},
+                                            S[m][x] * all.lo);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+          S[m][x] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)kt[s][x], w[s][m], S[m][x], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);  // in place
+    }
+    t += kFew;
+  } while (t < t1);
+  if (a.frozen) return;
+  const int nq = (int)anew(4 * q);
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      const int n = 16 * x + nq;
+      if constexpr (WIDE) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, S[m][x]), to, place(m, n),
+                                               0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f[1] = {S[m][x][i]};
+          store_floats<1>(to, place(m, n + i), f);
+        }
+      }
+    }
+}
+
+template <typename T, int NX>
+static hipError_t launch_few(const DeltaArgs& a, hipStream_t s) {
+  constexpr int M = NX > 8 ? 2 : 4;
+  const dim3 grid(a.q.n_seqs, a.heads, (a.hd + 16 * M - 1) / (16 * M));
+  if (a.wide) return launch(k_delta_few<T, NX, M, true>, grid, dim3(64), 0, s, a);
+  return launch(k_delta_few<T, NX, M, false>, grid, dim3(64), 0, s, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -277,10 +515,8 @@ static hipError_t launch_rows_t(const DeltaArgs& a, int most, hipStream_t s) {
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
-typedef float v4f __attribute__((ext_vector_type(4)));
 
-constexpr int kC = 64;       // rows of a chunk
-constexpr int kShort = 32;   // sequences of up to these rows go row by row
+constexpr int kC = 64;  // rows of a chunk
 template <typename T>
 constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;  // of a value of K or Q
 constexpr int kTri = 6 * 2 * 1024;  // bytes of T or A: blocks of 16 rows and 32 columns on and below the diagonal
@@ -389,12 +625,6 @@ __device__ __forceinline__ Scale scale_of(float largest) {
 // size is made of (quotients and clamps are worked out in vector registers, and
 // a resource in those costs a loop around each access)
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// keeps what is cheaply worked out anew from being held in registers over a loop
-__device__ __forceinline__ uint32_t anew(uint32_t v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
 
 // the block's LDS accesses are done; global ones stay in flight
 __device__ __forceinline__ void lds_sync() {
@@ -1240,9 +1470,11 @@ static hipError_t launch_chunks(const DeltaArgs& a, const DeltaPlan& pl, hipStre
 
 template <typename T>
 static hipError_t launch_delta(const DeltaArgs& a, const DeltaPlan& pl, bool step, hipStream_t s) {
-  if (step) return launch_rows_t<T, true>(a, 1, s);
+  if (step) return launch_step_t<T>(a, s);
   if (a.q.seq_start || !pl.chunks) {
-    const hipError_t e = launch_rows_t<T, false>(a, kShort, s);
+    const hipError_t e = a.n <= 64    ? launch_few<T, 4>(a, s)
+                         : a.n <= 128 ? launch_few<T, 8>(a, s)
+                                      : launch_few<T, 16>(a, s);
     if (e != hipSuccess || !pl.chunks) return e;
   }
   switch (delta_nk(a.n)) {
