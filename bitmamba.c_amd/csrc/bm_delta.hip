@@ -1263,9 +1263,11 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       residue();
       float mw = solve();
       int from = first;  // the column's rows from here on are NaN
-      if (__ballot(!(mw * most <= kTop) || (mw < kLow && mw > 0.0f && unit < 0x1p100f))) {
-        const float ms = largest();
-        const bool over = !(mw * most <= kTop), under = mw < kLow && ms < kLow && unit < 0x1p100f;
+      // (no w at all may also be a state too small for its halves)
+      const bool faint = mw < kLow && unit < 0x1p100f;
+      if (__ballot(!(mw * most <= kTop) || (faint && (mw > 0.0f || bound > 0.0f)))) {
+        const float ms = bound = largest();
+        const bool over = !(mw * most <= kTop), under = faint && ms < kLow && (mw > 0.0f || ms > 0.0f);
         if (__ballot(over || under)) {
           // infinities and NaN leave the products; `at` is the first row of one
           int at = kC;

@@ -457,6 +457,11 @@ int bm_hip_ssm_step_dev(const bm_hip_ssm_t *op, void *stream);
  * and leaves them as they are: drafted tokens are scored, and the accepted
  * ones given again (bm_hip_verify_dev's split_start).
  *
+ * Sequences of more than 32 rows are worked out 64 rows at a time, with
+ * products of operands of 22 bits: S[p], w[p] and what they make are then
+ * good to 2^-13 of the largest that S[p] (as a vector) and b * v[p] are
+ * within such a chunk, 64 times better where the errors are independent.
+ *
  * A key with b * (sum of k's squares) above 2 makes the rule grow without
  * end; qk_norm with b in 0..2 cannot.  Where such a growth passes fp32, the
  * head's later rows of the sequence are infinite, NaN or undefined.
@@ -471,7 +476,7 @@ typedef struct {
     int n_heads, head_dim;         /* v, z, y rows: [n_heads][head_dim] */
     int n_groups, d_state;         /* q, k rows: [n_groups][d_state]; n_groups divides n_heads, d_state <= 256 */
     int dt_softplus, beta_sigmoid, qk_norm, frozen;
-    float norm_eps, scale;         /* norm_eps at least 0, read with qk_norm */
+    float norm_eps, scale;         /* norm_eps 2^-100 and more, read with qk_norm */
     int n_seqs, n_tokens;
     const int32_t *seq_start;      /* device [n_seqs + 1], or NULL */
     const int32_t *slots;          /* device [n_seqs], or NULL */

@@ -202,6 +202,21 @@ def test_sizes_that_change_within_a_sequence(hip, first):
     close(c.pool()[k], pool[k], stol[k], "f32", "state")
 
 
+@pytest.mark.parametrize("size", [-110, -60, -20, 0, 60])
+@pytest.mark.parametrize("lens", [[130, 20], [64, 33, 5]])
+def test_a_state_and_no_values(hip, lens, size):
+    """v of zeros: all that is read is what the slots hold, however small."""
+    note("no values, state 2^%d, %s" % (size, lens))
+    c = DeltaCase("f32", 2, 20, 1, 64, lens, seed=11, rate=0.5)
+    c.v.zero_()
+    c.pool_buf.mul_(2.0 ** size)
+    rows, tols, pool, stol = c.want()
+    c.run(hip)
+    check_rows(c.ybuf, c.y, rows, tols, "f32", (2, 20), "no values")
+    for k, want in stol.items():
+        close(c.pool()[k], pool[k], want, "f32", "slot %d" % k)
+
+
 @pytest.mark.parametrize("at_row", [0, 63, 64, 100, 129])
 @pytest.mark.parametrize("what", ["v", "v max", "k", "q", "dt", "beta", "state"])
 def test_infinities_and_nan_stay_where_they_belong(hip, what, at_row):
