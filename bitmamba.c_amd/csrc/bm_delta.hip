@@ -246,7 +246,7 @@ static hipError_t launch_step_t(const DeltaArgs& a, hipStream_t s) {
 //   y_j = (P_j X'_j + sum_{i<=j} G'_ij wu_i) scale / |q_j|,
 // and the state after them is P S + sum_i wu_i k_i^T, a product again.
 //
-// A wave takes 64 rows of the state, four tiles of 16.  A lane of a 16x16x4
+// A wave takes M tiles of 16 rows of the state.  A lane of a 16x16x4
 // product holds row (or column) lane % 16 of an operand at the step's value
 // lane / 16, and rows 4 (lane / 16) .. + 3 of column lane % 16 of the result; four
 // steps are four neighbours of a row, so that the state, n = 16 x + 4 (lane / 16)
@@ -282,7 +282,7 @@ __device__ __forceinline__ void transpose_groups(float (&x)[4]) {
 }
 
 template <typename T, int NX, int M, bool WIDE>
-__global__ __launch_bounds__(64, NX > 8 ? 1 : 2) void k_delta_few(DeltaArgs a) {
+__global__ __launch_bounds__(64, (NX > 8 ? 1 : 2) * (M == 1 ? 2 : 1)) void k_delta_few(DeltaArgs a) {
   const int b = blockIdx.x, h = blockIdx.y;
   const int lane = threadIdx.x, c = lane & 15, q = lane >> 4;
   const int first = blockIdx.z * (16 * M);
@@ -480,12 +480,21 @@ __global__ __launch_bounds__(64, NX > 8 ? 1 : 2) void k_delta_few(DeltaArgs a) {
     }
 }
 
-template <typename T, int NX>
-static hipError_t launch_few(const DeltaArgs& a, hipStream_t s) {
-  constexpr int M = NX > 8 ? 2 : 4;
+template <typename T, int NX, int M>
+static hipError_t launch_few_m(const DeltaArgs& a, hipStream_t s) {
   const dim3 grid(a.q.n_seqs, a.heads, (a.hd + 16 * M - 1) / (16 * M));
   if (a.wide) return launch(k_delta_few<T, NX, M, true>, grid, dim3(64), 0, s, a);
   return launch(k_delta_few<T, NX, M, false>, grid, dim3(64), 0, s, a);
+}
+template <typename T, int NX>
+static hipError_t launch_few(const DeltaArgs& a, hipStream_t s) {
+  // One tile per wave while that is up to a wave per SIMD: the wave's own time counts
+  // then, and not that each wave works out G.  Sequences of 5 rows, 32 heads of 128 x
+  // 128, one tile against four: 1024 tiles 15.3 us against 19.2 (frozen 8.8 and
+  // 9.6), 2048 tiles 28.1 against 27.8 (16.0 and 15.4), 4096 51.5 against 47.0.
+  const int64_t tiles = (int64_t)a.q.n_seqs * a.heads * ((a.hd + 15) / 16);
+  if (tiles <= 1024) return launch_few_m<T, NX, 1>(a, s);
+  return launch_few_m<T, NX, (NX > 8 ? 2 : 4)>(a, s);
 }
 
 // ---------------------------------------------------------------------------

@@ -107,6 +107,16 @@ def test_many_sequences_of_which_few_are_long(hip, longs):
     DeltaCase("bf16", 2, 18, 1, 48, lens, front=5, tail=3, seed=3).check(hip, "many")
 
 
+@pytest.mark.parametrize("frozen", [False, True])
+@pytest.mark.parametrize("type_name", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N", [40, 45, 100, 131, 252])
+def test_many_short_sequences(hip, type_name, N, frozen):
+    """More tiles of the states than the chip holds waves at once."""
+    note("short sequences %s N=%d frozen=%s" % (type_name, N, frozen))
+    DeltaCase(type_name, 40, 50, 8, N, [5, 1, 0, 8, 9, 17, 32, 3, 24], frozen=frozen,
+              seed=N).check(hip, "short")
+
+
 def test_a_sequence_alone_needs_no_starts(hip):
     for n in (1, 32, 33, 300):
         note("one sequence of %d" % n)
