@@ -101,6 +101,8 @@ __device__ __forceinline__ float value_of(const RawRow<T, V>& r, int i) {
 // once and U such groups.  S k and S q are both taken from the state before
 // the row, so that it is read once:
 //   S' q = a (S q) + w (k . q).
+// The state's bytes bound it: 128 sequences of 32 heads of 128 x 128 move 541 MB
+// in 95 us, 5.7 TB/s; one sequence (4.3 MB) takes 4.2 us, a launch's latency.
 // ---------------------------------------------------------------------------
 template <typename T, int TEAM, int V, int E, int U, bool STREAM>
 __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
@@ -214,7 +216,9 @@ static hipError_t launch_step(const DeltaArgs& a, hipStream_t s) {
   const int waves = (a.hd + kRows - 1) / kRows;
   const int nw = waves < 4 ? waves : 4;
   const dim3 grid(a.q.n_seqs, a.heads, (waves + nw - 1) / nw);
-  // as the scan's single tokens: states of 64 MiB or more go past the caches
+  // States of 64 MiB or more go past the caches: 32 heads of 128 x 128 of 32, 64 and 128
+  // sequences that lie in turn in memory take 28.3, 51.7 and 95.2 us, through
+  // the caches 34.3, 58.3 and 105.4.
   constexpr bool kLarge = V == 4;
   if (kLarge && (int64_t)a.q.n_seqs * a.heads * a.hd * a.n >= (1 << 24))
     return launch(k_delta_step<T, TEAM, V, E, U, kLarge>, grid, dim3(64 * nw), 0, s, a);
@@ -251,9 +255,17 @@ static hipError_t launch_step_t(const DeltaArgs& a, hipStream_t s) {
 // lane / 16, and rows 4 (lane / 16) .. + 3 of column lane % 16 of the result; four
 // steps are four neighbours of a row, so that the state, n = 16 x + 4 (lane / 16)
 // and on of row lane % 16, is operand and accumulator as it is loaded.
+//
+// 64 sequences of 5 rows, 32 heads of 128 x 128 in bf16, take 39 us frozen (134 MB
+// read, 3.4 TB/s) and 103 us with the states written (268 MB): two waves per SIMD
+// load, multiply (224 products of 32 cycles for four tiles) and store in turn.
+// Row after row on the vector units they take 60 us frozen, bound by instructions.
 // ---------------------------------------------------------------------------
 typedef float v4f __attribute__((ext_vector_type(4)));
-constexpr int kShort = 32;  // sequences of up to these rows go this way
+// Sequences of up to these rows go this way.  At 32 heads of 128 x 128 in bf16: 64
+// sequences of 32 rows 278 us, in chunks 356, two of them 37 and 23; of 24 rows
+// 222 and 237, two of them 23 and 26.
+constexpr int kShort = 32;
 constexpr int kFew = 8;
 
 // keeps what is cheaply worked out anew from being held in registers over a loop
@@ -762,6 +774,11 @@ __device__ __forceinline__ float eight_f32(const Eight<T, WIDE>& e, int i) {
 // ---------------------------------------------------------------------------
 // One chunk of one head: T, A and the rows' scalars; for a group's first head
 // also K and Q as operands.  Wave w has the rows of tile w (spread_row).
+// Bound by memory for long prompts: 16384 rows at 32 heads of 128 in 16 groups
+// read 164 MB and write 404 MB in 143 us, 4.0 TB/s; without the operands of K and
+// Q it takes 120 us, without the inverse 127.  A short prompt (1024 rows of fp32 at
+// 32 heads, 29 us) waits for its steps.  Two and three waves per SIMD take the
+// same time, four (128 registers, with spills) 184 us.
 // ---------------------------------------------------------------------------
 template <typename T, int NK, bool WIDE>
 __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) {
@@ -1028,6 +1045,14 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 // there two halves are good to 2^-22 of it.  w is looked at in every chunk; of S
 // a bound is carried on, and its values looked at when that passes kTopS.  What
 // leaves the range, or fp32, goes another way, which works the chunk out anew.
+//
+// Bound by the steps of a chunk, each of which waits for the one before: 2.35 us
+// per chunk (603 us for 16384 rows at 32 heads of 128 x 128, on 256 blocks), of
+// whose 5600 cycles the first wave spends 1300 on products and about as many on
+// other instructions.  With all operands in the caches it takes 546 us, without
+// the second wave 562.  Two blocks per SIMD pair do not pay: in 256 registers the
+// operands of the next chunk no longer fit ahead (713 us), and staged in LDS by a
+// third wave they take 643 us.
 // ---------------------------------------------------------------------------
 constexpr float kTop = 32768.0f, kTopS = 4096.0f, kLow = 0.125f;
 constexpr int kAim = 127 + 1;  // exponent bits of what a new unit makes the largest
