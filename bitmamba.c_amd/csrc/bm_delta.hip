@@ -774,11 +774,12 @@ __device__ __forceinline__ float eight_f32(const Eight<T, WIDE>& e, int i) {
 // ---------------------------------------------------------------------------
 // One chunk of one head: T, A and the rows' scalars; for a group's first head
 // also K and Q as operands.  Wave w has the rows of tile w (spread_row).
-// Bound by memory for long prompts: 16384 rows at 32 heads of 128 in 16 groups
-// read 164 MB and write 404 MB in 143 us, 4.0 TB/s; without the operands of K and
-// Q it takes 120 us, without the inverse 127.  A short prompt (1024 rows of fp32 at
-// 32 heads, 29 us) waits for its steps.  Two and three waves per SIMD take the
-// same time, four (128 registers, with spills) 184 us.
+// 16384 rows at 32 heads of 128 in 16 groups take 143 us: 413 MB written, 328 MB
+// read, vector instructions on 44 % of the cycles.  Without the operands of K and Q
+// it takes 120 us, without the inverse 127, without both 98.  What it waits for are
+// its own steps: with the heads of a group on one XCD it reads 133 MB in the same
+// time, with two and with three waves per SIMD too; four (128 registers, with
+// spills) take 184 us.  A short prompt (1024 rows of fp32) takes 29 us.
 // ---------------------------------------------------------------------------
 template <typename T, int NK, bool WIDE>
 __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) {
