@@ -1056,14 +1056,16 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 // third wave they take 643 us.
 // ---------------------------------------------------------------------------
 constexpr float kTop = 32768.0f, kTopS = 4096.0f, kLow = 0.125f;
-constexpr int kAim = 127 + 1;  // exponent bits of what a new unit makes the largest
+constexpr int kAim = 127 + 1, kTopAim = 127 + 10;  // exponent bits that a new unit gives the largest
 
 __device__ __forceinline__ int exponent_bits(float v) { return (int)(__float_as_uint(v) >> 23 & 255); }
 // The power of two, of up to 2^-126 and 2^100, that takes a magnitude with the
-// exponent bits e to kAim's, as far as `unit` times it stays in that range.
+// exponent bits e up to kAim's, where there is room to grow, or down to kTopAim's,
+// where smaller values of the column lose least, as far as `unit` times it stays
+// in that range.
 __device__ __forceinline__ float to_range(int e, float unit) {
-  const int ue = exponent_bits(unit);
-  const int d = min(max(kAim - e, max(1 - ue, -126)), min(227 - ue, 100));
+  const int ue = exponent_bits(unit), want = max(kAim, min(e, kTopAim));
+  const int d = min(max(want - e, max(1 - ue, -126)), min(227 - ue, 100));
   return __uint_as_float((uint32_t)(127 + d) << 23);
 }
 __device__ __forceinline__ v4f mfma_one(v8h a, v8h b, v4f c) {

@@ -212,6 +212,28 @@ def test_sizes_that_change_within_a_sequence(hip, first):
     close(c.pool()[k], pool[k], stol[k], "f32", "state")
 
 
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 16, 2.0 ** 20])
+def test_rows_before_a_large_one_of_their_chunk(hip, size):
+    """One v at the end of a chunk is `size` times the others.  The column's scale
+    takes it to 2^10 .. 2^11, so that other operands are good to 2^-25 of that or
+    size 2^-35.  As independent errors, w adds up 64 of them (8 times one) and y
+    64 of w's: size 2^-29, besides the 2^-19 of fp32 sums and operands of 22 bits
+    that kSpread allows."""
+    note("rows before v = %g" % size)
+    c = DeltaCase("f32", 2, 20, 1, 64, [128], seed=12, rate=0.5, gate=False)
+    c.v[63, 7] = size
+    c.v[127, 30] = -size
+    rows, tols, pool, stol = c.want()
+    c.run(hip)
+    check_rows(c.ybuf, c.y, rows, tols, "f32", (2, 20), "before")
+    got = f64(c.y).reshape(128, 2, 20)
+    for h, p, n in ((0, 7, 63), (1, 10, 127)):
+        off = np.array([got[t, h, p] - rows[t][h, p] for t in range(n)])
+        all_of_it = np.array([rows[t][h, p] for t in range(n)])
+        rms = lambda v: np.sqrt((v * v).mean())
+        assert rms(off) <= size * 2.0 ** -29 + rms(all_of_it) * 2.0 ** -19, (rms(off), rms(all_of_it))
+
+
 @pytest.mark.parametrize("size", [-110, -60, -20, 0, 60])
 @pytest.mark.parametrize("lens", [[130, 20], [64, 33, 5]])
 def test_a_state_and_no_values(hip, lens, size):
