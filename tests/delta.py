@@ -5,7 +5,8 @@ Bounds.  u = 2^-24.  One row takes S[p] to a S[p] (I - b k k^T) + b v[p] k^T, an
 with |k| <= 1 and 0 <= b <= 2 the matrix lengthens no vector, so an error in S[p]
 (as a vector of d_state values) does not grow, and the rows' own errors add up.
 
-Row after row (single tokens, sequences of up to 32 rows): a product of N
+Row after row (single tokens; sequences of up to 32 rows, eight at a time, whose
+sums are the same with up to eight terms more): a product of N
 factors is off by N u of the vectors' lengths, the decay by 10 u (1 + |A d|), the
 other operations by a few u each: per row
     u ((N + 16) b |S| + (24 + 10 |A d|) (|S| + |b v|)).
