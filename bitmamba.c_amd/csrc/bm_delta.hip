@@ -259,12 +259,14 @@ static hipError_t launch_step_t(const DeltaArgs& a, hipStream_t s) {
 // 64 sequences of 5 rows, 32 heads of 128 x 128 in bf16, take 39 us frozen (134 MB
 // read, 3.4 TB/s) and 103 us with the states written (268 MB): two waves per SIMD
 // load, multiply (224 products of 32 cycles for four tiles) and store in turn.
+// With keys and queries loaded before the state, and the next eight rows' during
+// these, the latter takes 5 % less, and one sequence 4 to 15 % more.
 // Row after row on the vector units they take 60 us frozen, bound by instructions.
 // ---------------------------------------------------------------------------
 typedef float v4f __attribute__((ext_vector_type(4)));
 // Sequences of up to these rows go this way.  At 32 heads of 128 x 128 in bf16: 64
-// sequences of 32 rows 278 us, in chunks 356, two of them 37 and 23; of 24 rows
-// 222 and 237, two of them 23 and 26.
+// sequences of 32 rows 279 us, in chunks 331, of 24 rows 222 and 216; two
+// sequences of 32 rows 37 and 22, of 24 rows 24 and 25.
 constexpr int kShort = 32;
 constexpr int kFew = 8;
 
@@ -503,7 +505,7 @@ static hipError_t launch_few(const DeltaArgs& a, hipStream_t s) {
   // One tile per wave while that is up to a wave per SIMD: the wave's own time counts
   // then, and not that each wave works out G.  Sequences of 5 rows, 32 heads of 128 x
   // 128, one tile against four: 1024 tiles 15.3 us against 19.2 (frozen 8.8 and
-  // 9.6), 2048 tiles 28.1 against 27.8 (16.0 and 15.4), 4096 51.5 against 47.0.
+  // 9.6), 2048 tiles 28.7 against 27.6 (17.0 and 16.3), 4096 51.2 against 46.0.
   const int64_t tiles = (int64_t)a.q.n_seqs * a.heads * ((a.hd + 15) / 16);
   if (tiles <= 1024) return launch_few_m<T, NX, 1>(a, s);
   return launch_few_m<T, NX, (NX > 8 ? 2 : 4)>(a, s);
