@@ -512,23 +512,27 @@ static hipError_t launch_few(const DeltaArgs& a, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Prompts: chunks of kC rows on the matrix cores.  With c_i the sum of the
-// exponents of a chunk's rows up to i and S the state before it, what the rows
-// write, w, solves
-//   w_i + sum_{j<i} L_ij w_j = b_i (v_i - e^{c_i} S k_i),
-//   L_ij = b_i e^{c_i - c_j} (k_i . k_j),
+// Prompts: chunks of kC rows on the matrix cores.  A key is taken as r_i k_i with
+// k_i of a length of 1 to 2 (r_i a power of two, and what norm_eps makes of it),
+// and instead of w_i, what row i writes, r_i w_i is worked out, which is the size
+// of what that leaves in the state whatever the key's length.  With c_i the sum of
+// the exponents of a chunk's rows up to i and S the state before it, r w =: w solves
+//   w_i + sum_{j<i} L_ij w_j = b_i r_i v_i - b_i r_i^2 e^{c_i} S k_i,
+//   L_ij = b_i r_i^2 e^{c_i - c_j} (k_i . k_j),
 // so with T = (I + L)^-1 (unit lower triangular) and A_ij = e^{c_i - c_j}
 // (q_i . k_j) for j <= i, as products of kC rows
-//   w = T (b (v - e^c K S)),  y = e^c Q S + A w,  S' = e^{c_C} S + (e^{c_C - c} K)^T w.
+//   R = b r v - b r^2 e^c K S,  w = T R,
+//   y = e^c Q S + A w,  S' = e^{c_C} S + K^T (e^{c_C - c} w).
 // T and A need no state: the first launch makes them for all chunks and heads
 // at once, the second walks each sequence's chunks.
 //
 // Precision.  MFMA operands are fp16.  A value is one half, or the sum of two
 // (22 bits) where it is computed or fp32; what leaves fp16's range of exponents
 // is scaled by powers of two: the rows of K, Q, T and A once, the columns of
-// the state and of w (one value of v each) as they grow and shrink.  The state
-// itself stays in fp32 accumulators.  bf16 in three pieces is as exact and
-// needs no scaling, but twice the products and 2.7 times the conversions.
+// the state, R and w (one value of v each) as they grow and shrink.  b is in R, not
+// in T: a value that is hardly written, or not at all, must not set that scale.
+// The state itself stays in fp32 accumulators.  bf16 in three pieces is as exact
+// and needs no scaling, but twice the products and 2.7 times the conversions.
 //
 // An infinity or NaN must not reach earlier rows of its chunk through a zero
 // of T or A: a head's first row of that kind (k, a or b) ends what its chunk
@@ -543,10 +547,10 @@ constexpr int kC = 64;  // rows of a chunk
 template <typename T>
 constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;  // of a value of K or Q
 constexpr int kTri = 6 * 2 * 1024;  // bytes of T or A: blocks of 16 rows and 32 columns on and below the diagonal
-// per place and head after T and A, 64 floats each: e^c of k; e^{c_C - c} of k; e^c of q; the
-// scales of A and T; then the decay (two parts), the first bad row, the largest of the second
-enum { kGrowK, kLeft, kGrowQ, kFacA, kFacT, kMisc };
-constexpr int kScalars = 6 * 256;
+// per place and head after T and A, 64 floats each: b r^2 e^c; b r; e^{c_C - c}; e^c of q; the
+// scales of A and T; then the decay (two parts) and the first bad row
+enum { kGrowK, kWrite, kLeft, kGrowQ, kFacA, kFacT, kMisc };
+constexpr int kScalars = 7 * 256;
 
 struct DeltaPlan {
   bool chunks;     // a sequence may have more than kShort rows
@@ -639,9 +643,17 @@ __device__ __forceinline__ float quads_add(float v) {
 struct Scale {
   float up, down;
 };
-__device__ __forceinline__ Scale scale_of(float largest) {
-  const int e = min(max((int)(__float_as_uint(largest) >> 23 & 255), 1), 253);
+__device__ __forceinline__ int exponent_bits(float v) { return (int)(__float_as_uint(v) >> 23 & 255); }
+__device__ __forceinline__ Scale scale_of_bits(int bits) {
+  const int e = min(max(bits, 1), 253);
   return Scale{__uint_as_float((uint32_t)(254 - e) << 23), __uint_as_float((uint32_t)e << 23)};
+}
+__device__ __forceinline__ Scale scale_of(float largest) { return scale_of_bits(exponent_bits(largest)); }
+// the same for its length, given the sum of its squares; lengths below 2^-50,
+// whose squares lose bits, go by the largest magnitude
+__device__ __forceinline__ Scale scale_of_length(float largest, float squares) {
+  const int e = exponent_bits(squares);
+  return scale_of_bits(e < 27 || e == 255 ? exponent_bits(largest) : 127 + ((e - 127) >> 1));
 }
 
 // a value that all lanes share, in a scalar register: what a buffer's address or
@@ -789,8 +801,7 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
   constexpr int kShared = 4 * kTile > kC * kRowL * 4 ? 4 * kTile : kC * kRowL * 4;
   __shared__ __attribute__((aligned(16))) uint8_t shK[kShared];  // K; then T
   __shared__ __attribute__((aligned(16))) float shL[kC * kRowL];
-  __shared__ __attribute__((aligned(16))) float shHi[kC], shLo[kC], shRk[kC];
-  __shared__ __attribute__((aligned(16))) float shB[kC];
+  __shared__ __attribute__((aligned(16))) float shHi[kC], shLo[kC];
   __shared__ float shKk[kC], shKd[kC], shQf[kC];
   float* shT = (float*)shK;
   Unit u = find_unit(a.q, (int)wide_block(), kC);
@@ -848,8 +859,8 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
         m = max_abs(m, v);
         kk = __builtin_fmaf(v, v, kk);
       }
-    const Scale sc = scale_of(quads_max(m));
     kk = quads_add(kk);
+    const Scale sc = scale_of_length(quads_max(m), kk);
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
       float v[8];
@@ -896,37 +907,32 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
   // the rows' scalars, in every wave alike
   const float squares = shKk[lane], rq = lane < rows ? shQf[lane] : 0.0f;
   const bool in = lane < rows;
-  const bool bad = in && !(expo <= 0.0f && __builtin_fabsf(beta) < __builtin_inff() &&
-                           squares < __builtin_inff());
+  // b r and b r^2; not finite where b, the key or b |k|^2 is not
+  const float rk = unit_of(a, squares) * shKd[lane], write = beta * rk, turn = write * rk;
+  const bool bad = in && !(expo <= 0.0f && __builtin_fabsf(turn) < __builtin_inff());
   const uint64_t bads = __ballot(bad);
   const int first = bads ? __ffsll((unsigned long long)bads) - 1 : kC;
   const bool live = in && lane < first;
   double cum = live ? (double)expo * 1.4426950408889634 : 0.0;
   cum = scan_f64(cum < -256.0 ? -256.0 : cum);
   const double whole = __shfl(cum, 63);
-  const float rk = live ? unit_of(a, squares) * shKd[lane] : 0.0f;
-  const float b = live ? beta : 0.0f;
   const float hi = (float)cum, grow = __builtin_amdgcn_exp2f(hi);
   shHi[lane] = hi;
   shLo[lane] = (float)(cum - (double)hi);
-  shRk[lane] = rk;
   float* scalars = (float*)(out + 2 * kTri);
   if (wave == 0) {
-    const float left = __builtin_amdgcn_exp2f((float)(whole - cum)) * rk;
-    shB[lane] = b;
-    scalars[kGrowK * 64 + lane] = grow * rk;
-    scalars[kLeft * 64 + lane] = left;
+    scalars[kGrowK * 64 + lane] = live ? grow * turn : 0.0f;
+    scalars[kWrite * 64 + lane] = live ? write : 0.0f;
+    scalars[kLeft * 64 + lane] = live ? __builtin_amdgcn_exp2f((float)(whole - cum)) : 0.0f;
     scalars[kGrowQ * 64 + lane] = grow * rq;
-    const float most = wave_max_f32(left);
     if (lane == 0) {
       const Decay d = decay_of((float)(whole * 0.6931471805599453));
       scalars[kMisc * 64] = d.hi;
       scalars[kMisc * 64 + 1] = d.lo;
       ((int*)scalars)[kMisc * 64 + 2] = first;
-      scalars[kMisc * 64 + 3] = most;
     }
   }
-  const float bi = __shfl(b * rk, mine), qi = __shfl(rq, mine);
+  const float bi = __shfl(live ? turn : 0.0f, mine), qi = __shfl(rq, mine);
 
   // (k_j . k_i) and (k_j . q_i): i a row of the wave's, by lane; j up to it
   v4f kk[4], kq[4];
@@ -978,14 +984,12 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
       const int j0 = 32 * sp + 8 * q;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float4 jh = *(const float4*)(shHi + j0 + 4 * k), jl = *(const float4*)(shLo + j0 + 4 * k),
-                     jr = *(const float4*)(shRk + j0 + 4 * k);
-        const float h4[4] = {jh.x, jh.y, jh.z, jh.w}, l4[4] = {jl.x, jl.y, jl.z, jl.w},
-                    r4[4] = {jr.x, jr.y, jr.z, jr.w};
+        const float4 jh = *(const float4*)(shHi + j0 + 4 * k), jl = *(const float4*)(shLo + j0 + 4 * k);
+        const float h4[4] = {jh.x, jh.y, jh.z, jh.w}, l4[4] = {jl.x, jl.y, jl.z, jl.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = j0 + 4 * k + e;
-          const float d = __builtin_amdgcn_exp2f((ihi - h4[e]) + (ilo - l4[e])) * r4[e];
+          const float d = __builtin_amdgcn_exp2f((ihi - h4[e]) + (ilo - l4[e]));
           const float lv = bi * (d * kk[2 * sp + k][e]), mv = qi * (d * kq[2 * sp + k][e]);
           l[4 * k + e] = j < mine && mine < first ? lv : 0.0f;
           m8[sp][4 * k + e] = j <= mine && j < first ? mv : 0.0f;
@@ -1022,12 +1026,11 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
       const int j0 = 32 * sp + 8 * q;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float4 x = *(const float4*)(shT + mine * kRowL + j0 + 4 * k),
-                     y = *(const float4*)(shB + j0 + 4 * k);
-        const float t4[4] = {x.x, x.y, x.z, x.w}, b4[4] = {y.x, y.y, y.z, y.w};
+        const float4 x = *(const float4*)(shT + mine * kRowL + j0 + 4 * k);
+        const float t4[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v8[sp][4 * k + e] = j0 + 4 * k + e <= mine ? t4[e] * b4[e] : 0.0f;
+          v8[sp][4 * k + e] = j0 + 4 * k + e <= mine ? t4[e] : 0.0f;
           mt = max_abs(mt, v8[sp][4 * k + e]);
         }
       }
@@ -1043,11 +1046,14 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 // the state and the w that the first leaves in LDS.  Nothing is exchanged
 // between lanes: results serve as operands (spread_row).
 //
-// The state S and w are held times a power of two per column, `unit`, so that the
-// largest of S and w is at least kLow and S and w pass neither kTopS nor kTop:
-// there two halves are good to 2^-22 of it.  w is looked at in every chunk; of S
-// a bound is carried on, and its values looked at when that passes kTopS.  What
-// leaves the range, or fp32, goes another way, which works the chunk out anew.
+// The state S and w (the prompts' r w, above) are held times a power of two per
+// column, `unit`, so that the largest of S and w is at least kLow and S and w pass
+// neither kTopS nor kTop: there two halves are good to 2^-23 of it.  The first unit
+// goes by the state and the first chunk's b r v.  w is looked at in every chunk; of
+// S a bound is carried on, and its values looked at when that passes kTopS.  What
+// leaves the range, or fp32, goes another way: a unit by the largest of S and b r v,
+// and the chunk worked out anew.  (Where these are in range and w and S still below
+// kLow, w is what is left of larger terms, and as good as they are.)
 //
 // Bound by the steps of a chunk, each of which waits for the one before: 2.35 us
 // per chunk (603 us for 16384 rows at 32 heads of 128 x 128, on 256 blocks), of
@@ -1057,10 +1063,9 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 // operands of the next chunk no longer fit ahead (713 us), and staged in LDS by a
 // third wave they take 643 us.
 // ---------------------------------------------------------------------------
-constexpr float kTop = 32768.0f, kTopS = 4096.0f, kLow = 0.125f;
-constexpr int kAim = 127 + 1, kTopAim = 127 + 10;  // exponent bits that a new unit gives the largest
+constexpr float kTop = 32768.0f, kTopS = 16384.0f, kLow = 1.0f;
+constexpr int kAim = 127 + 4, kTopAim = 127 + 10;  // exponent bits that a new unit gives the largest
 
-__device__ __forceinline__ int exponent_bits(float v) { return (int)(__float_as_uint(v) >> 23 & 255); }
 // The power of two, of up to 2^-126 and 2^100, that takes a magnitude with the
 // exponent bits e up to kAim's, where there is room to grow, or down to kTopAim's,
 // where smaller values of the column lose least, as far as `unit` times it stays
@@ -1201,7 +1206,7 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
     // operands of the next chunk are loaded when those of this one are done with
     v8h kf[NK][4][KP], kt[2][NT][KP], tf[6][2];
     uint32_t vr[4][4];
-    v4f grow[4], left[4], fac[4];
+    v4f grow[4], write[4], left[4], fac[4];
     auto fetch_k = [&](__amdgpu_buffer_rsrc_t k) {
 #pragma unroll
       for (int x = 0; x < NK; ++x)
@@ -1240,17 +1245,40 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       fetch_k(k);
       values(a.v, a.vs, 0, vr);
       scalars(o, kGrowK, grow);
+      scalars(o, kWrite, write);
       triangle(o, 0, tf);
       scalars(o, kFacT, fac);
       fetch_kt(k);
       scalars(o, kLeft, left);
     }
-    bound = __builtin_inff();
+    // the unit by the largest finite of the state, ms, and of b r v
+    auto aim = [&](bool off, float ms) {
+      float mv = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = __builtin_fabsf(raw_f32<T>(vr[w][i]) * write[w][i]);
+          mv = v < __builtin_inff() ? fmaxf(mv, v) : mv;
+        }
+      mv = quads_max(mv);
+      int bits = max(mv > 0.0f ? exponent_bits(mv) + exponent_bits(unit) - 127 : 0,
+                     ms > 0.0f && ms < __builtin_inff() ? exponent_bits(ms) : 0);
+      off = off && bits > 0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // one power of two may not reach
+        const float f = off ? to_range(bits, unit) : 1.0f;
+        rescale(f);
+        bits += exponent_bits(f) - 127;
+      }
+    };
+    bound = largest();
+    aim(true, bound);
     for (int c = 0; c < chunks; ++c) {
       const int next = c + 1 < chunks ? c + 1 : c;
       const auto head1 = head_of(next), keys1 = keys_of(next);
       const float* misc = (const float*)(heads0 + c * head_step + 2 * kTri) + kMisc * 64;
-      const float dec_hi = misc[0], dec_lo = misc[1], most = fmaxf(misc[3], 1.0f);
+      const float dec_hi = misc[0], dec_lo = misc[1];
       const int first = ((const int*)misc)[2];
       uint8_t* buf = sh[c & 1];
       if (__ballot(!(bound <= kTopS))) {
@@ -1276,14 +1304,14 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       product([&](int x, const v8h (&sf)[2]) { mfma_many(X, kf[x], sf); });
       __builtin_amdgcn_sched_barrier(0);
       fetch_k(keys1);
-      // R = v - e^c K S, w = T b R
+      // R = b r v - b r^2 e^c K S, w = T R
       v4f R[4], W[4];
       auto residue = [&]() {
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            R[w][i] = __builtin_fmaf(-grow[w][i], X[w][i], raw_f32<T>(vr[w][i]) * unit);
+            R[w][i] = __builtin_fmaf(-grow[w][i], X[w][i], raw_f32<T>(vr[w][i]) * write[w][i] * unit);
       };
       auto solve = [&]() {
         v8h rf[2][2];
@@ -1304,10 +1332,11 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       int from = first;  // the column's rows from here on are NaN
       // (no w at all may also be a state too small for its halves)
       const bool faint = mw < kLow && unit < 0x1p100f;
-      if (__ballot(!(mw * most <= kTop) || (faint && (mw > 0.0f || bound > 0.0f)))) {
-        const float ms = bound = largest();
-        const bool over = !(mw * most <= kTop), under = faint && ms < kLow && (mw > 0.0f || ms > 0.0f);
-        if (__ballot(over || under)) {
+      if (__ballot(!(mw <= kTop) || (faint && (mw > 0.0f || bound > 0.0f)))) {
+        const float ms = bound = largest(), unit0 = unit;
+        const bool over = !(mw <= kTop);
+        aim(over || (faint && ms < kLow), ms);
+        if (__ballot(over || unit != unit0)) {  // all of it anew
           // infinities and NaN leave the products; `at` is the first row of one
           int at = kC;
           auto tame = [&](v4f (&v)[4]) {
@@ -1324,27 +1353,6 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
               }
             return quads_max(m);
           };
-          // A unit by the largest finite of v and the state, in bits of an
-          // exponent; then all of it anew.
-          float mv = 0.0f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v = __builtin_fabsf(raw_f32<T>(vr[w][i]));
-              mv = v < __builtin_inff() ? fmaxf(mv, v) : mv;
-            }
-          mv = quads_max(mv);
-          int bits = max(mv > 0.0f ? exponent_bits(mv) + exponent_bits(unit) - 127 : 0,
-                         ms > 0.0f && ms < __builtin_inff() ? exponent_bits(ms) : 0);
-          const bool off = (over || under) && bits > 0;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {  // one power of two may not reach
-            const float f = off ? to_range(bits, unit) : 1.0f;
-            rescale(f);
-            bits += exponent_bits(f) - 127;
-          }
-          bound = ms;
           const auto k = keys_of(c);
           product([&](int x, const v8h (&sf)[2]) {
 #pragma unroll
@@ -1362,7 +1370,7 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
           for (int w = 0; w < 4; ++w) R[w] *= f;
           (void)solve();
           mw = tame(W);
-          f = mw * most > kTop ? to_range(exponent_bits(mw) + exponent_bits(most) - 127, unit) : 1.0f;
+          f = mw > kTop ? to_range(exponent_bits(mw), unit) : 1.0f;
           rescale(f);
           mw *= f;
 #pragma unroll
@@ -1375,6 +1383,7 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       __builtin_amdgcn_sched_barrier(0);
       values(a.v, a.vs, next, vr);
       scalars(head1, kGrowK, grow);
+      scalars(head1, kWrite, write);
       triangle(head1, 0, tf);
       scalars(head1, kFacT, fac);
       // w for the other wave, and times e^{c_C - c} for the state
@@ -1392,7 +1401,7 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       // so that the product over all chunks is good to 2^-24.
       const float low = __builtin_fmaf(dec_hi, lost, dec_lo), decay = dec_hi + low;
       lost = decay > 0.0f ? ((dec_hi - decay) + low) * __builtin_amdgcn_rcpf(decay) : 0.0f;
-      bound = __builtin_fmaf(bound, decay, 128.0f * mw * most);  // |K| < 2, 64 rows
+      bound = __builtin_fmaf(bound, decay, 128.0f * mw);  // |K| < 2, 64 rows
       const float by = from < kC ? __builtin_nanf("") : decay;
 #pragma unroll
       for (int t = 0; t < NT; ++t) S[t] *= by;

@@ -458,8 +458,8 @@ int bm_hip_ssm_step_dev(const bm_hip_ssm_t *op, void *stream);
  * ones given again (bm_hip_verify_dev's split_start).
  *
  * Sequences of more than 32 rows are worked out 64 rows at a time, with
- * products of operands of 22 bits: S[p], w[p] and what they make are then
- * good to 2^-13 of the largest that S[p] (as a vector) and b * v[p] are
+ * products of operands of 22 bits: S[p] and what is read from it are then
+ * good to 2^-13 of the largest that S[p] and b * v[p] * k (as vectors) are
  * within such a chunk, 64 times better where the errors are independent.
  *
  * A key with b * (sum of k's squares) above 2 makes the rule grow without
