@@ -1262,9 +1262,10 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
           mv = v < __builtin_inff() ? fmaxf(mv, v) : mv;
         }
       mv = quads_max(mv);
-      int bits = max(mv > 0.0f ? exponent_bits(mv) + exponent_bits(unit) - 127 : 0,
-                     ms > 0.0f && ms < __builtin_inff() ? exponent_bits(ms) : 0);
-      off = off && bits > 0;
+      constexpr int kNone = -1000;
+      int bits = max(mv > 0.0f ? exponent_bits(mv) + exponent_bits(unit) - 127 : kNone,
+                     ms > 0.0f && ms < __builtin_inff() ? exponent_bits(ms) : kNone);
+      off = off && bits != kNone;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {  // one power of two may not reach
         const float f = off ? to_range(bits, unit) : 1.0f;
@@ -1330,12 +1331,12 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       residue();
       float mw = solve();
       int from = first;  // the column's rows from here on are NaN
-      // (no w at all may also be a state too small for its halves)
-      const bool faint = mw < kLow && unit < 0x1p100f;
-      if (__ballot(!(mw <= kTop) || (faint && (mw > 0.0f || bound > 0.0f)))) {
+      // (no w at all may also be values or a state too small for their halves)
+      const bool over = !(mw <= kTop), faint = mw < kLow && unit < 0x1p100f && p < a.hd;
+      if (__ballot(over || faint)) {
         const float ms = bound = largest(), unit0 = unit;
-        const bool over = !(mw <= kTop);
-        aim(over || (faint && ms < kLow), ms);
+        const bool off = over || (faint && ms < kLow);
+        if (__ballot(off)) aim(off, ms);
         if (__ballot(over || unit != unit0)) {  // all of it anew
           // infinities and NaN leave the products; `at` is the first row of one
           int at = kC;

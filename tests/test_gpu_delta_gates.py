@@ -82,6 +82,27 @@ def test_gates_that_open_and_shut(hip):
     c.check(hip, "open and shut")
 
 
+@pytest.mark.parametrize("size", [-20, -30, -60])
+def test_small_values_after_none(hip, size):
+    """A chunk in which nothing is written to a state of zeros comes first."""
+    note("2^%d after nothing" % size)
+    c = case(lens=[200, 40], seed=7)
+    c.pool_buf.zero_()
+    c.v[:100] = 0.0
+    c.v[100:].mul_(2.0 ** size)
+    c.check(hip, "after none")
+
+
+def test_small_values_after_large_ones_that_are_gone(hip):
+    """2^90 first, then 2^-70, with decays that leave nothing of a row two rows on."""
+    note("2^-70 after 2^90")
+    c = case(lens=[300], seed=8)
+    c.A.fill_(-200.0)
+    c.v[:100].mul_(2.0 ** 90)
+    c.v[100:].mul_(2.0 ** -70)
+    c.check(hip, "after large ones")
+
+
 @pytest.mark.parametrize("step", [False, True])
 @pytest.mark.parametrize("size", [-20, -8, 8, 20])
 def test_keys_of_any_length(hip, size, step):
