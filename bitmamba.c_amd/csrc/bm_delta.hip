@@ -34,9 +34,11 @@ __device__ __forceinline__ float exponent_of(const DeltaArgs& a, float A, float 
   const float p = A * (a.softplus ? softplus_f32(dt) : dt);
   return p > 0.0f ? 0.0f : p;
 }
+// (NaN for an infinite one, which would leave infinities of either sign)
 __device__ __forceinline__ float beta_of(const DeltaArgs& a, float b) {
   if (!a.beta) return 1.0f;
-  return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_f32(-b)) : b;
+  if (a.sigmoid) return __builtin_amdgcn_rcpf(1.0f + exp_f32(-b));
+  return __builtin_fabsf(b) < __builtin_inff() ? b : __builtin_nanf("");
 }
 // what a row of q or k is multiplied by; NaN where its squares' sum is not finite
 __device__ __forceinline__ float unit_of(const DeltaArgs& a, float squares) {

@@ -2,11 +2,12 @@
 shut, values that no gate lets through, keys of any length.  What a row writes,
 b v |k|, and the state are then far from v, and both are held to the bounds of
 tests/delta.py, which go by them alone."""
+import numpy as np
 import pytest
 import torch
 
 from delta import DeltaCase
-from recurrence import check_rows, close
+from recurrence import check_rows, close, f64
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +151,26 @@ def test_b_up_to_two(hip, keys, step):
     check_rows(c.ybuf, c.y, rows, tols, "f32", (2, 20), "b up to 2")
     for k, tol in stol.items():
         close(c.pool()[k], pool[k], tol, "f32", "slot %d" % k)
+
+
+@pytest.mark.parametrize("lens,at_row", [([130], 70), ([130], 0), ([20], 7), ([1], 0)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_an_infinite_b(hip, value, lens, at_row):
+    """The head is NaN from its row on, y and state, in prompts, short sequences
+    and single tokens; the sigmoid of an infinite logit is 0 or 1."""
+    note("b = %r, %s" % (value, lens))
+    for step in ([True, False] if lens == [1] else [False]):
+        c = DeltaCase("f32", 2, 20, 1, 64, lens, seed=9, step=step, beta="raw", gate=False)
+        rows, tols, pool, stol = c.want()
+        c.beta[at_row, 1] = value
+        c.run(hip)
+        got, state = f64(c.y).reshape(-1, 2, 20), c.pool()[c.slots[0]]
+        assert np.isnan(got[at_row:, 1]).all() and np.isnan(state[1]).all()
+        for t in rows:
+            ok = slice(0, 1 if t >= at_row else 2)
+            close(got[t][ok], rows[t][ok], tols[t][ok], "f32", "row %d" % t)
+        close(state[0], pool[c.slots[0]][0], stol[c.slots[0]][0], "f32", "state")
+        if value == value:
+            c = DeltaCase("f32", 2, 20, 1, 64, lens, seed=9, step=step)
+            c.beta[at_row, 1] = value
+            c.check(hip, "logit")
