@@ -1050,10 +1050,9 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 //
 // The state S and w (the prompts' r w, above) are held times a power of two per
 // column, `unit`, so that the largest of S and w is at least kLow and S and w pass
-// neither kTopS nor kTop: there two halves are good to 2^-23 of it.  The first unit
-// goes by the state and the first chunk's b r v.  w is looked at in every chunk; of
-// S a bound is carried on, and its values looked at when that passes kTopS.  What
-// leaves the range, or fp32, goes another way: a unit by the largest of S and b r v,
+// neither kTopS nor kTop: there two halves are good to 2^-23 of it.  w is looked at
+// in every chunk; of S a bound is carried on, and its values looked at when that
+// passes kTopS.  What leaves the range, or fp32, goes another way: a unit by the largest of S and b r v,
 // and the chunk worked out anew.  (Where these are in range and w and S still below
 // kLow, w is what is left of larger terms, and as good as they are.)
 //
@@ -1067,6 +1066,10 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 // ---------------------------------------------------------------------------
 constexpr float kTop = 32768.0f, kTopS = 16384.0f, kLow = 1.0f;
 constexpr int kAim = 127 + 4, kTopAim = 127 + 10;  // exponent bits that a new unit gives the largest
+// The first unit: the largest of a state and its first chunk's b r v are as a rule
+// 2^-5 to 2^9.  To look at them all first takes 10 us more of 338 (64 prompts of 33
+// rows at 32 heads of 128 x 128).
+constexpr float kFirst = 32.0f;
 
 // The power of two, of up to 2^-126 and 2^100, that takes a magnitude with the
 // exponent bits e up to kAim's, where there is room to grow, or down to kTopAim's,
@@ -1259,24 +1262,30 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
 #pragma unroll
       for (int w = 0; w < 4; ++w)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = __builtin_fabsf(raw_f32<T>(vr[w][i]) * write[w][i]);
-          mv = v < __builtin_inff() ? fmaxf(mv, v) : mv;
-        }
+        for (int i = 0; i < 4; ++i) mv = fmaxf(mv, __builtin_fabsf(raw_f32<T>(vr[w][i]) * write[w][i]));
+      if (__ballot(mv == __builtin_inff())) {
+        mv = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = __builtin_fabsf(raw_f32<T>(vr[w][i]) * write[w][i]);
+            mv = v < __builtin_inff() ? fmaxf(mv, v) : mv;
+          }
+      }
       mv = quads_max(mv);
       constexpr int kNone = -1000;
       int bits = max(mv > 0.0f ? exponent_bits(mv) + exponent_bits(unit) - 127 : kNone,
                      ms > 0.0f && ms < __builtin_inff() ? exponent_bits(ms) : kNone);
       off = off && bits != kNone;
-#pragma unroll
       for (int k = 0; k < 2; ++k) {  // one power of two may not reach
         const float f = off ? to_range(bits, unit) : 1.0f;
+        if (!__ballot(f != 1.0f)) break;
         rescale(f);
         bits += exponent_bits(f) - 127;
       }
     };
-    bound = largest();
-    aim(true, bound);
+    bound = __builtin_inff();
     for (int c = 0; c < chunks; ++c) {
       const int next = c + 1 < chunks ? c + 1 : c;
       const auto head1 = head_of(next), keys1 = keys_of(next);
@@ -1286,7 +1295,8 @@ __global__ __launch_bounds__(128, 1) void k_delta_scan(
       uint8_t* buf = sh[c & 1];
       if (__ballot(!(bound <= kTopS))) {
         bound = largest();
-        const float f = bound > kTopS && bound < __builtin_inff() ? to_range(exponent_bits(bound), unit) : 1.0f;
+        float f = bound > kTopS && bound < __builtin_inff() ? to_range(exponent_bits(bound), unit) : 1.0f;
+        if (c == 0 && bound <= kTopS / kFirst) f = kFirst;
         rescale(f);
       }
       // K S, and S for the other wave
