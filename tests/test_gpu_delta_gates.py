@@ -50,6 +50,17 @@ def test_small_b(hip, size, step):
         c.check(hip, "small b")
 
 
+@pytest.mark.parametrize("type_name", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("H,P,G,N", [(2, 17, 1, 100), (1, 5, 1, 7), (4, 1, 4, 1), (2, 33, 2, 256),
+                                     (2, 40, 1, 128), (1, 16, 1, 65)])
+def test_gates_nearly_shut_of_any_size(hip, type_name, H, P, G, N):
+    note("shut, %s %s" % (type_name, (H, P, G, N)))
+    c = DeltaCase(type_name, H, P, G, N, [130, 33, 20, 200], seed=N, rate=0.5)
+    c.beta.sub_(9.0)
+    c.pool_buf.mul_(2.0 ** -12)
+    c.check(hip, "shut")
+
+
 @pytest.mark.parametrize("step", [False, True])
 @pytest.mark.parametrize("size", [0, -7, -14, -20, -27, -60])
 def test_no_gate_and_a_small_state(hip, size, step):
