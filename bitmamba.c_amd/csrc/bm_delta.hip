@@ -258,17 +258,17 @@ static hipError_t launch_step_t(const DeltaArgs& a, hipStream_t s) {
 // steps are four neighbours of a row, so that the state, n = 16 x + 4 (lane / 16)
 // and on of row lane % 16, is operand and accumulator as it is loaded.
 //
-// 64 sequences of 5 rows, 32 heads of 128 x 128 in bf16, take 39 us frozen (134 MB
-// read, 3.4 TB/s) and 103 us with the states written (268 MB): two waves per SIMD
+// 64 sequences of 5 rows, 32 heads of 128 x 128 in bf16, take 41 us frozen (134 MB
+// read, 3.3 TB/s) and 103 us with the states written (268 MB): two waves per SIMD
 // load, multiply (224 products of 32 cycles for four tiles) and store in turn.
 // With keys and queries loaded before the state, and the next eight rows' during
 // these, the latter takes 5 % less, and one sequence 4 to 15 % more.
 // Row after row on the vector units they take 60 us frozen, bound by instructions.
 // ---------------------------------------------------------------------------
 typedef float v4f __attribute__((ext_vector_type(4)));
-// Sequences of up to these rows go this way.  At 32 heads of 128 x 128 in bf16: 64
-// sequences of 32 rows 279 us, in chunks 331, of 24 rows 222 and 216; two
-// sequences of 32 rows 37 and 22, of 24 rows 24 and 25.
+// Sequences of up to these rows go this way.  At 32 heads of 128 x 128 in bf16, all of
+// the call: 64 sequences of 32 rows 163 us, of 33 rows, in chunks, 338; two
+// sequences 27 and 24.
 constexpr int kShort = 32;
 constexpr int kFew = 8;
 
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(64, (NX > 8 ? 1 : 2) * (M == 1 ? 2 : 1)) void k_del
       float sq = __builtin_fmaf(seen[8 + j], all.lo, seen[8 + j] * all.hi);
 #pragma unroll
       for (int i = 0; i < j; ++i) {
-        wu[i] *= decay.hi;
+        wu[i] *= decay.hi;  // its rounding, 2^-25 of what a row wrote, at most 7 times
         sk = __builtin_fmaf(dot(j, i), wu[i], sk);
         sq = __builtin_fmaf(dot(8 + j, i), wu[i], sq);
       }
@@ -790,12 +790,12 @@ __device__ __forceinline__ float eight_f32(const Eight<T, WIDE>& e, int i) {
 // ---------------------------------------------------------------------------
 // One chunk of one head: T, A and the rows' scalars; for a group's first head
 // also K and Q as operands.  Wave w has the rows of tile w (spread_row).
-// 16384 rows at 32 heads of 128 in 16 groups take 143 us: 413 MB written, 328 MB
-// read, vector instructions on 44 % of the cycles.  Without the operands of K and Q
-// it takes 120 us, without the inverse 127, without both 98.  What it waits for are
-// its own steps: with the heads of a group on one XCD it reads 133 MB in the same
-// time, with two and with three waves per SIMD too; four (128 registers, with
-// spills) take 184 us.  A short prompt (1024 rows of fp32) takes 29 us.
+// 16384 rows at 32 heads of 128 in 16 groups take 140 us: 415 MB written, 336 MB
+// read, vector instructions on 43 % of the cycles.  An earlier form of 143 us took 120
+// without the operands of K and Q, 127 without the inverse, 98 without both.  What
+// it waits for are its own steps: with the heads of a group on one XCD it read 133 MB
+// in the same time, with two and with three waves per SIMD too; four (128 registers,
+// with spills) took 184 us.  A short prompt (1024 rows of fp32) takes 31 us.
 // ---------------------------------------------------------------------------
 template <typename T, int NK, bool WIDE>
 __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) {
@@ -1057,12 +1057,14 @@ __global__ __launch_bounds__(256) void k_delta_chunk(DeltaArgs a, DeltaPlan pl) 
 // kLow, w is what is left of larger terms, and as good as they are.)
 //
 // Bound by the steps of a chunk, each of which waits for the one before: 2.35 us
-// per chunk (603 us for 16384 rows at 32 heads of 128 x 128, on 256 blocks), of
+// per chunk (600 us for 16384 rows at 32 heads of 128 x 128, on 256 blocks), of
 // whose 5600 cycles the first wave spends 1300 on products and about as many on
-// other instructions.  With all operands in the caches it takes 546 us, without
-// the second wave 562.  Two blocks per SIMD pair do not pay: in 256 registers the
-// operands of the next chunk no longer fit ahead (713 us), and staged in LDS by a
-// third wave they take 643 us.
+// other instructions.  An earlier form of 603 us took 546 with all operands in the
+// caches and 562 without the second wave.  Two blocks per SIMD pair did not pay: in
+// 256 registers the operands of the next chunk no longer fit ahead (713 us), and
+// staged in LDS by a third wave they took 643 us.  In fp32 with more than 128 values
+// of state the operands do not fit 512 registers either: 488 of them spill, and 1024
+// rows take 576 us where 128 values take 84.
 // ---------------------------------------------------------------------------
 constexpr float kTop = 32768.0f, kTopS = 16384.0f, kLow = 1.0f;
 constexpr int kAim = 127 + 4, kTopAim = 127 + 10;  // exponent bits that a new unit gives the largest

@@ -10,8 +10,9 @@
 // greedy target needs the first two only.
 //
 // A draw falls between two neighbouring tokens of up to 256000, so every
-// error of a running sum moves draws by that much: exponentials and sums are
-// in fp64 (2^-47 of each), in an order that depends on the sizes alone.
+// error of a running sum moves draws by that much: exponentials and sums are in
+// fp64, in an order that depends on the sizes alone.  The exponential's polynomial
+// is off by 2^-46 of it, the rounding of its argument t, in bits, by |t| 2^-53 at most.
 #include <math.h>
 
 #include "bm_dev.h"

@@ -464,7 +464,10 @@ int bm_hip_ssm_step_dev(const bm_hip_ssm_t *op, void *stream);
  *
  * A key with b * (sum of k's squares) above 2 makes the rule grow without
  * end; qk_norm with b in 0..2 cannot.  Where such a growth passes fp32, the
- * head's later rows of the sequence are infinite, NaN or undefined.
+ * head's rows of the sequence from up to 15 before on are infinite, NaN or
+ * undefined.  Shorter sequences and single tokens take the sums of S[p] * k,
+ * S[p] * q and k * q, and w[p] / |k|, in fp32 before anything is divided by
+ * a length: these must not pass its range either.
  *
  * Where a head's a or b is NaN or b infinite, or the sum of k's squares is
  * either (in fp32), the head is NaN from that row on, y and state; where that
@@ -557,6 +560,7 @@ int bm_hip_slots_compact_dev(const bm_hip_slots_t *pools, int n_pools,
 /*   A target row without any p > 0 refuses, and has next_token -1 if   */
 /*   it is the one drawn from.                                          */
 /* - Sums and exponentials are in 64 bits; nothing depends on an order. */
+/* - Outputs and workspace must not overlap the inputs or each other.   */
 /* - A sequence without rows gets n_accepted 0 and next_token -1.       */
 /* - 0, -2 for arguments that do not fit (nothing is launched), -1 for  */
 /*   a HIP error; the reason is in bm_hip_last_error().                 */
