@@ -213,6 +213,10 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
 
 template <typename T, int TEAM, int V, int E>
 static hipError_t launch_step(const DeltaArgs& a, hipStream_t s) {
+  // Groups of rows per wave, with half and with twice as many: 128 sequences of 32
+  // heads of 128 take, with 8 values of state, 13.5 us against 20.4 and 10.2, with 32
+  // 26.8 (38.4, 25.8), with 64 47.6 (46.2, 48.5), with 128 94.7 (93.0, 91.8); 16
+  // sequences with 64 values 9.4 (9.1, 10.9), with 128 13.1 (12.3, 14.5).
   constexpr int U = E >= 4 ? 2 : (E == 2 ? 4 : (TEAM >= 16 ? 8 : 2));
   constexpr int kRows = 64 / TEAM * U;  // rows of the state per wave
   const int waves = (a.hd + kRows - 1) / kRows;
@@ -229,6 +233,9 @@ static hipError_t launch_step(const DeltaArgs& a, hipStream_t s) {
 
 template <typename T>
 static hipError_t launch_step_t(const DeltaArgs& a, hipStream_t s) {
+  // Other teams, for 16 and for 128 sequences as above: 64 values in 8 lanes 9.3 and
+  // 47.8 us (in 16: 9.4 and 47.6), 128 in 32 lanes 14.1 and 95.4 (13.1 and 94.7), 61
+  // values one by one in 64 lanes 12.4 and 73.5 (in 16: 9.7 and 74.2).
   if (a.n % 4 == 0) {  // a state row's loads of four floats need no more than a float's alignment
     if (a.n <= 16) return launch_step<T, 4, 4, 1>(a, s);
     if (a.n <= 32) return launch_step<T, 8, 4, 1>(a, s);
@@ -297,6 +304,8 @@ __device__ __forceinline__ void transpose_groups(float (&x)[4]) {
   swap(rows, x[2], x[3]);
 }
 
+// Two waves per SIMD, one with more than 128 values of state; twice as many of one
+// tile, where rows on no load's alignment spill 19 to 29 registers.
 template <typename T, int NX, int M, bool WIDE>
 __global__ __launch_bounds__(64, (NX > 8 ? 1 : 2) * (M == 1 ? 2 : 1)) void k_delta_few(DeltaArgs a) {
   const int b = blockIdx.x, h = blockIdx.y;
